@@ -410,6 +410,107 @@ int sdrb_visit_fill(const sdrb_batch* a, const sdrb_batch* b, int which, unsigne
                     uint32_t* this_pos, uint32_t* arg_pos, void* stream);
 
 /*
+ * Sparse rows of ids against DENSE matrices in device memory: the product of a batch with a matrix and its gradients, and
+ * the step from dense scores back to sparse rows.  The reference's products take sparse operands only (inner,
+ * row_major_mul_vec, SDR.hpp:1682-1750); these are the engine's own.
+ *
+ * Rows: a batch's (sdrb_batch_rows), or any arrays in device memory -- the tokens of a sequence are rows of one id each, the
+ * result of sdrb_winners is rows of k.  Ids need be neither ascending nor distinct here, and an id that lies outside the
+ * dense matrix contributes nothing, whatever its weight (a padded place holds -1).
+ * Matrices: row-major, any element alignment, elements of a row adjacent.  Sums are kept in binary32 (or wider) and rounded
+ * once, to the nearest, to the type of the output.  Additions have a fixed order: a call repeated with the same shapes
+ * gives the same bits.
+ * None of these calls allocates, waits for the GPU or keeps anything: they can be captured into a graph.  Scratch is the
+ * caller's (its size from sdrb_*_scratch, any 16-byte aligned device memory; NULL where the size is 0), and calls that may
+ * run at the same time need scratch of their own.  An output may not overlap an input or the scratch.
+ */
+#define SDRB_F32 0
+#define SDRB_F16 1
+#define SDRB_BF16 2
+
+typedef struct sdrb_rows {
+    uint64_t n_rows;
+    uint64_t n_elems;              /* ids in all; at most 2^32-1 */
+    const uint32_t* row_offsets;   /* device, [n_rows+1]; NULL: every row holds n_elems / n_rows ids */
+    const void* ids;               /* device, int32 or int64 [n_elems] */
+    const float* weights;          /* device, [n_elems]; NULL: all 1 */
+    int id_bits;                   /* 32 or 64 */
+} sdrb_rows;
+
+typedef struct sdrb_dense {
+    void* data;       /* device */
+    uint64_t n_rows;
+    uint64_t n_cols;  /* at most 2^24 */
+    uint64_t ld;      /* elements from one row to the next, >= n_cols */
+    int type;         /* SDRB_F32, SDRB_F16 or SDRB_BF16 */
+} sdrb_dense;
+
+/* The rows of a batch as arrays, payloads as weights (valid until the next upload / destroy).  Ids keep their width. */
+int sdrb_batch_rows(const sdrb_batch* batch, sdrb_rows* rows);
+
+/*
+ * out[r, :] = scale * sum over the ids of row r, in their order, of weight * table[id, :]  (out: n_rows x table columns).
+ * An embedding lookup where rows hold one id; a row without ids, or with none inside the table, yields zeros.
+ */
+int sdrb_lookup_scratch(const sdrb_rows* rows, uint64_t n_cols, size_t* bytes);
+int sdrb_lookup(int device, const sdrb_rows* rows, const sdrb_dense* table, float scale, const sdrb_dense* out, void* scratch,
+                size_t scratch_bytes, void* stream);
+
+/*
+ * The lookup's gradient to its table: out[v, :] = scale * sum over all elements with id v of weight * grad[row, :], where
+ * grad (n_rows x out columns) is the gradient of the lookup's result; rows of `out` that no element names become 0.
+ * accumulate != 0: the sums are added to what `out` holds, in one rounding, and rows that no element names are not touched.
+ * The elements are sorted by id on the way; those of one id are added in their order.
+ */
+int sdrb_lookup_grad_table_scratch(const sdrb_rows* rows, uint64_t n_table_rows, uint64_t n_cols, size_t* bytes);
+int sdrb_lookup_grad_table(int device, const sdrb_rows* rows, const sdrb_dense* grad, float scale, int accumulate,
+                           const sdrb_dense* out, void* scratch, size_t scratch_bytes, void* stream);
+
+/*
+ * The lookup's gradient to its weights (rows->weights plays no part): out[e] = scale * <grad[row of e, :], table[id of e, :]>,
+ * 0 for an id outside the table.  out: device, float [n_elems].
+ */
+int sdrb_lookup_grad_weights(int device, const sdrb_rows* rows, const sdrb_dense* grad, const sdrb_dense* table, float scale,
+                             float* out, void* stream);
+
+/*
+ * The k winners of every row of dense scores (rows x ids) -- experts a token is routed to, the active ids of a sparse code --
+ * as rows of k ids, ascending, with their weights; -1 and 0 in the last places of a row with fewer than k candidates.
+ *   u    softmax over the row's scores, or the sigmoid of each.  A score of -inf or NaN has no share and never wins.
+ *   key  u + bias[id], or the score where no bias is given and no keys are summed.  A key of -inf or NaN never wins.
+ *   groups > 1: ids are cut into that many equal groups; a group's score is the sum of its group_top (1 or 2) largest keys,
+ *        and only ids in the top_groups best groups can win.
+ *   The k largest keys win; equal ones go to the lowest group and the lowest id.  Keys are compared as binary64.
+ *   weight = scale * u, or with `renormalise` scale * u / (sum of the winners' u), computed so that it also holds where every
+ *        u underflows.  The bias chooses; it does not enter the weights.
+ * Limits: 1 <= k <= ids <= 16384, k <= 1024, groups <= 256.
+ */
+#define SDRB_SCORE_SOFTMAX 0
+#define SDRB_SCORE_SIGMOID 1
+
+typedef struct sdrb_winners_spec {
+    uint32_t k;
+    int score;           /* SDRB_SCORE_SOFTMAX or SDRB_SCORE_SIGMOID */
+    int renormalise;
+    uint32_t groups;     /* 1: no groups */
+    uint32_t top_groups; /* 1 .. groups */
+    uint32_t group_top;  /* 1 or 2 */
+    float scale;
+    const float* bias;   /* device, [ids], or NULL */
+} sdrb_winners_spec;
+
+int sdrb_winners(int device, const sdrb_dense* scores, const sdrb_winners_spec* spec, int32_t* out_ids, float* out_weights,
+                 void* stream);
+
+/*
+ * The gradient of the winners' weights to the scores: from `ids` (rows x k, as sdrb_winners lists them; distinct in a row) and
+ * the weights' gradient grad_weights (rows x k; places with id -1 are not read as gradients), out (rows x ids, any type) is
+ * written whole.  The choice of the ids is constant; bias, groups and top_groups of the spec play no part.
+ */
+int sdrb_winners_grad(int device, const sdrb_dense* scores, const sdrb_winners_spec* spec, const int32_t* ids,
+                      const float* grad_weights, const sdrb_dense* out, void* stream);
+
+/*
  * Device-memory helpers for callers that do not link a HIP runtime themselves (the C++
  * SDRBatch front end, ctypes/cgo/JNI bindings).  sdrb_memcpy_* synchronise.
  */

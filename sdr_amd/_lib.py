@@ -42,12 +42,30 @@ class SdrbError(RuntimeError):
         self.code = code
 
 
+class Rows(C.Structure):
+    """sdrb_rows"""
+    _fields_ = [("n_rows", C.c_uint64), ("n_elems", C.c_uint64), ("row_offsets", C.c_void_p), ("ids", C.c_void_p),
+                ("weights", C.c_void_p), ("id_bits", C.c_int)]
+
+
+class Dense(C.Structure):
+    """sdrb_dense"""
+    _fields_ = [("data", C.c_void_p), ("n_rows", C.c_uint64), ("n_cols", C.c_uint64), ("ld", C.c_uint64), ("type", C.c_int)]
+
+
+class WinnersSpec(C.Structure):
+    """sdrb_winners_spec"""
+    _fields_ = [("k", C.c_uint32), ("score", C.c_int), ("renormalise", C.c_int), ("groups", C.c_uint32), ("top_groups", C.c_uint32),
+                ("group_top", C.c_uint32), ("scale", C.c_float), ("bias", C.c_void_p)]
+
+
 # name -> (restype, argtypes); every symbol include/sdr_amd.h declares
 _u64p = C.POINTER(C.c_uint64)
 _u32p = C.POINTER(C.c_uint32)
 _i32p = C.POINTER(C.c_int32)
 _f32p = C.POINTER(C.c_float)
 _vp = C.c_void_p
+_rows, _dense, _spec, _sizep = C.POINTER(Rows), C.POINTER(Dense), C.POINTER(WinnersSpec), C.POINTER(C.c_size_t)
 PROTOTYPES = {
     "sdrb_last_error": (C.c_char_p, []),
     "sdrb_device_count": (C.c_int, [C.POINTER(C.c_int)]),
@@ -93,6 +111,14 @@ PROTOTYPES = {
     "sdrb_visit_count": (C.c_int, [_vp, _vp, C.c_int, C.c_uint, _vp, _u64p, _vp]),
     "sdrb_visit_fill": (C.c_int, [_vp, _vp, C.c_int, C.c_uint, _vp, _vp, _vp, _vp]),
     "sdrb_elem_op_fill": (C.c_int, [_vp, _vp, C.c_int, C.c_uint, _vp, _vp, _vp, _vp]),
+    "sdrb_batch_rows": (C.c_int, [_vp, _rows]),
+    "sdrb_lookup_scratch": (C.c_int, [_rows, C.c_uint64, _sizep]),
+    "sdrb_lookup": (C.c_int, [C.c_int, _rows, _dense, C.c_float, _dense, _vp, C.c_size_t, _vp]),
+    "sdrb_lookup_grad_table_scratch": (C.c_int, [_rows, C.c_uint64, C.c_uint64, _sizep]),
+    "sdrb_lookup_grad_table": (C.c_int, [C.c_int, _rows, _dense, C.c_float, C.c_int, _dense, _vp, C.c_size_t, _vp]),
+    "sdrb_lookup_grad_weights": (C.c_int, [C.c_int, _rows, _dense, _dense, C.c_float, _vp, _vp]),
+    "sdrb_winners": (C.c_int, [C.c_int, _dense, _spec, _vp, _vp, _vp]),
+    "sdrb_winners_grad": (C.c_int, [C.c_int, _dense, _spec, _vp, _vp, _dense, _vp]),
     "sdrb_malloc": (C.c_int, [C.c_int, C.c_size_t, C.POINTER(_vp)]),
     "sdrb_free": (C.c_int, [C.c_int, _vp]),
     "sdrb_memcpy_h2d": (C.c_int, [C.c_int, _vp, _vp, C.c_size_t, _vp]),

@@ -37,6 +37,14 @@ def _stream_handle(device: int, stream) -> int:
     return int(stream)
 
 
+def _torch_stream(device: int, stream):
+    """``stream`` (None: the current one) as torch knows it."""
+    torch = _torch()
+    if stream is None or hasattr(stream, "cuda_stream"):
+        return torch.cuda.current_stream(device) if stream is None else stream
+    return torch.cuda.ExternalStream(int(stream), device=device)
+
+
 def rows_to_csr(rows: Iterable, with_data: bool):
     """``rows``: iterable of id sequences, or of ``(ids, data)`` pairs when ``with_data``."""
     offsets = [0]
@@ -506,6 +514,51 @@ class SDRBatch:
         check(self._lib.sdrb_inner(self._h, other._h, flags, out.data_ptr(), out.stride(0),
                                    _stream_handle(other.device, stream)))
         return out
+
+    # -- products with dense matrices, and their gradients (dense.py) ----------------------------------------------
+    def _rows(self) -> "_lib.Rows":
+        rows = _lib.Rows()
+        check(self._lib.sdrb_batch_rows(self._h, C.byref(rows)))
+        return rows
+
+    def lookup(self, table, *, scale: float = 1.0, dtype=None, out=None, stream=None):
+        """``out[i] = scale * sum of payload * table[id]`` over the elements of row i, in id order: the rows as sparse
+        vectors times a dense matrix on their device, ``row_major_mul_vec`` (SDR.hpp:1729-1750) with a dense operand.
+        Rows without payloads count every id once.  See :func:`sdr_amd.lookup`."""
+        from . import dense
+        return dense._lookup(self._lib, self._rows(), self.device, table, scale, dtype, out, stream)
+
+    def lookup_grad_table(self, grad, n_table_rows=None, *, scale: float = 1.0, dtype=None, out=None, accumulate: bool = False,
+                          stream=None):
+        """The gradient of :meth:`lookup` to its table (``n_table_rows``: by default the batch's declared width).  See
+        :func:`sdr_amd.lookup_grad_table`."""
+        from . import dense
+        if n_table_rows is None and out is None and not self.width:
+            raise ValueError("a batch without a declared width needs n_table_rows")
+        return dense._lookup_grad_table(self._lib, self._rows(), self.device, grad, self.width if n_table_rows is None else n_table_rows,
+                                        scale, dtype, out, accumulate, stream)
+
+    def lookup_grad_data(self, grad, table, *, scale: float = 1.0, out=None, stream=None):
+        """The gradient of :meth:`lookup` to the payloads: float32 ``[nnz]``, in element order.  See
+        :func:`sdr_amd.lookup_grad_weights`."""
+        from . import dense
+        return dense._lookup_grad_weights(self._lib, self._rows(), self.device, grad, table, scale, (self.nnz,), out, stream)
+
+    @classmethod
+    def from_winners(cls, ids, weights=None, *, width: int = 0, kind=None, stream=None) -> "SDRBatch":
+        """The rows that :func:`sdr_amd.winners` chose as a batch: without the places that hold no id, with the weights as
+        payloads where they are given (``kind`` "arith" by default; "unit" for weights in [0, 1])."""
+        torch = _torch()
+        if ids.dim() != 2 or ids.dtype != torch.int32 or (weights is not None and weights.shape != ids.shape):
+            raise ValueError("ids must be int32 [rows, k], and weights have their shape")
+        device = ids.device.index
+        b = cls(device, width, kind if kind is not None else ("arith" if weights is not None else "empty"))
+        with torch.cuda.stream(_torch_stream(device, stream)):
+            there = ids >= 0
+            offsets = torch.zeros(ids.shape[0] + 1, dtype=torch.int32, device=ids.device)
+            offsets[1:] = there.sum(1).cumsum(0)
+            b.upload_device(offsets, ids[there], None if weights is None else weights[there], stream=stream)
+        return b
 
     def allpairs_topk(self, other: "SDRBatch", k: int, *, exclude_offset: int = -1, stream=None, algo=None):
         """For every row i of ``self``: the ``k`` rows j of ``other`` with the largest id overlap

@@ -1,0 +1,87 @@
+// Sparse rows of ids against dense matrices: what the kernels of lookup.hip, lookup_grad.hip and winners.hip share.
+#pragma once
+
+#include "sdrb_internal.h"
+
+namespace sdrb {
+
+// ---- element types: SDRB_F32 / SDRB_F16 / SDRB_BF16, arithmetic always in binary32 or wider ----
+using f16 = _Float16;
+using bf16 = __bf16;
+
+__device__ __forceinline__ float to_f32(float v) { return v; }
+__device__ __forceinline__ float to_f32(f16 v) { return (float)v; }
+__device__ __forceinline__ float to_f32(bf16 v) { return (float)v; }
+// round to nearest even, the one rounding of a result to its type
+template <typename T>
+__device__ __forceinline__ T from_f32(float v) {
+    return (T)v;
+}
+
+// N consecutive elements starting at any multiple of the element's own size (the unaligned access mode of the target
+// makes these single wide loads and stores)
+template <int N, typename T>
+__device__ __forceinline__ void load_n(const T* p, float (&v)[N]) {
+    T t[N];
+    __builtin_memcpy(t, p, sizeof t);
+#pragma unroll
+    for (int k = 0; k < N; ++k) v[k] = to_f32(t[k]);
+}
+template <int N, typename T>
+__device__ __forceinline__ void store_n(T* p, const float (&v)[N]) {
+    T t[N];
+#pragma unroll
+    for (int k = 0; k < N; ++k) t[k] = from_f32<T>(v[k]);
+    __builtin_memcpy(p, t, sizeof t);
+}
+
+// Calls f(T{}) with the element type named by `type` (checked by the caller).
+template <typename F>
+int with_type(int type, F&& f) {
+    switch (type) {
+        case SDRB_F16: return f(f16{});
+        case SDRB_BF16: return f(bf16{});
+        default: return f(float{});
+    }
+}
+inline size_t type_size(int type) { return type == SDRB_F32 ? 4 : 2; }
+
+// A ragged sum: out[s, :] (+)= scale * sum over p in [start[s], start[s+1]) of weight[p] * src[index[p], :].
+// lookup.hip runs it over a batch's rows, lookup_grad.hip over the elements sorted by id.
+struct GatherSum {
+    int device;
+    uint64_t n_segments;
+    uint64_t n_elems;
+    const uint32_t* start;     // [n_segments + 1], or null: every segment holds n_elems / n_segments elements
+    const void* index;         // [n_elems]
+    int index_bits;            // 32 or 64; an index outside [0, src_rows) contributes nothing
+    const float* weight;       // [n_elems] or null: 1
+    const void* src;
+    int src_type;
+    uint64_t src_rows, src_ld;
+    uint32_t dim;
+    void* out;
+    int out_type;
+    uint64_t out_ld;
+    float scale;
+    bool accumulate;           // segments without elements are then left as they are
+    float* partials;           // gather_partial_bytes(...) of scratch, null where none is needed
+};
+// Scratch for the sums of segments too long for one group of lanes: 0 when no segment can be that long.
+size_t gather_partial_bytes(uint64_t n_segments, uint64_t n_elems, bool ragged, uint32_t dim);
+int launch_gather_sum(const GatherSum& g, hipStream_t stream);
+
+// lookup_grad.hip
+size_t table_grad_scratch_bytes(uint64_t n_elems, uint64_t n_table_rows, uint32_t dim);
+int launch_table_grad(int device, const sdrb_rows& rows, const sdrb_dense& grad, float scale, bool accumulate,
+                      const sdrb_dense& out, void* scratch, hipStream_t stream);
+int launch_weight_grad(const sdrb_rows& rows, const sdrb_dense& grad, const sdrb_dense& table, float scale, float* out,
+                       hipStream_t stream);
+
+// winners.hip
+constexpr uint32_t kWinnersMaxIds = 16384, kWinnersMaxK = 1024, kWinnersMaxGroups = 256;
+int launch_winners(const sdrb_dense& scores, const sdrb_winners_spec& spec, int32_t* ids, float* weights, hipStream_t stream);
+int launch_winners_grad(const sdrb_dense& scores, const sdrb_winners_spec& spec, const int32_t* ids, const float* grad_weights,
+                        const sdrb_dense& out, hipStream_t stream);
+
+}  // namespace sdrb

@@ -1,0 +1,213 @@
+"""Sparse rows of ids against dense matrices: lookups, their gradients, and the winners of dense scores.
+
+Rows are given as tensors: ``ids`` [n] -- one id a row (the tokens of a sequence), ``ids`` [n, k] -- k ids a row (the result of
+:func:`winners`), or ``ids`` [elements] with ``offsets`` [n + 1] -- ragged rows; the same operators are methods of
+:class:`~sdr_amd.SDRBatch` for rows that a batch holds.  Ids are int32 or int64 and need be neither ascending nor distinct; an
+id outside the dense matrix (a padded place holds -1) contributes nothing.  ``weights`` are float32, one an id.
+
+Matrices are float32, float16 or bfloat16, with adjacent elements in a row and any row stride.  Sums are kept in binary32 and
+rounded once to the output's type, in an order that the shapes and offsets fix: calls repeat bit for bit.
+
+Everything is enqueued on ``stream`` (a torch stream or a handle; the current stream of the tensors' device by default), outputs
+and scratch are allocated on that stream, and nothing waits for the GPU, so the calls can be captured into a graph.  All
+computation happens in ``libsdr_amd.so``; torch is used only to allocate and to name streams.
+"""
+from __future__ import annotations
+
+import ctypes as C
+
+from . import _lib
+from ._lib import Dense, Rows, WinnersSpec, check
+from .batch import _torch_stream
+
+_SCORES = {"softmax": 0, "sigmoid": 1}
+_types = {}
+
+
+def _torch():
+    import torch  # plumbing only: device buffers and streams
+    if not _types:
+        _types.update({torch.float32: 0, torch.float16: 1, torch.bfloat16: 2})
+    return torch
+
+
+def _device_of(t) -> int:
+    if not t.is_cuda:
+        raise ValueError("tensors must be on a GPU")
+    return t.device.index
+
+
+def _matrix(name, t, device) -> Dense:
+    if t.dim() != 2 or t.dtype not in _types:
+        raise ValueError(f"{name} must be a 2-d float32, float16 or bfloat16 tensor")
+    if not t.is_cuda or t.device.index != device:
+        raise ValueError(f"{name} must be on cuda:{device} like the other tensors")
+    n, m = t.shape
+    ld = t.stride(0) if n > 1 else m
+    if (m > 1 and t.stride(1) != 1) or ld < m:
+        raise ValueError(f"{name} must have adjacent elements in a row and rows that do not overlap (call .contiguous())")
+    return Dense(t.data_ptr(), n, m, ld, _types[t.dtype])
+
+
+def _vector(name, t, dtype, device, shape=None):
+    if t.dtype != dtype or not t.is_contiguous() or (shape is not None and t.shape != shape):
+        raise ValueError(f"{name} must be a contiguous {dtype} tensor" + ("" if shape is None else f" of shape {tuple(shape)}"))
+    if not t.is_cuda or t.device.index != device:
+        raise ValueError(f"{name} must be on cuda:{device} like the other tensors")
+    return t.data_ptr()
+
+
+def _rows(torch, ids, weights, offsets) -> Rows:
+    device = _device_of(ids)
+    if ids.dtype not in (torch.int32, torch.int64) or not ids.is_contiguous() or ids.dim() not in (1, 2):
+        raise ValueError("ids must be a contiguous 1-d or 2-d int32 or int64 tensor")
+    off = None
+    if offsets is not None:
+        if ids.dim() != 1 or offsets.dim() != 1 or offsets.numel() < 1:
+            raise ValueError("offsets ([rows + 1]) go with 1-d ids")
+        off = _vector("offsets", offsets, torch.int32, device)
+        n = offsets.numel() - 1
+    else:
+        n = ids.shape[0]
+    w = None if weights is None else _vector("weights", weights, torch.float32, device, ids.shape)
+    return Rows(n, ids.numel(), off, ids.data_ptr(), w, 64 if ids.dtype == torch.int64 else 32)
+
+
+def _empty(torch, shape, dtype, device, stream):
+    if stream is None:
+        return torch.empty(shape, dtype=dtype, device=torch.device("cuda", device))
+    with torch.cuda.stream(_torch_stream(device, stream)):   # memory that this stream may write at once
+        return torch.empty(shape, dtype=dtype, device=torch.device("cuda", device))
+
+
+def _output(torch, out, shape, dtype, device, stream):
+    if out is None:
+        return _empty(torch, shape, dtype, device, stream)
+    if tuple(out.shape) != tuple(shape) or (dtype is not None and out.dtype != dtype):
+        raise ValueError(f"out must have shape {tuple(shape)}" + ("" if dtype is None else f" and type {dtype}"))
+    return out
+
+
+def _scratch(torch, size, device, stream):
+    return (None, 0, None) if size == 0 else (t := _empty(torch, size, torch.uint8, device, stream), size, t.data_ptr())
+
+
+def _handle(torch, device, stream) -> int:
+    return (torch.cuda.current_stream(device) if stream is None else _torch_stream(device, stream)).cuda_stream
+
+
+def _lookup(lib, rows, device, table, scale, dtype, out, stream):
+    torch = _torch()
+    t = _matrix("table", table, device)
+    out = _output(torch, out, (rows.n_rows, t.n_cols), dtype if out is not None else dtype or table.dtype, device, stream)
+    need = C.c_size_t()
+    check(lib.sdrb_lookup_scratch(C.byref(rows), t.n_cols, C.byref(need)))
+    keep, size, at = _scratch(torch, need.value, device, stream)
+    o = _matrix("out", out, device)
+    check(lib.sdrb_lookup(device, C.byref(rows), C.byref(t), scale, C.byref(o), at, size, _handle(torch, device, stream)))
+    return out
+
+
+def _lookup_grad_table(lib, rows, device, grad, n_table_rows, scale, dtype, out, accumulate, stream):
+    torch = _torch()
+    g = _matrix("grad", grad, device)
+    if accumulate and out is None:
+        raise ValueError("accumulate needs the tensor to add to as out")
+    if n_table_rows is None:
+        n_table_rows = out.shape[0]
+    if n_table_rows < 0:
+        raise ValueError("n_table_rows must not be negative")
+    out = _output(torch, out, (n_table_rows, g.n_cols), dtype if out is not None else dtype or torch.float32, device, stream)
+    o = _matrix("out", out, device)
+    need = C.c_size_t()
+    check(lib.sdrb_lookup_grad_table_scratch(C.byref(rows), n_table_rows, g.n_cols, C.byref(need)))
+    keep, size, at = _scratch(torch, need.value, device, stream)
+    check(lib.sdrb_lookup_grad_table(device, C.byref(rows), C.byref(g), scale, int(accumulate), C.byref(o), at, size,
+                                     _handle(torch, device, stream)))
+    return out
+
+
+def _lookup_grad_weights(lib, rows, device, grad, table, scale, shape, out, stream):
+    torch = _torch()
+    g, t = _matrix("grad", grad, device), _matrix("table", table, device)
+    out = _output(torch, out, shape, torch.float32, device, stream)
+    check(lib.sdrb_lookup_grad_weights(device, C.byref(rows), C.byref(g), C.byref(t), scale,
+                                       _vector("out", out, torch.float32, device), _handle(torch, device, stream)))
+    return out
+
+
+def lookup(ids, table, weights=None, *, offsets=None, scale: float = 1.0, dtype=None, out=None, stream=None):
+    """``out[r] = scale * sum of weight * table[id]`` over the ids of row r, in their order: [rows, table columns], of the
+    table's type unless ``dtype`` (or ``out``) says otherwise.  An embedding lookup where rows hold one id; a row without
+    ids, or with none inside the table, yields zeros."""
+    rows = _rows(_torch(), ids, weights, offsets)
+    return _lookup(_lib.load(), rows, ids.device.index, table, scale, dtype, out, stream)
+
+
+def lookup_grad_table(ids, grad, n_table_rows=None, weights=None, *, offsets=None, scale: float = 1.0, dtype=None, out=None,
+                      accumulate: bool = False, stream=None):
+    """The gradient of :func:`lookup` to its table, from the gradient ``grad`` [rows, columns] of its result:
+    ``out[v] = scale * sum over the elements with id v of weight * grad[their row]``, [n_table_rows, columns], float32 unless
+    ``dtype`` (or ``out``) says otherwise; zeros where no row names v.  ``accumulate``: the sums are added to ``out``, and its rows
+    that no id names are not touched.  The elements are sorted by id on the way; no atomic addition is used."""
+    rows = _rows(_torch(), ids, weights, offsets)
+    if n_table_rows is None and out is None:
+        raise ValueError("give n_table_rows or out")
+    return _lookup_grad_table(_lib.load(), rows, ids.device.index, grad, n_table_rows, scale, dtype, out, accumulate, stream)
+
+
+def lookup_grad_weights(ids, grad, table, *, offsets=None, scale: float = 1.0, out=None, stream=None):
+    """The gradient of :func:`lookup` to its weights: ``scale * <grad[row], table[id]>`` an id, float32 in the shape of
+    ``ids``; 0 for an id outside the table."""
+    rows = _rows(_torch(), ids, None, offsets)
+    return _lookup_grad_weights(_lib.load(), rows, ids.device.index, grad, table, scale, ids.shape, out, stream)
+
+
+def _spec(torch, k, score, renormalise, scale, device, bias=None, groups=1, top_groups=None, group_top=1, n_ids=0) -> WinnersSpec:
+    if score not in _SCORES:
+        raise ValueError("score must be 'softmax' or 'sigmoid'")
+    if min(groups, group_top, 1 if top_groups is None else top_groups) < 1:
+        raise ValueError("groups, top_groups and group_top must be positive")
+    b = None if bias is None else _vector("bias", bias, torch.float32, device, torch.Size((n_ids,)))
+    return WinnersSpec(k, _SCORES[score], int(renormalise), groups, groups if top_groups is None else top_groups, group_top, scale, b)
+
+
+def winners(scores, k: int, *, score: str = "softmax", bias=None, groups: int = 1, top_groups=None, group_top: int = 1,
+            renormalise: bool = False, scale: float = 1.0, stream=None):
+    """The ``k`` winning ids of every row of ``scores`` [rows, ids], ascending, and their weights: ``(ids, weights)``, int32 and
+    float32 [rows, k], -1 and 0 in the last places of a row with fewer candidates.  Routing of tokens to experts, or dense
+    activations made into sparse codes (:meth:`SDRBatch.from_winners`).
+
+    An id's share is the ``score`` -- "softmax" over the row, or "sigmoid" -- and its key the share plus ``bias`` (float32 [ids],
+    which balances the choice and does not enter the weights).  With ``groups`` > 1 only ids of the ``top_groups`` groups win
+    whose ``group_top`` (1 or 2) largest keys have the largest sums.  The largest keys win, equal ones by the lowest id; scores
+    of -inf or NaN never do.  Weights are ``scale`` times the shares, or with ``renormalise`` the shares' parts of their sum."""
+    torch = _torch()
+    device = _device_of(scores)
+    s = _matrix("scores", scores, device)
+    if not 1 <= k <= s.n_cols:
+        raise ValueError("k must be 1 .. ids")
+    spec = _spec(torch, k, score, renormalise, scale, device, bias, groups, top_groups, group_top, s.n_cols)
+    ids = _empty(torch, (s.n_rows, k), torch.int32, device, stream)
+    weights = _empty(torch, (s.n_rows, k), torch.float32, device, stream)
+    check(_lib.load().sdrb_winners(device, C.byref(s), C.byref(spec), ids.data_ptr(), weights.data_ptr(), _handle(torch, device, stream)))
+    return ids, weights
+
+
+def winners_grad(scores, ids, grad_weights, *, score: str = "softmax", renormalise: bool = False, scale: float = 1.0, dtype=None,
+                 out=None, stream=None):
+    """The gradient of :func:`winners`' weights to ``scores``: [rows, ids], of the scores' type unless ``dtype`` (or ``out``) says
+    otherwise, from the ``ids`` [rows, k] it chose (distinct in a row; their choice is constant) and the gradient ``grad_weights``
+    of the weights.  ``score``, ``renormalise`` and ``scale`` as in the forward call; a bias and groups have no part in it."""
+    torch = _torch()
+    device = _device_of(scores)
+    s = _matrix("scores", scores, device)
+    if ids.dim() != 2 or ids.shape[0] != s.n_rows:
+        raise ValueError("ids must be [rows, k]")
+    i = _vector("ids", ids, torch.int32, device)
+    g = _vector("grad_weights", grad_weights, torch.float32, device, ids.shape)
+    spec = _spec(torch, ids.shape[1], score, renormalise, scale, device)
+    out = _output(torch, out, (s.n_rows, s.n_cols), dtype if out is not None else dtype or scores.dtype, device, stream)
+    o = _matrix("out", out, device)
+    check(_lib.load().sdrb_winners_grad(device, C.byref(s), C.byref(spec), i, g, C.byref(o), _handle(torch, device, stream)))
+    return out
