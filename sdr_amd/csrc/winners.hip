@@ -2,256 +2,687 @@
 //
 // Shares: u = softmax of a row's live scores, or their sigmoids; a score of -inf or NaN is not live.  Keys: u + bias, or the
 // scores where nothing is added to the shares (the same order).  A group's score is the sum of its one or two largest
-// keys; the k largest keys inside the best groups win, ties go to the lowest group and id.  Keys are compared in binary64:
-// whether an id wins hangs on the difference of two of them, which binary32 exponentials would decide by their own error.
+// keys; the k largest keys inside the best groups win, ties go to the lowest group and id.
 // Weights: scale * u, or, renormalised, scale * p with p = u / sum of the winners' u -- a softmax over the winners of
 // l = s (softmax) or l = log sigmoid(s), which holds where every u underflows.
+//
+// A wave owns a row and holds its keys in registers, R a lane, read once; rows of more than 2048 ids are shared by eight
+// waves.  The k-th largest key is found by bisection over the keys' order-preserving integers: a step is a compare and a
+// population count a register, whatever k is, and it ends as soon as exactly k keys lie at or above the middle.  The
+// bisection starts between the smallest of the lanes' largest keys (for k up to the number of lanes at least k keys lie at
+// or above it) and the largest key, so that it takes six to twelve steps on scores without ties.
+// Shares that enter keys are computed in binary64: whether an id wins hangs on the difference of two keys, which binary32
+// exponentials would decide by their own error.  The hardware does binary64 arithmetic at the rate of binary32.
+// Bound: instruction issue, not memory.
 #include "dense_rows.h"
 
 namespace sdrb {
 
 namespace {
 
-constexpr uint32_t kThreads = 256;
-
-__device__ __forceinline__ bool live_score(float s) { return s > -INFINITY; }
-__device__ __forceinline__ double sigmoid(double x) { return 1.0 / (1.0 + exp(-x)); }
-// x - m for an exponential whose largest argument is m: infinities of the same sign differ by nothing
-__device__ __forceinline__ double below(double x, double m) { return x == m ? 0.0 : x - m; }
-__device__ __forceinline__ double logit(double x, bool sig) { return sig ? fmin(x, 0.0) - log1p(exp(-fabs(x))) : x; }
-
-template <typename F>
-__device__ __forceinline__ double block_reduce(double v, double* shared, F op) {
-#pragma unroll
-    for (int s = 32; s >= 1; s >>= 1) v = op(v, __shfl_xor(v, s, 64));
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) shared[threadIdx.x >> 6] = v;
-    __syncthreads();
-    v = shared[0];
-    for (uint32_t k = 1; k < kThreads / 64; ++k) v = op(v, shared[k]);
-    return v;
+// ---- a wave's reductions, by data-parallel moves: 6 steps without LDS ----
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int dpp(int other, int v) {
+    return __builtin_amdgcn_update_dpp(other, v, CTRL, ROWS, 0xF, false);
 }
-__device__ __forceinline__ double block_max(double v, double* shared) {
-    return block_reduce(v, shared, [](double a, double b) { return a > b ? a : b; });
+template <int CTRL, int ROWS>
+__device__ __forceinline__ float dpp(float other, float v) {
+    return __builtin_bit_cast(float, dpp<CTRL, ROWS>(__builtin_bit_cast(int, other), __builtin_bit_cast(int, v)));
 }
-__device__ __forceinline__ double block_sum(double v, double* shared) {
-    return block_reduce(v, shared, [](double a, double b) { return a + b; });
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double dpp(double other, double v) {
+    const long long o = __builtin_bit_cast(long long, other), x = __builtin_bit_cast(long long, v);
+    const uint32_t lo = (uint32_t)dpp<CTRL, ROWS>((int)o, (int)x), hi = (uint32_t)dpp<CTRL, ROWS>((int)(o >> 32), (int)(x >> 32));
+    return __builtin_bit_cast(double, (long long)(((uint64_t)hi << 32) | lo));
 }
-
-// the position of the largest key, the lowest of equal ones; every key must be > -inf to count
-__device__ __forceinline__ int block_best(const double* key, uint32_t n, double* shared_v, int* shared_i) {
-    double best = -INFINITY;
-    int at = -1;
-    for (uint32_t e = threadIdx.x; e < n; e += kThreads)
-        if (key[e] > best) {
-            best = key[e];
-            at = (int)e;
-        }
-#pragma unroll
-    for (int s = 32; s >= 1; s >>= 1) {
-        const double v = __shfl_xor(best, s, 64);
-        const int i = __shfl_xor(at, s, 64);
-        if (i >= 0 && (v > best || (v == best && (at < 0 || i < at)))) {
-            best = v;
-            at = i;
-        }
-    }
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) {
-        shared_v[threadIdx.x >> 6] = best;
-        shared_i[threadIdx.x >> 6] = at;
-    }
-    __syncthreads();
-    best = shared_v[0];
-    at = shared_i[0];
-    for (uint32_t k = 1; k < kThreads / 64; ++k)
-        if (shared_i[k] >= 0 && (shared_v[k] > best || (shared_v[k] == best && (at < 0 || shared_i[k] < at)))) {
-            best = shared_v[k];
-            at = shared_i[k];
-        }
-    __syncthreads();
-    return at;
+__device__ __forceinline__ int last_lane(int v) { return __builtin_amdgcn_readlane(v, 63); }
+__device__ __forceinline__ float last_lane(float v) { return __builtin_bit_cast(float, last_lane(__builtin_bit_cast(int, v))); }
+__device__ __forceinline__ double last_lane(double v) {
+    const long long x = __builtin_bit_cast(long long, v);
+    const uint32_t lo = (uint32_t)last_lane((int)x), hi = (uint32_t)last_lane((int)(x >> 32));
+    return __builtin_bit_cast(double, (long long)(((uint64_t)hi << 32) | lo));
 }
-
+// `none` leaves every value as it is under op; the result is uniform
+template <typename T, typename F>
+__device__ __forceinline__ T wave_reduce(T v, T none, F op) {
+    v = op(v, dpp<0xB1, 0xF>(v, v));        // lanes 1 0 3 2
+    v = op(v, dpp<0x4E, 0xF>(v, v));        // lanes 2 3 0 1
+    v = op(v, dpp<0x141, 0xF>(v, v));       // the other half of 8
+    v = op(v, dpp<0x140, 0xF>(v, v));       // the other half of 16
+    v = op(v, dpp<0x142, 0xA>(none, v));    // lane 15 of the row of 16 below, into rows 1 and 3
+    v = op(v, dpp<0x143, 0xC>(none, v));    // lane 31, into rows 2 and 3
+    return last_lane(v);
+}
 template <typename T>
-__global__ __launch_bounds__(kThreads) void k_winners(const T* __restrict__ scores, uint64_t ld, uint32_t n_ids, sdrb_winners_spec w,
-                                                      int32_t* __restrict__ out_ids, float* __restrict__ out_weights) {
-    extern __shared__ double key[];   // [n_ids], then the groups' [groups]
-    __shared__ double sv[4];
-    __shared__ int si[4];
-    __shared__ uint32_t won[kWinnersMaxIds / 32];
-    double* group = key + n_ids;
-    const uint64_t row = blockIdx.x;
-    const T* s = scores + row * ld;
-    const bool sig = w.score == SDRB_SCORE_SIGMOID;
-    const bool shares = w.bias || (w.groups > 1 && w.group_top > 1);
-    double top = -INFINITY, sum = 1.0;
-    if (!sig) {
-        for (uint32_t e = threadIdx.x; e < n_ids; e += kThreads) top = fmax(top, (double)to_f32(s[e]));   // (a NaN is passed over)
-        top = block_max(top, sv);
-        sum = 0.0;
-        for (uint32_t e = threadIdx.x; e < n_ids; e += kThreads)
-            if (live_score(to_f32(s[e]))) sum += exp(below(to_f32(s[e]), top));
-        sum = block_sum(sum, sv);
-    }
-    const auto share = [&](double x) { return sig ? sigmoid(x) : exp(below(x, top)) / sum; };
-    for (uint32_t e = threadIdx.x; e < n_ids; e += kThreads) {
-        const float x = to_f32(s[e]);
-        double k = -INFINITY;
-        if (live_score(x)) k = shares ? share(x) + (w.bias ? (double)w.bias[e] : 0.0) : (double)x;
-        key[e] = k > -INFINITY ? k : -INFINITY;
-    }
-    for (uint32_t i = threadIdx.x; i < (n_ids + 31) / 32; i += kThreads) won[i] = 0;
-    __syncthreads();
-    if (w.groups > 1) {
-        const uint32_t size = n_ids / w.groups;
-        for (uint32_t g = threadIdx.x; g < w.groups; g += kThreads) {
-            double a = -INFINITY, b = -INFINITY;
-            for (uint32_t e = g * size; e < (g + 1) * size; ++e) {
-                const double k = key[e];
-                b = k > a ? a : (k > b ? k : b);
-                a = k > a ? k : a;
-            }
-            group[g] = w.group_top > 1 && b > -INFINITY ? a + b : a;
+__device__ __forceinline__ T max_of(T a, T b) {
+    return a > b ? a : b;
+}
+
+// ---- the waves of a row: WAVES == 1, or 8 that meet in LDS ----
+template <int WAVES>
+struct Meet {
+    double* slot;   // [2][WAVES] where WAVES > 1
+    uint32_t turn;
+
+    template <typename T, typename F>
+    __device__ __forceinline__ T all(T v, F op) {   // v: uniform in the wave
+        if constexpr (WAVES == 1) {
+            return v;
+        } else {
+            double* s = slot + (turn++ & 1) * WAVES;   // the turn before may still be read while this one is written
+            if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = (double)v;
+            __syncthreads();
+            T r = (T)s[0];
+#pragma unroll
+            for (int k = 1; k < WAVES; ++k) r = op(r, (T)s[k]);
+            return r;
         }
-        __syncthreads();
-        for (uint32_t t = 0; t < w.top_groups; ++t) {   // the best groups are marked by -inf
-            const int g = block_best(group, w.groups, sv, si);
-            if (g < 0) break;
-            if (threadIdx.x == 0) {
-                group[g] = -INFINITY;
-                won[g >> 5] |= 1u << (g & 31);
+    }
+    template <typename T>
+    __device__ __forceinline__ T sum(T v) {
+        return all(wave_reduce(v, T(0), [](T a, T b) { return a + b; }), [](T a, T b) { return a + b; });
+    }
+    template <typename T>
+    __device__ __forceinline__ T max(T v) {
+        return all(wave_reduce(v, (T)-INFINITY, max_of<T>), max_of<T>);
+    }
+    __device__ __forceinline__ uint32_t total(uint32_t uniform) {
+        return all(uniform, [](uint32_t a, uint32_t b) { return a + b; });
+    }
+};
+
+// ---- keys as integers of the same order ----
+template <typename K>
+struct Ordered;
+template <>
+struct Ordered<float> {
+    using U = uint32_t;
+    static constexpr U kSign = 0x80000000u;
+};
+template <>
+struct Ordered<double> {
+    using U = uint64_t;
+    static constexpr U kSign = 0x8000000000000000ull;
+};
+template <typename K>
+__device__ __forceinline__ typename Ordered<K>::U order_of(K key) {
+    using U = typename Ordered<K>::U;
+    const U u = __builtin_bit_cast(U, key);
+    return u & Ordered<K>::kSign ? ~u : u | Ordered<K>::kSign;
+}
+template <typename K>
+__device__ __forceinline__ K key_at(typename Ordered<K>::U order) {
+    using U = typename Ordered<K>::U;
+    return __builtin_bit_cast(K, order & Ordered<K>::kSign ? (U)(order & ~Ordered<K>::kSign) : (U)~order);
+}
+
+// Where a lane's register r stands in the row: registers are read C at a time, 64 lanes side by side.
+template <int R, int WAVES>
+struct Layout {
+    static constexpr int C = R < 4 ? R : 4;
+    static constexpr int kIds = 64 * R * WAVES;
+    __device__ __forceinline__ static uint32_t id(int r) {
+        const uint32_t thread = threadIdx.x & (64 * WAVES - 1);
+        return ((uint32_t)(r / C) * (64 * WAVES) + thread) * C + r % C;
+    }
+};
+
+// The row's values, `fill` beyond its end.
+template <int R, int WAVES, typename T>
+__device__ __forceinline__ void read_row(const T* __restrict__ row, uint32_t n, float fill, float (&v)[R]) {
+    using L = Layout<R, WAVES>;
+#pragma unroll
+    for (int q = 0; q < R / L::C; ++q) {
+        const uint32_t first = L::id(q * L::C);
+        float part[L::C];
+        if (first + L::C <= n) {
+            load_n<L::C>(row + first, part);
+        } else {
+#pragma unroll
+            for (int j = 0; j < L::C; ++j) part[j] = first + j < n ? to_f32(row[first + j]) : fill;
+        }
+#pragma unroll
+        for (int j = 0; j < L::C; ++j) v[q * L::C + j] = part[j];
+    }
+}
+
+// Selects the k largest keys > -inf, the lowest places first among equal ones: won has bit r for register r.
+// Places ascend with the chunk r / C, then the thread, then r % C.  Returns how many were selected.
+template <int R, int C, int WAVES, typename K>
+__device__ __forceinline__ uint32_t select_largest(const K (&key)[R], uint32_t k, Meet<WAVES>& meet, uint32_t& won) {
+    using U = typename Ordered<K>::U;
+    const auto count = [&](K least) {
+        uint32_t c = 0;
+#pragma unroll
+        for (int r = 0; r < R; ++r) c += (uint32_t)__builtin_popcountll(__builtin_amdgcn_ballot_w64(key[r] >= least));
+        return meet.total(c);
+    };
+    K top = key[0];
+#pragma unroll
+    for (int r = 1; r < R; ++r) top = max_of(top, key[r]);
+    const K largest = meet.max(top);
+    won = 0;
+    uint32_t live = 0;
+#pragma unroll
+    for (int r = 0; r < R; ++r) live += (uint32_t)__builtin_popcountll(__builtin_amdgcn_ballot_w64(key[r] > (K)-INFINITY));
+    live = meet.total(live);
+    if (live <= k) {
+#pragma unroll
+        for (int r = 0; r < R; ++r) won |= key[r] > (K)-INFINITY ? 1u << r : 0u;
+        return live;
+    }
+    U lo = order_of((K)-INFINITY), hi = order_of(largest) + 1;   // at least k keys are >= lo, fewer than k >= hi
+    if (k <= 64 * WAVES) lo = order_of(-meet.max(-top));
+    bool exact = false;
+    while (hi - lo > 1) {
+        const U mid = lo + (hi - lo) / 2;
+        const uint32_t c = count(key_at<K>(mid));
+        if (c >= k) lo = mid;
+        else hi = mid;
+        if (c == k) {
+            exact = true;
+            break;
+        }
+    }
+    const K least = key_at<K>(lo);
+#pragma unroll
+    for (int r = 0; r < R; ++r) won |= key[r] >= least ? 1u << r : 0u;
+    if (exact) return k;
+    // `least` is a key: what lies above it wins, and the first of those equal to it
+    uint32_t above = 0;
+#pragma unroll
+    for (int r = 0; r < R; ++r) above += (uint32_t)__builtin_popcountll(__builtin_amdgcn_ballot_w64(key[r] > least));
+    uint32_t room = k - meet.total(above);
+    const uint32_t lane = threadIdx.x & 63, wave = WAVES > 1 ? threadIdx.x >> 6 : 0;
+#pragma unroll
+    for (int q = 0; q < R / C; ++q) {
+        uint32_t before = 0, here = 0;   // equal keys of this chunk: in the lanes below, and in the wave
+#pragma unroll
+        for (int j = 0; j < C; ++j) {
+            const unsigned long long eq = __builtin_amdgcn_ballot_w64(key[q * C + j] == least);
+            before += (uint32_t)__builtin_popcountll(eq & ((1ull << lane) - 1ull));
+            here += (uint32_t)__builtin_popcountll(eq);
+        }
+        if constexpr (WAVES > 1) {
+            double* s = meet.slot + (meet.turn++ & 1) * WAVES;
+            if (lane == 0) s[wave] = (double)here;
+            __syncthreads();
+            here = 0;
+#pragma unroll
+            for (int w = 0; w < WAVES; ++w) {
+                before += (uint32_t)w < wave ? (uint32_t)s[w] : 0u;
+                here += (uint32_t)s[w];
             }
+        }
+#pragma unroll
+        for (int j = 0; j < C; ++j)
+            if (key[q * C + j] == least) {
+                if (before >= room) won &= ~(1u << (q * C + j));
+                ++before;
+            }
+        room -= here < room ? here : room;
+    }
+    return k;
+}
+
+// v_exp_f32 and v_rcp_f32 are within a step of their value; arguments are rounded once more on the way to base 2
+__device__ __forceinline__ float exp_fast(float x) { return __builtin_amdgcn_exp2f(x * 1.44269504088896341f); }
+__device__ __forceinline__ float rcp_fast(float x) { return __builtin_amdgcn_rcpf(x); }
+// x - m for an exponential whose largest argument is m: infinities of the same sign differ by nothing
+template <typename K>
+__device__ __forceinline__ K below(K x, K m) {
+    return x == m ? (K)0 : x - m;
+}
+__device__ __forceinline__ float sigmoid(float x) { return rcp_fast(1.0f + exp_fast(-x)); }
+__device__ __forceinline__ double sigmoid(double x) { return 1.0 / (1.0 + exp(-x)); }
+// sigmoid(x) e^-c, c <= 0 no smaller than any x that is negative: ratios of sigmoids that would all underflow
+__device__ __forceinline__ float sigmoid_over(float x, float c) {
+    const float t = rcp_fast(1.0f + exp_fast(-fabsf(x)));
+    return x < 0.0f ? exp_fast(below(x, c)) * t : t;
+}
+
+struct WinnersArgs {
+    sdrb_winners_spec w;
+    uint64_t n_rows, ld;
+    uint32_t n_ids;
+    uint32_t group_size, group_lanes_log2;   // ids of a group; lanes that look at one group together
+    uint32_t lds_row;                        // bytes of dynamic LDS a row has
+};
+
+// K: float, keys are the scores; double, keys are shares (+ bias)
+template <int R, int WAVES, typename K, typename T>
+__global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) void k_winners(WinnersArgs a, const T* __restrict__ scores,
+                                                                           int32_t* __restrict__ out_ids,
+                                                                           float* __restrict__ out_weights) {
+    using L = Layout<R, WAVES>;
+    constexpr int C = L::C;
+    extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
+    __shared__ double slots[2 * WAVES];
+    __shared__ uint32_t starts[WAVES == 1 ? 1 : WAVES * (R / C)];
+    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const uint64_t row = WAVES == 1 ? (uint64_t)blockIdx.x * 4 + wave : blockIdx.x;
+    if (row >= a.n_rows) return;
+    unsigned char* mine = lds + (WAVES == 1 ? wave * a.lds_row : 0u);
+    Meet<WAVES> meet{slots, 0};
+    const auto sync = [] {   // LDS written by this row's waves before, read after
+        if constexpr (WAVES == 1) {
+            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+            __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+        } else {
             __syncthreads();
         }
-        for (uint32_t e = threadIdx.x; e < n_ids; e += kThreads)
-            if (!(won[(e / size) >> 5] >> ((e / size) & 31) & 1u)) key[e] = -INFINITY;
+    };
+    const T* s_row = scores + row * a.ld;
+    const sdrb_winners_spec& w = a.w;
+    const bool sig = w.score == SDRB_SCORE_SIGMOID;
+
+    float s[R];
+    read_row<R, WAVES>(s_row, a.n_ids, -INFINITY, s);
+#pragma unroll
+    for (int r = 0; r < R; ++r) s[r] = s[r] > -INFINITY ? s[r] + 0.0f : -INFINITY;   // NaN is no score; -0 is 0
+
+    // keys; top and inv_sum of a softmax over the row where one is needed
+    float top = 0.0f, inv_sum = 0.0f;
+    const bool over_row = !sig && (sizeof(K) == 8 || !w.renormalise);
+    if (over_row) {
+        float m = s[0];
+#pragma unroll
+        for (int r = 1; r < R; ++r) m = max_of(m, s[r]);
+        top = meet.max(m);
+    }
+    K key[R];
+    if constexpr (sizeof(K) == 8) {
+        if (sig) {
+#pragma unroll
+            for (int r = 0; r < R; ++r) key[r] = sigmoid((double)s[r]);
+        } else {
+            double sum = 0.0;
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                key[r] = exp(below((double)s[r], (double)top));
+                if (s[r] > -INFINITY) sum += key[r];   // (a row without live scores has top = -inf)
+            }
+            sum = meet.sum(sum);
+            const double inv = 1.0 / sum;
+            inv_sum = (float)inv;
+#pragma unroll
+            for (int r = 0; r < R; ++r) key[r] *= inv;
+        }
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            const uint32_t id = L::id(r);
+            double k = key[r];
+            if (w.bias && id < a.n_ids) k += (double)w.bias[id];
+            key[r] = s[r] > -INFINITY && k > -INFINITY ? k : -INFINITY;
+        }
+    } else {
+        if (over_row) {
+            float sum = 0.0f;
+#pragma unroll
+            for (int r = 0; r < R; ++r)
+                if (s[r] > -INFINITY) sum += exp_fast(below(s[r], top));
+            inv_sum = rcp_fast(meet.sum(sum));
+        }
+#pragma unroll
+        for (int r = 0; r < R; ++r) key[r] = s[r];
+    }
+
+    if (w.groups > 1) {
+        // every group's one or two largest keys, by 2^group_lanes_log2 threads a group; then the groups are selected like ids
+        K* keys = reinterpret_cast<K*>(mine);
+        K* group = keys + a.n_ids;                                             // [groups]
+        uint32_t* kept = reinterpret_cast<uint32_t*>(group + w.groups);        // a bit a group
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+            if (L::id(r) < a.n_ids) keys[L::id(r)] = key[r];
+        sync();
+        const uint32_t thread = WAVES == 1 ? lane : threadIdx.x, lanes = 1u << a.group_lanes_log2;
+        for (uint32_t g0 = 0; g0 < w.groups; g0 += (64 * WAVES) >> a.group_lanes_log2) {
+            const uint32_t g = g0 + (thread >> a.group_lanes_log2);
+            K best = (K)-INFINITY, next = (K)-INFINITY;
+            if (g < w.groups)
+                for (uint32_t e = thread & (lanes - 1); e < a.group_size; e += lanes) {
+                    const K k = keys[g * a.group_size + e];
+                    next = k > best ? best : (k > next ? k : next);
+                    best = max_of(best, k);
+                }
+            for (uint32_t d = 1; d < lanes; d <<= 1) {
+                const K b = __shfl_xor(best, (int)d, 64), n = __shfl_xor(next, (int)d, 64);
+                next = b > best ? max_of(best, n) : max_of(next, b);
+                best = max_of(best, b);
+            }
+            if (g < w.groups && (thread & (lanes - 1)) == 0) group[g] = w.group_top > 1 && next > (K)-INFINITY ? best + next : best;
+        }
+        sync();
+        if (WAVES == 1 || wave == 0) {   // the first 64 threads: group 4 * lane + j (256 groups at most)
+            K of[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) of[j] = 4 * lane + j < w.groups ? group[4 * lane + j] : (K)-INFINITY;
+            uint32_t won;
+            Meet<1> alone{nullptr, 0};
+            select_largest<4, 4, 1>(of, w.top_groups, alone, won);
+            uint32_t bits = won << ((lane & 7) * 4);   // 8 lanes a word of 32 groups
+            bits |= (uint32_t)__shfl_xor((int)bits, 1, 64);
+            bits |= (uint32_t)__shfl_xor((int)bits, 2, 64);
+            bits |= (uint32_t)__shfl_xor((int)bits, 4, 64);
+            if ((lane & 7) == 0) kept[lane >> 3] = bits;
+        }
+        sync();
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            const uint32_t id = L::id(r);
+            if (id < a.n_ids) {
+                const uint32_t g = id / a.group_size;
+                if (!(kept[g >> 5] >> (g & 31) & 1u)) key[r] = (K)-INFINITY;
+            }
+        }
+        sync();
+    }
+
+    uint32_t won;
+    const uint32_t found = select_largest<R, C, WAVES>(key, w.k, meet, won);
+
+    // the winners into LDS in ascending order: a winner's place is the number of winners in the chunks and lanes before it
+    int32_t* win_id = reinterpret_cast<int32_t*>(mine);
+    float* win_s = reinterpret_cast<float*>(win_id + w.k);
+    if constexpr (WAVES > 1) {
+#pragma unroll
+        for (int q = 0; q < R / C; ++q) {
+            uint32_t here = 0;
+#pragma unroll
+            for (int j = 0; j < C; ++j) here += (uint32_t)__builtin_popcountll(__builtin_amdgcn_ballot_w64((won >> (q * C + j)) & 1u));
+            if (lane == 0) starts[q * WAVES + wave] = here;
+        }
         __syncthreads();
-        for (uint32_t i = threadIdx.x; i < (n_ids + 31) / 32; i += kThreads) won[i] = 0;
+        if (threadIdx.x == 0) {
+            uint32_t at = 0;
+            for (int k = 0; k < WAVES * (R / C); ++k) {
+                const uint32_t n = starts[k];
+                starts[k] = at;
+                at += n;
+            }
+        }
         __syncthreads();
     }
-    uint32_t found = 0;
-    double best_logit = -INFINITY, logits = 0.0;
-    for (; found < w.k; ++found) {
-        const int e = block_best(key, n_ids, sv, si);
-        if (e < 0) break;
-        if (threadIdx.x == 0) {
-            key[e] = -INFINITY;
-            won[e >> 5] |= 1u << (e & 31);
+    uint32_t base = 0;
+#pragma unroll
+    for (int q = 0; q < R / C; ++q) {
+        uint32_t place = WAVES > 1 ? starts[q * WAVES + wave] : base;
+#pragma unroll
+        for (int j = 0; j < C; ++j) {
+            const unsigned long long m = __builtin_amdgcn_ballot_w64((won >> (q * C + j)) & 1u);
+            place += (uint32_t)__builtin_popcountll(m & ((1ull << lane) - 1ull));
+            base += (uint32_t)__builtin_popcountll(m);
         }
-        best_logit = fmax(best_logit, logit(to_f32(s[e]), sig));
-        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < C; ++j)
+            if ((won >> (q * C + j)) & 1u) {
+                win_id[place] = (int32_t)L::id(q * C + j);
+                win_s[place] = s[q * C + j];
+                ++place;
+            }
+    }
+    sync();
+
+    // the weights, a winner a thread
+    const uint32_t thread = WAVES == 1 ? lane : threadIdx.x;
+    float shift = 0.0f, norm = w.scale;
+    if (w.renormalise) {
+        float m = -INFINITY;
+        for (uint32_t i = thread; i < found; i += 64 * WAVES) m = max_of(m, win_s[i]);
+        shift = meet.max(m);
+        if (sig) shift = shift < 0.0f ? shift : 0.0f;
+        float sum = 0.0f;
+        for (uint32_t i = thread; i < found; i += 64 * WAVES) sum += sig ? sigmoid_over(win_s[i], shift) : exp_fast(below(win_s[i], shift));
+        norm = w.scale * rcp_fast(meet.sum(sum));
     }
     int32_t* ids = out_ids + row * w.k;
     float* weights = out_weights + row * w.k;
-    // ascending ids: a winner's place is the number of winners below it
-    for (uint32_t e = threadIdx.x; e < n_ids; e += kThreads) {
-        if (!(won[e >> 5] >> (e & 31) & 1u)) continue;
-        uint32_t place = __popc(won[e >> 5] & ((1u << (e & 31)) - 1u));
-        for (uint32_t i = 0; i < (e >> 5); ++i) place += __popc(won[i]);
-        ids[place] = (int32_t)e;
-        if (w.renormalise) logits += exp(below(logit(to_f32(s[e]), sig), best_logit));
-        else weights[place] = (float)((double)w.scale * share(to_f32(s[e])));
-    }
-    if (w.renormalise) {
-        logits = block_sum(logits, sv);
-        for (uint32_t e = threadIdx.x; e < n_ids; e += kThreads) {
-            if (!(won[e >> 5] >> (e & 31) & 1u)) continue;
-            uint32_t place = __popc(won[e >> 5] & ((1u << (e & 31)) - 1u));
-            for (uint32_t i = 0; i < (e >> 5); ++i) place += __popc(won[i]);
-            weights[place] = (float)((double)w.scale * exp(below(logit(to_f32(s[e]), sig), best_logit)) / logits);
+    for (uint32_t i = thread; i < w.k; i += 64 * WAVES) {
+        int32_t id = -1;
+        float weight = 0.0f;
+        if (i < found) {
+            id = win_id[i];
+            const float x = win_s[i];
+            if (sig) weight = norm * (w.renormalise ? sigmoid_over(x, shift) : sigmoid(x));
+            else weight = norm * (w.renormalise ? exp_fast(below(x, shift)) : exp_fast(below(x, top)) * inv_sum);
         }
-    }
-    for (uint32_t i = found + threadIdx.x; i < w.k; i += kThreads) {
-        ids[i] = -1;
-        weights[i] = 0.0f;
+        ids[i] = id;
+        weights[i] = weight;
     }
 }
 
-// d scores of a row, from its winners and their weights' gradient
-template <typename T, typename O>
-__global__ __launch_bounds__(kThreads) void k_winners_grad(const T* __restrict__ scores, uint64_t ld, uint32_t n_ids, sdrb_winners_spec w,
-                                                           const int32_t* __restrict__ ids_in, const float* __restrict__ grad_in,
-                                                           O* __restrict__ out, uint64_t out_ld) {
-    extern __shared__ double grad_of[];   // [n_ids]: the gradient at a winner; elsewhere 0
-    __shared__ double sv[4];
-    __shared__ uint32_t won[kWinnersMaxIds / 32];
-    const uint64_t row = blockIdx.x;
-    const T* s = scores + row * ld;
-    const int32_t* ids = ids_in + row * w.k;
-    const float* grad = grad_in + row * w.k;
+struct WinnersGradArgs {
+    sdrb_winners_spec w;
+    uint64_t n_rows, ld, out_ld;
+    uint32_t n_ids;
+    uint32_t lds_row;
+};
+
+// d scores of a row, from its winners and their weights' gradient, laid out in LDS: a row of zeros into which the winners'
+// values are put.  Only a softmax over the whole row reads the row; the other gradients read the winners' scores alone.
+// Bound: the write of the result.
+template <int R, int WAVES, bool WHOLE, typename T, typename O>
+__global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) void k_winners_grad(WinnersGradArgs a, const T* __restrict__ scores,
+                                                                                const int32_t* __restrict__ ids_in,
+                                                                                const float* __restrict__ grad_in,
+                                                                                O* __restrict__ out) {
+    using L = Layout<R, WAVES>;
+    constexpr int C = L::C;
+    extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
+    __shared__ double slots[2 * WAVES];
+    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const uint64_t row = WAVES == 1 ? (uint64_t)blockIdx.x * 4 + wave : blockIdx.x;
+    if (row >= a.n_rows) return;
+    float* line = reinterpret_cast<float*>(lds + (WAVES == 1 ? wave * a.lds_row : 0u));   // [L::kIds]
+    Meet<WAVES> meet{slots, 0};
+    const auto sync = [] {
+        if constexpr (WAVES == 1) {
+            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+            __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+        } else {
+            __syncthreads();
+        }
+    };
+    const uint32_t thread = WAVES == 1 ? lane : threadIdx.x;
+    const T* s_row = scores + row * a.ld;
+    const int32_t* ids = ids_in + row * a.w.k;
+    const float* grad = grad_in + row * a.w.k;
+    const sdrb_winners_spec& w = a.w;
     const bool sig = w.score == SDRB_SCORE_SIGMOID;
-    for (uint32_t i = threadIdx.x; i < (n_ids + 31) / 32; i += kThreads) won[i] = 0;
-    for (uint32_t e = threadIdx.x; e < n_ids; e += kThreads) grad_of[e] = 0.0;
-    __syncthreads();
-    const auto winner = [&](uint32_t i) { return ids[i] >= 0 && (uint32_t)ids[i] < n_ids && live_score(to_f32(s[ids[i]])); };
-    for (uint32_t i = threadIdx.x; i < w.k; i += kThreads)
-        if (winner(i)) {
-            grad_of[ids[i]] = grad[i];
-            atomicOr(&won[ids[i] >> 5], 1u << (ids[i] & 31));
+    float s[WHOLE ? R : 1];
+    if constexpr (WHOLE) read_row<R, WAVES>(s_row, a.n_ids, -INFINITY, s);
+    const float zeros[C] = {};
+#pragma unroll
+    for (int q = 0; q < R / C; ++q) store_n<C>(line + L::id(q * C), zeros);
+    sync();
+    // a thread's winners: the score of place i, -inf where it holds none
+    const auto score_at = [&](uint32_t i, int32_t& id) {
+        id = ids[i];
+        if (id < 0 || (uint32_t)id >= a.n_ids) return -INFINITY;
+        const float x = to_f32(s_row[id]);
+        return x > -INFINITY ? x : -INFINITY;   // (a NaN never won)
+    };
+    if constexpr (WHOLE) {
+        for (uint32_t i = thread; i < w.k; i += 64 * WAVES) {
+            int32_t id;
+            if (score_at(i, id) > -INFINITY) line[id] = grad[i];
         }
-    __syncthreads();
-    const bool whole = !sig && !w.renormalise;   // a softmax over every live score
-    double top = -INFINITY, sum = 0.0, dot = 0.0;
-    const auto counts = [&](uint32_t e) { return whole ? live_score(to_f32(s[e])) : (won[e >> 5] >> (e & 31) & 1u) != 0; };
-    if (whole || w.renormalise) {
-        for (uint32_t e = threadIdx.x; e < n_ids; e += kThreads)
-            if (counts(e)) top = fmax(top, logit(to_f32(s[e]), sig));
-        top = block_max(top, sv);
-        for (uint32_t e = threadIdx.x; e < n_ids; e += kThreads)
-            if (counts(e)) {
-                const double p = exp(below(logit(to_f32(s[e]), sig), top));
-                sum += p;
-                dot += p * grad_of[e];
-            }
-        sum = block_sum(sum, sv);
-        dot = block_sum(dot, sv) / sum;
-    }
-    for (uint32_t e = threadIdx.x; e < n_ids; e += kThreads) {
-        double d = 0.0;
-        if (counts(e)) {
-            const double x = to_f32(s[e]);
-            if (whole || w.renormalise) {
-                d = exp(below(logit(x, sig), top)) / sum * (grad_of[e] - dot);
-                if (sig) d *= sigmoid(-x);
+        sync();
+        float m = -INFINITY;
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            s[r] = s[r] > -INFINITY ? s[r] : -INFINITY;   // (a NaN has no share)
+            m = max_of(m, s[r]);
+        }
+        m = meet.max(m);
+        float g[R], sum = 0.0f, dot = 0.0f;
+#pragma unroll
+        for (int q = 0; q < R / C; ++q) {
+            float part[C];
+            load_n<C>(line + L::id(q * C), part);
+#pragma unroll
+            for (int j = 0; j < C; ++j) g[q * C + j] = part[j];
+        }
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            s[r] = s[r] > -INFINITY ? exp_fast(below(s[r], m)) : 0.0f;
+            sum += s[r];
+            dot = fmaf(s[r], g[r], dot);
+        }
+        const float inv = rcp_fast(meet.sum(sum));
+        dot = meet.sum(dot) * inv;
+        const float scale = w.scale * inv;
+#pragma unroll
+        for (int r = 0; r < R; ++r) s[r] = s[r] > 0.0f ? scale * s[r] * (g[r] - dot) : 0.0f;
+#pragma unroll
+        for (int q = 0; q < R / C; ++q) {
+            const uint32_t first = L::id(q * C);
+            O* to = out + row * a.out_ld + first;
+            if (first + C <= a.n_ids) {
+                float part[C];
+#pragma unroll
+                for (int j = 0; j < C; ++j) part[j] = s[q * C + j];
+                store_n<C>(to, part);
             } else {
-                d = grad_of[e] * sigmoid(x) * sigmoid(-x);
+#pragma unroll
+                for (int j = 0; j < C; ++j)
+                    if (first + j < a.n_ids) to[j] = from_f32<O>(s[q * C + j]);
             }
         }
-        out[row * out_ld + e] = from_f32<O>((float)((double)w.scale * d));
+    } else {
+        float shift = 0.0f, inv = 1.0f, dot = 0.0f;
+        const auto part_of = [&](float x) { return sig ? sigmoid_over(x, shift) : exp_fast(below(x, shift)); };
+        if (w.renormalise) {
+            float m = -INFINITY, sum = 0.0f;
+            int32_t id;
+            for (uint32_t i = thread; i < w.k; i += 64 * WAVES) m = max_of(m, score_at(i, id));
+            shift = meet.max(m);
+            if (sig) shift = shift < 0.0f ? shift : 0.0f;
+            for (uint32_t i = thread; i < w.k; i += 64 * WAVES) {
+                const float x = score_at(i, id);
+                if (x > -INFINITY) {
+                    const float p = part_of(x);
+                    sum += p;
+                    dot = fmaf(p, grad[i], dot);
+                }
+            }
+            inv = rcp_fast(meet.sum(sum));
+            dot = meet.sum(dot) * inv;
+        }
+        for (uint32_t i = thread; i < w.k; i += 64 * WAVES) {
+            int32_t id;
+            const float x = score_at(i, id);
+            if (x > -INFINITY) {
+                float d = w.renormalise ? part_of(x) * inv * (grad[i] - dot) : grad[i] * sigmoid(x);
+                if (sig) d *= sigmoid(-x);
+                line[id] = w.scale * d;
+            }
+        }
+        sync();
+        constexpr int V = 16 / sizeof(O);   // 16 bytes of the result a lane
+        for (uint32_t first = thread * V; first < a.n_ids; first += 64 * WAVES * V) {
+            float part[V];
+            load_n<V>(line + first, part);
+            O* to = out + row * a.out_ld + first;
+            if (first + V <= a.n_ids) {
+                store_n<V>(to, part);
+            } else {
+                for (int j = 0; j < V; ++j)
+                    if (first + j < a.n_ids) to[j] = from_f32<O>(part[j]);
+            }
+        }
     }
+}
+
+// calls f(R, WAVES) with the smallest layout that holds n ids
+template <typename F>
+int with_layout(uint32_t n, F&& f) {
+    using std::integral_constant;
+    const auto one = integral_constant<int, 1>{};
+    const auto eight = integral_constant<int, 8>{};
+    if (n <= 64) return f(integral_constant<int, 1>{}, one);
+    if (n <= 128) return f(integral_constant<int, 2>{}, one);
+    if (n <= 256) return f(integral_constant<int, 4>{}, one);
+    if (n <= 512) return f(integral_constant<int, 8>{}, one);
+    if (n <= 1024) return f(integral_constant<int, 16>{}, one);
+    if (n <= 2048) return f(integral_constant<int, 32>{}, one);
+    if (n <= 4096) return f(integral_constant<int, 8>{}, eight);
+    if (n <= 8192) return f(integral_constant<int, 16>{}, eight);
+    return f(integral_constant<int, 32>{}, eight);
+}
+
+// more than 64 KiB of dynamic LDS has to be asked for
+template <typename F>
+int allow_lds(F* kernel, size_t bytes) {
+    if (bytes > 65536) SDRB_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+    return SDRB_OK;
 }
 
 }  // namespace
 
 int launch_winners(const sdrb_dense& scores, const sdrb_winners_spec& spec, int32_t* ids, float* weights, hipStream_t stream) {
-    const uint32_t n_ids = (uint32_t)scores.n_cols;
-    const size_t lds = (size_t)(n_ids + spec.groups) * sizeof(double);
-    return with_type(scores.type, [&](auto t) {
-        using T = decltype(t);
-        SDRB_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(&k_winners<T>), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
-        hipLaunchKernelGGL((k_winners<T>), dim3((uint32_t)scores.n_rows), dim3(kThreads), lds, stream, static_cast<const T*>(scores.data),
-                           scores.ld, n_ids, spec, ids, weights);
-        SDRB_HIP(hipGetLastError());
-        return SDRB_OK;
+    WinnersArgs a{};
+    a.w = spec;
+    a.n_rows = scores.n_rows;
+    a.ld = scores.ld;
+    a.n_ids = (uint32_t)scores.n_cols;
+    a.group_size = a.n_ids / spec.groups;
+    const bool shares = spec.bias || (spec.groups > 1 && spec.group_top > 1);
+    return with_layout(a.n_ids, [&](auto r, auto waves) {
+        constexpr int R = decltype(r)::value, WAVES = decltype(waves)::value;
+        a.group_lanes_log2 = 0;
+        while (a.group_lanes_log2 < 6 && (spec.groups << (a.group_lanes_log2 + 1)) <= 64u * WAVES) ++a.group_lanes_log2;
+        return with_type(scores.type, [&](auto t) {
+            using T = decltype(t);
+            const auto go = [&](auto k) {
+                using K = decltype(k);
+                const size_t grouped = spec.groups > 1 ? (size_t)(a.n_ids + spec.groups) * sizeof(K) + kWinnersMaxGroups / 8 : 0;
+                const size_t listed = (size_t)spec.k * 8;
+                a.lds_row = (uint32_t)(((grouped > listed ? grouped : listed) + 15) / 16 * 16);
+                const size_t lds = (size_t)a.lds_row * (WAVES == 1 ? 4 : 1);
+                const uint64_t blocks = WAVES == 1 ? (a.n_rows + 3) / 4 : a.n_rows;
+                if (const int rc = allow_lds(&k_winners<R, WAVES, K, T>, lds)) return rc;
+                hipLaunchKernelGGL((k_winners<R, WAVES, K, T>), dim3((uint32_t)blocks), dim3(WAVES == 1 ? 256 : 64 * WAVES), lds, stream, a,
+                                   static_cast<const T*>(scores.data), ids, weights);
+                SDRB_HIP(hipGetLastError());
+                return SDRB_OK;
+            };
+            return shares ? go(double{}) : go(float{});
+        });
     });
 }
 
 int launch_winners_grad(const sdrb_dense& scores, const sdrb_winners_spec& spec, const int32_t* ids, const float* grad_weights,
                         const sdrb_dense& out, hipStream_t stream) {
-    const uint32_t n_ids = (uint32_t)scores.n_cols;
-    return with_type(scores.type, [&](auto t) {
-        return with_type(out.type, [&](auto o) {
-            using T = decltype(t);
-            using O = decltype(o);
-            const size_t lds = (size_t)n_ids * sizeof(double);
-            SDRB_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(&k_winners_grad<T, O>), hipFuncAttributeMaxDynamicSharedMemorySize,
-                                         (int)lds));
-            hipLaunchKernelGGL((k_winners_grad<T, O>), dim3((uint32_t)scores.n_rows), dim3(kThreads), lds, stream,
-                               static_cast<const T*>(scores.data), scores.ld, n_ids, spec, ids, grad_weights, static_cast<O*>(out.data),
-                               out.ld);
-            SDRB_HIP(hipGetLastError());
-            return SDRB_OK;
+    WinnersGradArgs a{};
+    a.w = spec;
+    a.n_rows = scores.n_rows;
+    a.ld = scores.ld;
+    a.out_ld = out.ld;
+    a.n_ids = (uint32_t)scores.n_cols;
+    const bool whole = spec.score == SDRB_SCORE_SOFTMAX && !spec.renormalise;
+    return with_layout(a.n_ids, [&](auto r, auto waves) {
+        constexpr int R = decltype(r)::value, WAVES = decltype(waves)::value;
+        a.lds_row = (uint32_t)(Layout<R, WAVES>::kIds + 8) * sizeof(float);   // (16 bytes of result are read at a time)
+        const size_t lds = (size_t)a.lds_row * (WAVES == 1 ? 4 : 1);
+        const uint64_t blocks = WAVES == 1 ? (a.n_rows + 3) / 4 : a.n_rows;
+        return with_type(scores.type, [&](auto t) {
+            return with_type(out.type, [&](auto o) {
+                using T = decltype(t);
+                using O = decltype(o);
+                const auto go = [&](auto all) {
+                    constexpr bool WHOLE = decltype(all)::value;
+                    if (const int rc = allow_lds(&k_winners_grad<R, WAVES, WHOLE, T, O>, lds)) return rc;
+                    hipLaunchKernelGGL((k_winners_grad<R, WAVES, WHOLE, T, O>), dim3((uint32_t)blocks), dim3(WAVES == 1 ? 256 : 64 * WAVES),
+                                       lds, stream, a, static_cast<const T*>(scores.data), ids, grad_weights, static_cast<O*>(out.data));
+                    SDRB_HIP(hipGetLastError());
+                    return SDRB_OK;
+                };
+                return whole ? go(std::true_type{}) : go(std::false_type{});
+            });
         });
     });
 }
