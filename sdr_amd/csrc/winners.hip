@@ -6,14 +6,20 @@
 // Weights: scale * u, or, renormalised, scale * p with p = u / sum of the winners' u -- a softmax over the winners of
 // l = s (softmax) or l = log sigmoid(s), which holds where every u underflows.
 //
-// A wave owns a row and holds its keys in registers, R a lane, read once; rows of more than 2048 ids are shared by eight
-// waves.  The k-th largest key is found by bisection over the keys' order-preserving integers: a step is a compare and a
-// population count a register, whatever k is, and it ends as soon as exactly k keys lie at or above the middle.  The
-// bisection starts between the smallest of the lanes' largest keys (for k up to the number of lanes at least k keys lie at
-// or above it) and the largest key, so that it takes six to twelve steps on scores without ties.
-// Shares that enter keys are computed in binary64: whether an id wins hangs on the difference of two keys, which binary32
-// exponentials would decide by their own error.  The hardware does binary64 arithmetic at the rate of binary32.
+// A wave owns a row and holds its scores in registers, R a lane, read once; rows of more than 2048 ids are shared by eight
+// waves.  Two steps choose the winners:
+//  1. Candidates.  Of the lanes' largest keys a threshold is found that k of them reach (a compare and a population count a
+//     step), so at least k keys reach it, and few more: about 62 of 2048 for k = 40.  Keys are binary32 here; where shares
+//     enter them the threshold is lowered by what their arithmetic can be off, so that no winner is lost.
+//  2. The candidates' ids go to LDS in ascending order, one a thread from there on; their keys are computed exactly, and the
+//     k-th largest is found by bisection over the keys' order-preserving integers, which ends as soon as exactly k keys lie
+//     at or above the middle.
+// Shares that enter keys are computed in binary64 in the second step: whether an id wins hangs on the difference of two keys,
+// which binary32 exponentials would decide by their own error.  Rows whose candidates are too many (many equal scores, a k
+// near the number of lanes) or whose groups cannot be told apart in binary32 bisect over all their keys instead.
 // Bound: instruction issue, not memory.
+#include <type_traits>
+
 #include "dense_rows.h"
 
 namespace sdrb {
@@ -119,7 +125,7 @@ __device__ __forceinline__ K key_at(typename Ordered<K>::U order) {
 // Where a lane's register r stands in the row: registers are read C at a time, 64 lanes side by side.
 template <int R, int WAVES>
 struct Layout {
-    static constexpr int C = R < 4 ? R : 4;
+    static constexpr int C = R < 8 ? R : 8;
     static constexpr int kIds = 64 * R * WAVES;
     __device__ __forceinline__ static uint32_t id(int r) {
         const uint32_t thread = threadIdx.x & (64 * WAVES - 1);
@@ -234,11 +240,90 @@ __device__ __forceinline__ K below(K x, K m) {
     return x == m ? (K)0 : x - m;
 }
 __device__ __forceinline__ float sigmoid(float x) { return rcp_fast(1.0f + exp_fast(-x)); }
-__device__ __forceinline__ double sigmoid(double x) { return 1.0 / (1.0 + exp(-x)); }
+// e^x in binary64: x = n ln 2 + r with |r| <= ln 2 / 2, the Taylor polynomial of degree 13 in r (its first missing term is
+// below 2^-57), scaled by 2^n.  Within two steps of its value; arguments beyond +-800 give infinity and 0.
+__device__ __forceinline__ double exp64(double x) {
+    x = fmin(fmax(x, -800.0), 800.0);
+    const double n = rint(x * 1.44269504088896340736);
+    double r = fma(n, -6.93147180369123816490e-01, x);   // ln 2 in two parts, the first short enough that n times it is exact
+    r = fma(n, -1.90821492927058770002e-10, r);
+    double p = 1.0 / 6227020800.0;
+    p = fma(p, r, 1.0 / 479001600.0);
+    p = fma(p, r, 1.0 / 39916800.0);
+    p = fma(p, r, 1.0 / 3628800.0);
+    p = fma(p, r, 1.0 / 362880.0);
+    p = fma(p, r, 1.0 / 40320.0);
+    p = fma(p, r, 1.0 / 5040.0);
+    p = fma(p, r, 1.0 / 720.0);
+    p = fma(p, r, 1.0 / 120.0);
+    p = fma(p, r, 1.0 / 24.0);
+    p = fma(p, r, 1.0 / 6.0);
+    p = fma(p, r, 0.5);
+    p = fma(p, r, 1.0);
+    p = fma(p, r, 1.0);
+    return ldexp(p, (int)n);
+}
+// 1 / x for 1 <= x < 1e305: the hardware's approximation and two Newton steps
+__device__ __forceinline__ double rcp64(double x) {
+    double y = __builtin_amdgcn_rcp(x);
+    y = fma(y, fma(-x, y, 1.0), y);
+    return fma(y, fma(-x, y, 1.0), y);
+}
+__device__ __forceinline__ double sigmoid(double x) { return rcp64(1.0 + exp64(fmin(fmax(-x, -700.0), 700.0))); }
 // sigmoid(x) e^-c, c <= 0 no smaller than any x that is negative: ratios of sigmoids that would all underflow
 __device__ __forceinline__ float sigmoid_over(float x, float c) {
     const float t = rcp_fast(1.0f + exp_fast(-fabsf(x)));
     return x < 0.0f ? exp_fast(below(x, c)) * t : t;
+}
+
+__device__ __forceinline__ uint32_t bits_in(unsigned long long mask) { return (uint32_t)__builtin_popcountll(mask); }
+
+// inclusive sums over the lanes of a wave
+__device__ __forceinline__ uint32_t scan_lanes(uint32_t v) {
+    v += (uint32_t)dpp<0x111, 0xF>(0, (int)v);   // one lane up in a row of 16, two, four, eight
+    v += (uint32_t)dpp<0x112, 0xF>(0, (int)v);
+    v += (uint32_t)dpp<0x114, 0xF>(0, (int)v);
+    v += (uint32_t)dpp<0x118, 0xF>(0, (int)v);
+    v += (uint32_t)dpp<0x142, 0xA>(0, (int)v);
+    v += (uint32_t)dpp<0x143, 0xC>(0, (int)v);
+    return v;
+}
+
+// here[q]: what this thread holds in chunk q (at most 8).  place[q]: what stands before it, chunks first, then threads; returns
+// the total.
+template <int Q, int WAVES>
+__device__ __forceinline__ uint32_t places(const uint32_t (&here)[Q], uint32_t (&place)[Q], uint32_t* starts) {
+    uint32_t total = 0, packed[(Q + 1) / 2], sums[(Q + 1) / 2];
+    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll
+    for (int p = 0; p < (Q + 1) / 2; ++p) {
+        packed[p] = here[2 * p] | (2 * p + 1 < Q ? here[2 * p + 1] << 16 : 0u);
+        sums[p] = scan_lanes(packed[p]);
+    }
+#pragma unroll
+    for (int q = 0; q < Q; ++q) {
+        const uint32_t in_wave = ((uint32_t)last_lane((int)sums[q / 2]) >> (q % 2 * 16)) & 0xFFFFu;
+        place[q] = ((sums[q / 2] - packed[q / 2]) >> (q % 2 * 16)) & 0xFFFFu;
+        if constexpr (WAVES == 1) {
+            place[q] += total;
+            total += in_wave;
+        } else {
+            if (lane == 0) starts[q * WAVES + wave] = in_wave;
+        }
+    }
+    if constexpr (WAVES > 1) {
+        __syncthreads();
+        uint32_t at = 0;
+#pragma unroll
+        for (int q = 0; q < Q; ++q)
+            for (int w = 0; w < WAVES; ++w) {
+                if ((uint32_t)w == wave) place[q] += at;
+                at += starts[q * WAVES + w];
+            }
+        total = at;
+        __syncthreads();
+    }
+    return total;
 }
 
 struct WinnersArgs {
@@ -246,25 +331,36 @@ struct WinnersArgs {
     uint64_t n_rows, ld;
     uint32_t n_ids;
     uint32_t group_size, group_lanes_log2;   // ids of a group; lanes that look at one group together
+    uint32_t group_magic;                    // id * group_magic >> 31 is the id's group
     uint32_t lds_row;                        // bytes of dynamic LDS a row has
 };
 
-// K: float, keys are the scores; double, keys are shares (+ bias)
-template <int R, int WAVES, typename K, typename T>
-__global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) void k_winners(WinnersArgs a, const T* __restrict__ scores,
-                                                                           int32_t* __restrict__ out_ids,
-                                                                           float* __restrict__ out_weights) {
+// candidates a thread takes at most; the threshold is looked for where k is at most this part of the lanes
+constexpr int kHeld = 4;
+constexpr uint32_t kLanePart = 48;
+
+// A row of scores in its threads' registers, and the steps that choose its winners.  SHARES: keys are shares (+ bias), exactly
+// so in binary64; else the scores.
+template <int R, int WAVES, bool SHARES, typename T>
+struct Row {
     using L = Layout<R, WAVES>;
-    constexpr int C = L::C;
-    extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
-    __shared__ double slots[2 * WAVES];
-    __shared__ uint32_t starts[WAVES == 1 ? 1 : WAVES * (R / C)];
-    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const uint64_t row = WAVES == 1 ? (uint64_t)blockIdx.x * 4 + wave : blockIdx.x;
-    if (row >= a.n_rows) return;
-    unsigned char* mine = lds + (WAVES == 1 ? wave * a.lds_row : 0u);
-    Meet<WAVES> meet{slots, 0};
-    const auto sync = [] {   // LDS written by this row's waves before, read after
+    using K = std::conditional_t<SHARES, double, float>;
+    static constexpr int C = L::C, Q = R / C;
+
+    const WinnersArgs& a;
+    const T* s_row;
+    unsigned char* mine;    // LDS of the row
+    uint32_t* starts;       // LDS, [WAVES][at most 8] where WAVES > 1
+    Meet<WAVES> meet;
+    float s[R];
+    float top, inv_sum;     // of a softmax over the row
+
+    __device__ __forceinline__ bool sig() const { return a.w.score == SDRB_SCORE_SIGMOID; }
+    __device__ __forceinline__ uint32_t thread() const { return WAVES == 1 ? threadIdx.x & 63 : threadIdx.x; }
+    // the winners in LDS, ascending
+    __device__ __forceinline__ int32_t* win_ids() const { return reinterpret_cast<int32_t*>(mine); }
+    __device__ __forceinline__ float* win_scores() const { return reinterpret_cast<float*>(mine) + a.w.k; }
+    __device__ __forceinline__ void sync() const {   // LDS written by this row's waves before, read after
         if constexpr (WAVES == 1) {
             __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
             __builtin_amdgcn_wave_barrier();
@@ -272,170 +368,260 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) void k_winners(Winne
         } else {
             __syncthreads();
         }
-    };
-    const T* s_row = scores + row * a.ld;
-    const sdrb_winners_spec& w = a.w;
-    const bool sig = w.score == SDRB_SCORE_SIGMOID;
-
-    float s[R];
-    read_row<R, WAVES>(s_row, a.n_ids, -INFINITY, s);
-#pragma unroll
-    for (int r = 0; r < R; ++r) s[r] = s[r] > -INFINITY ? s[r] + 0.0f : -INFINITY;   // NaN is no score; -0 is 0
-
-    // keys; top and inv_sum of a softmax over the row where one is needed
-    float top = 0.0f, inv_sum = 0.0f;
-    const bool over_row = !sig && (sizeof(K) == 8 || !w.renormalise);
-    if (over_row) {
-        float m = s[0];
-#pragma unroll
-        for (int r = 1; r < R; ++r) m = max_of(m, s[r]);
-        top = meet.max(m);
-    }
-    K key[R];
-    if constexpr (sizeof(K) == 8) {
-        if (sig) {
-#pragma unroll
-            for (int r = 0; r < R; ++r) key[r] = sigmoid((double)s[r]);
-        } else {
-            double sum = 0.0;
-#pragma unroll
-            for (int r = 0; r < R; ++r) {
-                key[r] = exp(below((double)s[r], (double)top));
-                if (s[r] > -INFINITY) sum += key[r];   // (a row without live scores has top = -inf)
-            }
-            sum = meet.sum(sum);
-            const double inv = 1.0 / sum;
-            inv_sum = (float)inv;
-#pragma unroll
-            for (int r = 0; r < R; ++r) key[r] *= inv;
-        }
-#pragma unroll
-        for (int r = 0; r < R; ++r) {
-            const uint32_t id = L::id(r);
-            double k = key[r];
-            if (w.bias && id < a.n_ids) k += (double)w.bias[id];
-            key[r] = s[r] > -INFINITY && k > -INFINITY ? k : -INFINITY;
-        }
-    } else {
-        if (over_row) {
-            float sum = 0.0f;
-#pragma unroll
-            for (int r = 0; r < R; ++r)
-                if (s[r] > -INFINITY) sum += exp_fast(below(s[r], top));
-            inv_sum = rcp_fast(meet.sum(sum));
-        }
-#pragma unroll
-        for (int r = 0; r < R; ++r) key[r] = s[r];
     }
 
-    if (w.groups > 1) {
-        // every group's one or two largest keys, by 2^group_lanes_log2 threads a group; then the groups are selected like ids
-        K* keys = reinterpret_cast<K*>(mine);
-        K* group = keys + a.n_ids;                                             // [groups]
-        uint32_t* kept = reinterpret_cast<uint32_t*>(group + w.groups);        // a bit a group
+    // 1 / sum of the row's exponentials, which every share of a softmax has as a factor
+    __device__ __forceinline__ double exact_inverse_sum() {
+        double sum = 0.0;
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+            if (s[r] > -INFINITY) sum += exp64(below((double)s[r], (double)top));
+        return 1.0 / meet.sum(sum);
+    }
+    __device__ __forceinline__ double exact_key(float x, uint32_t id, double inverse_sum) const {
+        double key = sig() ? sigmoid((double)x) : exp64(below((double)x, (double)top)) * inverse_sum;
+        if (a.w.bias) key += (double)a.w.bias[id];
+        return x > -INFINITY && key > -INFINITY ? key : -INFINITY;   // (a NaN of the bias is no key)
+    }
+
+    // keys of the kept groups stay; false where `slack` > 0 and binary32 keys do not tell the groups apart.  slack: how far
+    // a key may be off, beside its own rounding
+    template <typename F>
+    __device__ __forceinline__ bool keep_groups(F (&key)[R], F slack) {
+        const sdrb_winners_spec& w = a.w;
+        F* keys = reinterpret_cast<F*>(mine);
+        F* group = keys + a.n_ids;                                          // [groups]
+        uint32_t* kept = reinterpret_cast<uint32_t*>(group + w.groups);     // a bit a group
 #pragma unroll
         for (int r = 0; r < R; ++r)
             if (L::id(r) < a.n_ids) keys[L::id(r)] = key[r];
         sync();
-        const uint32_t thread = WAVES == 1 ? lane : threadIdx.x, lanes = 1u << a.group_lanes_log2;
+        // a group's one or two largest keys, by 2^group_lanes_log2 threads a group
+        const uint32_t lanes = 1u << a.group_lanes_log2, lane = threadIdx.x & 63;
+        F size = (F)0;   // of the keys that are summed
         for (uint32_t g0 = 0; g0 < w.groups; g0 += (64 * WAVES) >> a.group_lanes_log2) {
-            const uint32_t g = g0 + (thread >> a.group_lanes_log2);
-            K best = (K)-INFINITY, next = (K)-INFINITY;
+            const uint32_t g = g0 + (thread() >> a.group_lanes_log2);
+            F best = (F)-INFINITY, next = (F)-INFINITY;
             if (g < w.groups)
-                for (uint32_t e = thread & (lanes - 1); e < a.group_size; e += lanes) {
-                    const K k = keys[g * a.group_size + e];
+                for (uint32_t e = thread() & (lanes - 1); e < a.group_size; e += lanes) {
+                    const F k = keys[g * a.group_size + e];
                     next = k > best ? best : (k > next ? k : next);
                     best = max_of(best, k);
                 }
             for (uint32_t d = 1; d < lanes; d <<= 1) {
-                const K b = __shfl_xor(best, (int)d, 64), n = __shfl_xor(next, (int)d, 64);
+                const F b = __shfl_xor(best, (int)d, 64), n = __shfl_xor(next, (int)d, 64);
                 next = b > best ? max_of(best, n) : max_of(next, b);
                 best = max_of(best, b);
             }
-            if (g < w.groups && (thread & (lanes - 1)) == 0) group[g] = w.group_top > 1 && next > (K)-INFINITY ? best + next : best;
+            const bool two = w.group_top > 1 && next > (F)-INFINITY;
+            if (g < w.groups && (thread() & (lanes - 1)) == 0) group[g] = two ? best + next : best;
+            if (best > (F)-INFINITY) size = max_of(size, (best < 0 ? -best : best) + (two ? (next < 0 ? -next : next) : (F)0));
         }
         sync();
-        if (WAVES == 1 || wave == 0) {   // the first 64 threads: group 4 * lane + j (256 groups at most)
-            K of[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) of[j] = 4 * lane + j < w.groups ? group[4 * lane + j] : (K)-INFINITY;
-            uint32_t won;
-            Meet<1> alone{nullptr, 0};
-            select_largest<4, 4, 1>(of, w.top_groups, alone, won);
-            uint32_t bits = won << ((lane & 7) * 4);   // 8 lanes a word of 32 groups
-            bits |= (uint32_t)__shfl_xor((int)bits, 1, 64);
-            bits |= (uint32_t)__shfl_xor((int)bits, 2, 64);
-            bits |= (uint32_t)__shfl_xor((int)bits, 4, 64);
-            if ((lane & 7) == 0) kept[lane >> 3] = bits;
+        bool sure = true;
+        if (slack > (F)0) size = meet.max(size);
+        if (WAVES == 1 || threadIdx.x < 64) {
+            // a group is kept if fewer than top_groups groups stand before it; thread lane + 64 j looks at one each
+            F worst = (F)INFINITY, lost = (F)-INFINITY;
+            for (uint32_t g0 = 0; g0 < w.groups; g0 += 64) {
+                const uint32_t g = g0 + lane;
+                const F mine_is = g < w.groups ? group[g] : (F)-INFINITY;
+                uint32_t before = 0;
+                for (uint32_t o = 0; o < w.groups; ++o) {
+                    const F other = group[o];
+                    before += other > mine_is || (other == mine_is && o < g) ? 1u : 0u;
+                }
+                const bool in = mine_is > (F)-INFINITY && before < w.top_groups;
+                const unsigned long long m = __builtin_amdgcn_ballot_w64(in);
+                if (lane == 0) {
+                    kept[g0 / 32] = (uint32_t)m;
+                    kept[g0 / 32 + 1] = (uint32_t)(m >> 32);
+                }
+                if (in) worst = mine_is < worst ? mine_is : worst;
+                else lost = max_of(lost, mine_is);
+            }
+            if (slack > (F)0) {
+                worst = -wave_reduce(-worst, (F)-INFINITY, max_of<F>);
+                lost = wave_reduce(lost, (F)-INFINITY, max_of<F>);
+                // two sums, of two keys each: every one off by slack and three roundings of at most `size`
+                if (lost > (F)-INFINITY && !(worst - lost > 4 * slack + size * (F)0x1p-20)) sure = false;
+            }
         }
+        if (WAVES > 1 && slack > (F)0) sure = meet.total(threadIdx.x < 64 && !sure ? 1u : 0u) == 0;
         sync();
 #pragma unroll
         for (int r = 0; r < R; ++r) {
-            const uint32_t id = L::id(r);
-            if (id < a.n_ids) {
-                const uint32_t g = id / a.group_size;
-                if (!(kept[g >> 5] >> (g & 31) & 1u)) key[r] = (K)-INFINITY;
+            const uint32_t g = __umulhi(2 * L::id(r), a.group_magic);   // (ids beyond the row have no key)
+            if (key[r] > (F)-INFINITY && !(kept[g >> 5] >> (g & 31) & 1u)) key[r] = (F)-INFINITY;
+        }
+        sync();
+        return sure;
+    }
+
+    // the winners among keys that the threads hold C at a time, to LDS
+    template <int H, int CH, typename F, typename G>
+    __device__ __forceinline__ uint32_t put_winners(const K (&key)[H], F id_of, G score_of) {
+        uint32_t won, here[H / CH], place[H / CH];
+        const uint32_t found = select_largest<H, CH, WAVES>(key, a.w.k, meet, won);
+#pragma unroll
+        for (int q = 0; q < H / CH; ++q) here[q] = __popc((won >> (q * CH)) & (uint32_t)((1ull << CH) - 1));
+        places<H / CH, WAVES>(here, place, starts);
+#pragma unroll
+        for (int j = 0; j < H; ++j)
+            if ((won >> j) & 1u) {
+                win_ids()[place[j / CH]] = id_of(j);
+                win_scores()[place[j / CH]++] = score_of(j);
+            }
+        sync();
+        return found;
+    }
+
+    // the candidates that a threshold leaves, and the winners among them; false where the row needs choose_among_all
+    __device__ __forceinline__ bool choose_among_candidates(uint32_t& found) {
+        const sdrb_winners_spec& w = a.w;
+        if (w.k > kLanePart * WAVES) return false;
+        float rough[R], slack = 0.0f;
+        if constexpr (SHARES) {
+            // Off by less than 3.1 * 2^-24 for the sigmoid -- 1.5 |x| + 2 steps in its exponential t, which enter the result
+            // with t / (1 + t)^2, and two roundings -- and than 2^-17 of the largest share for the softmax, 67 * 2^-24 by its
+            // own exponential and a sum of at most 32 + 6 + 8 additions.
+            slack = sig() ? 0x1p-22f : inv_sum * 0x1p-17f;
+#pragma unroll
+            for (int r = 0; r < R; ++r) rough[r] = sig() ? sigmoid(s[r]) : exp_fast(below(s[r], top)) * inv_sum;
+            if (w.bias) {
+                float b[R];
+                read_row<R, WAVES>(w.bias, a.n_ids, 0.0f, b);
+#pragma unroll
+                for (int r = 0; r < R; ++r) rough[r] += b[r];
+            }
+#pragma unroll
+            for (int r = 0; r < R; ++r) rough[r] = s[r] > -INFINITY && rough[r] > -INFINITY ? rough[r] : -INFINITY;
+        } else {
+#pragma unroll
+            for (int r = 0; r < R; ++r) rough[r] = s[r];
+        }
+        if (w.groups > 1 && !keep_groups<float>(rough, slack)) return false;
+
+        float mine_top = rough[0];
+#pragma unroll
+        for (int r = 1; r < R; ++r) mine_top = max_of(mine_top, rough[r]);
+        const auto reach = [&](float t) { return meet.total(bits_in(__builtin_amdgcn_ballot_w64(mine_top >= t))); };
+        float t = -INFINITY;
+        if (meet.total(bits_in(__builtin_amdgcn_ballot_w64(mine_top > -INFINITY))) >= w.k) {
+            const float least = -meet.max(mine_top > -INFINITY ? -mine_top : -INFINITY);   // of the live lanes
+            uint32_t lo = order_of(least), hi = order_of(meet.max(mine_top)) + 1;
+            const uint32_t enough = w.k + w.k / 8 + 1;
+            while (hi - lo > 1) {
+                const uint32_t mid = lo + (hi - lo) / 2, c = reach(key_at<float>(mid));
+                if (c >= w.k) lo = mid;
+                else hi = mid;
+                if (c >= w.k && c <= enough) break;
+            }
+            t = key_at<float>(lo);
+            // k keys are no smaller than t less what a key can be off; a key as large may seem smaller by as much again
+            if (SHARES) t -= 2.0f * slack + fabsf(t) * 0x1p-21f;   // (an infinite t becomes NaN, which nothing reaches)
+        }
+        uint32_t bits = 0, here[Q], place[Q];
+#pragma unroll
+        for (int r = 0; r < R; ++r) bits |= rough[r] >= t && rough[r] > -INFINITY ? 1u << r : 0u;
+#pragma unroll
+        for (int q = 0; q < Q; ++q) here[q] = __popc((bits >> (q * C)) & ((1u << C) - 1u));
+        const uint32_t n = places<Q, WAVES>(here, place, starts);
+        if (n > 64u * WAVES * kHeld || (n < w.k && t != -INFINITY)) return false;
+        int32_t* list = reinterpret_cast<int32_t*>(mine);
+#pragma unroll
+        for (int q = 0; q < Q; ++q) {
+            uint32_t b = (bits >> (q * C)) & ((1u << C) - 1u), at = place[q];
+            while (b) {
+                list[at++] = (int32_t)(L::id(q * C) + (uint32_t)__builtin_ctz(b));
+                b &= b - 1;
             }
         }
         sync();
+        found = n <= 64 * WAVES ? choose_from_list<1>(list, n) : choose_from_list<kHeld>(list, n);
+        return true;
     }
-
-    uint32_t won;
-    const uint32_t found = select_largest<R, C, WAVES>(key, w.k, meet, won);
-
-    // the winners into LDS in ascending order: a winner's place is the number of winners in the chunks and lanes before it
-    int32_t* win_id = reinterpret_cast<int32_t*>(mine);
-    float* win_s = reinterpret_cast<float*>(win_id + w.k);
-    if constexpr (WAVES > 1) {
+    template <int H>
+    __device__ __forceinline__ uint32_t choose_from_list(const int32_t* list, uint32_t n) {
+        K key[H];
+        float x[H];
+        int32_t id[H];
+        const double inverse_sum = SHARES && !sig() ? exact_inverse_sum() : 0.0;
 #pragma unroll
-        for (int q = 0; q < R / C; ++q) {
-            uint32_t here = 0;
-#pragma unroll
-            for (int j = 0; j < C; ++j) here += (uint32_t)__builtin_popcountll(__builtin_amdgcn_ballot_w64((won >> (q * C + j)) & 1u));
-            if (lane == 0) starts[q * WAVES + wave] = here;
-        }
-        __syncthreads();
-        if (threadIdx.x == 0) {
-            uint32_t at = 0;
-            for (int k = 0; k < WAVES * (R / C); ++k) {
-                const uint32_t n = starts[k];
-                starts[k] = at;
-                at += n;
+        for (int j = 0; j < H; ++j) {
+            const uint32_t i = j * 64 * WAVES + thread();
+            key[j] = (K)-INFINITY;
+            x[j] = -INFINITY;
+            id[j] = -1;
+            if (i < n) {
+                id[j] = list[i];
+                x[j] = to_f32(s_row[id[j]]) + 0.0f;   // -0 is 0
+                if constexpr (SHARES) key[j] = exact_key(x[j], (uint32_t)id[j], inverse_sum);
+                else key[j] = x[j];
             }
         }
-        __syncthreads();
+        return put_winners<H, 1>(key, [&](int j) { return id[j]; }, [&](int j) { return x[j]; });
     }
-    uint32_t base = 0;
+
+    // bisection over all keys
+    __device__ __forceinline__ uint32_t choose_among_all() {
+        K key[R];
+        const double inverse_sum = SHARES && !sig() ? exact_inverse_sum() : 0.0;
 #pragma unroll
-    for (int q = 0; q < R / C; ++q) {
-        uint32_t place = WAVES > 1 ? starts[q * WAVES + wave] : base;
-#pragma unroll
-        for (int j = 0; j < C; ++j) {
-            const unsigned long long m = __builtin_amdgcn_ballot_w64((won >> (q * C + j)) & 1u);
-            place += (uint32_t)__builtin_popcountll(m & ((1ull << lane) - 1ull));
-            base += (uint32_t)__builtin_popcountll(m);
+        for (int r = 0; r < R; ++r) {
+            if constexpr (SHARES) key[r] = L::id(r) < a.n_ids ? exact_key(s[r], L::id(r), inverse_sum) : -INFINITY;
+            else key[r] = s[r];
         }
-#pragma unroll
-        for (int j = 0; j < C; ++j)
-            if ((won >> (q * C + j)) & 1u) {
-                win_id[place] = (int32_t)L::id(q * C + j);
-                win_s[place] = s[q * C + j];
-                ++place;
-            }
+        if (a.w.groups > 1) keep_groups<K>(key, (K)0);
+        return put_winners<R, C>(key, [&](int r) { return (int32_t)L::id(r); }, [&](int r) { return s[r]; });
     }
-    sync();
+};
+
+template <int R, int WAVES, bool SHARES, typename T>
+__global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) void k_winners(WinnersArgs a, const T* __restrict__ scores,
+                                                                           int32_t* __restrict__ out_ids,
+                                                                           float* __restrict__ out_weights) {
+    extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
+    __shared__ double slots[2 * WAVES];
+    __shared__ uint32_t starts[WAVES == 1 ? 1 : WAVES * 8];
+    const uint32_t wave = threadIdx.x >> 6;
+    const uint64_t row = WAVES == 1 ? (uint64_t)blockIdx.x * 4 + wave : blockIdx.x;
+    if (row >= a.n_rows) return;
+    const sdrb_winners_spec& w = a.w;
+    Row<R, WAVES, SHARES, T> x{a, scores + row * a.ld, lds + (WAVES == 1 ? wave * a.lds_row : 0u), starts, {slots, 0}, {}, 0.0f, 0.0f};
+    const bool sig = x.sig();
+    read_row<R, WAVES>(x.s_row, a.n_ids, -INFINITY, x.s);
+#pragma unroll
+    for (int r = 0; r < R; ++r) x.s[r] = x.s[r] > -INFINITY ? x.s[r] + 0.0f : -INFINITY;   // NaN is no score; -0 is 0
+    if (!sig && (SHARES || !w.renormalise)) {   // a softmax over the row
+        float m = x.s[0], sum = 0.0f;
+#pragma unroll
+        for (int r = 1; r < R; ++r) m = max_of(m, x.s[r]);
+        x.top = x.meet.max(m);
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+            if (x.s[r] > -INFINITY) sum += exp_fast(below(x.s[r], x.top));
+        x.inv_sum = rcp_fast(x.meet.sum(sum));
+    }
+    uint32_t found;
+    if (!x.choose_among_candidates(found)) {
+        x.sync();
+        found = x.choose_among_all();
+    }
 
     // the weights, a winner a thread
-    const uint32_t thread = WAVES == 1 ? lane : threadIdx.x;
+    const uint32_t thread = x.thread();
+    const int32_t* win_id = x.win_ids();
+    const float* win_s = x.win_scores();
     float shift = 0.0f, norm = w.scale;
     if (w.renormalise) {
         float m = -INFINITY;
         for (uint32_t i = thread; i < found; i += 64 * WAVES) m = max_of(m, win_s[i]);
-        shift = meet.max(m);
+        shift = x.meet.max(m);
         if (sig) shift = shift < 0.0f ? shift : 0.0f;
         float sum = 0.0f;
         for (uint32_t i = thread; i < found; i += 64 * WAVES) sum += sig ? sigmoid_over(win_s[i], shift) : exp_fast(below(win_s[i], shift));
-        norm = w.scale * rcp_fast(meet.sum(sum));
+        norm = w.scale * rcp_fast(x.meet.sum(sum));
     }
     int32_t* ids = out_ids + row * w.k;
     float* weights = out_weights + row * w.k;
@@ -444,9 +630,9 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) void k_winners(Winne
         float weight = 0.0f;
         if (i < found) {
             id = win_id[i];
-            const float x = win_s[i];
-            if (sig) weight = norm * (w.renormalise ? sigmoid_over(x, shift) : sigmoid(x));
-            else weight = norm * (w.renormalise ? exp_fast(below(x, shift)) : exp_fast(below(x, top)) * inv_sum);
+            const float v = win_s[i];
+            if (sig) weight = norm * (w.renormalise ? sigmoid_over(v, shift) : sigmoid(v));
+            else weight = norm * (w.renormalise ? exp_fast(below(v, shift)) : exp_fast(below(v, x.top)) * x.inv_sum);
         }
         ids[i] = id;
         weights[i] = weight;
@@ -630,6 +816,7 @@ int launch_winners(const sdrb_dense& scores, const sdrb_winners_spec& spec, int3
     a.ld = scores.ld;
     a.n_ids = (uint32_t)scores.n_cols;
     a.group_size = a.n_ids / spec.groups;
+    a.group_magic = ((1u << 31) + a.group_size - 1) / a.group_size;   // exact for ids below 2^17
     const bool shares = spec.bias || (spec.groups > 1 && spec.group_top > 1);
     return with_layout(a.n_ids, [&](auto r, auto waves) {
         constexpr int R = decltype(r)::value, WAVES = decltype(waves)::value;
@@ -637,20 +824,22 @@ int launch_winners(const sdrb_dense& scores, const sdrb_winners_spec& spec, int3
         while (a.group_lanes_log2 < 6 && (spec.groups << (a.group_lanes_log2 + 1)) <= 64u * WAVES) ++a.group_lanes_log2;
         return with_type(scores.type, [&](auto t) {
             using T = decltype(t);
-            const auto go = [&](auto k) {
-                using K = decltype(k);
-                const size_t grouped = spec.groups > 1 ? (size_t)(a.n_ids + spec.groups) * sizeof(K) + kWinnersMaxGroups / 8 : 0;
-                const size_t listed = (size_t)spec.k * 8;
+            const auto go = [&](auto s) {
+                constexpr bool SHARES = decltype(s)::value;
+                const size_t of_key = SHARES ? sizeof(double) : sizeof(float);
+                const size_t grouped = spec.groups > 1 ? (a.n_ids + spec.groups) * of_key + kWinnersMaxGroups / 8 : 0;
+                const size_t held = (a.n_ids < 64u * WAVES * kHeld ? a.n_ids : 64u * WAVES * kHeld) * sizeof(int32_t);
+                const size_t listed = spec.k * 8 > held ? spec.k * 8 : held;
                 a.lds_row = (uint32_t)(((grouped > listed ? grouped : listed) + 15) / 16 * 16);
                 const size_t lds = (size_t)a.lds_row * (WAVES == 1 ? 4 : 1);
                 const uint64_t blocks = WAVES == 1 ? (a.n_rows + 3) / 4 : a.n_rows;
-                if (const int rc = allow_lds(&k_winners<R, WAVES, K, T>, lds)) return rc;
-                hipLaunchKernelGGL((k_winners<R, WAVES, K, T>), dim3((uint32_t)blocks), dim3(WAVES == 1 ? 256 : 64 * WAVES), lds, stream, a,
-                                   static_cast<const T*>(scores.data), ids, weights);
+                if (const int rc = allow_lds(&k_winners<R, WAVES, SHARES, T>, lds)) return rc;
+                hipLaunchKernelGGL((k_winners<R, WAVES, SHARES, T>), dim3((uint32_t)blocks), dim3(WAVES == 1 ? 256 : 64 * WAVES), lds,
+                                   stream, a, static_cast<const T*>(scores.data), ids, weights);
                 SDRB_HIP(hipGetLastError());
                 return SDRB_OK;
             };
-            return shares ? go(double{}) : go(float{});
+            return shares ? go(std::true_type{}) : go(std::false_type{});
         });
     });
 }
