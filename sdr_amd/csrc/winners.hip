@@ -17,7 +17,7 @@
 //     at or above the middle.
 // Shares that enter keys are computed in binary64 in the second step: whether an id wins hangs on the difference of two keys,
 // which binary32 exponentials would decide by their own error.  Rows whose candidates are too many (many equal scores, a k
-// near the number of threads) or whose groups cannot be told apart in binary32 bisect over all their keys instead.
+// near the number of threads) bisect over all their keys instead; groups that binary32 does not tell apart are scored again.
 // Bound: instruction issue, not memory.
 #include <type_traits>
 
@@ -82,6 +82,9 @@ __device__ __forceinline__ float key_at(uint32_t order) {
     return __builtin_bit_cast(float, order & 0x80000000u ? order & 0x7FFFFFFFu : ~order);
 }
 constexpr uint32_t kOrderOfNone = 0x007FFFFFu;   // of -inf
+// Low bits of a score's order that its type leaves alike: a bisection stops short of them.
+template <typename T>
+constexpr int kAlike = std::is_same_v<T, bf16> ? 16 : std::is_same_v<T, f16> ? 13 : 0;
 
 // ---- the threads of a row: 16 lanes, a wave, or eight waves that meet in LDS ----
 template <int THREADS>
@@ -227,12 +230,12 @@ __device__ __forceinline__ void read_row(const T* __restrict__ row, uint32_t n, 
         for (int j = 0; j < L::C; ++j) v[q * L::C + j] = part[j];
     }
 }
-// scores: a NaN is none; -0 is 0
+// scores: a NaN is none (the maximum of it and -inf is -inf); -0 is 0
 template <int R, int THREADS, typename T>
 __device__ __forceinline__ void read_scores(const T* __restrict__ row, uint32_t n, float (&v)[R]) {
     read_row<R, THREADS>(row, n, -INFINITY, v);
 #pragma unroll
-    for (int r = 0; r < R; ++r) v[r] = v[r] > -INFINITY ? v[r] + 0.0f : -INFINITY;
+    for (int r = 0; r < R; ++r) v[r] = fmaxf(v[r] + 0.0f, -INFINITY);
 }
 
 // Selects the k largest orders above `none`, the lowest places first among equal ones: won has bit r for register r.
@@ -280,6 +283,18 @@ __device__ __forceinline__ uint32_t select_largest(const U (&key)[R], U none, ui
     for (int r = 0; r < R; ++r)
         if (key[r] == lo && place[r / C]++ >= room) won &= ~(1u << r);
     return k;
+}
+
+// The same for one key a lane of a row of 16: a key's rank is the number of keys before it, met by turning the row 15 times.
+template <int N>
+__device__ __forceinline__ uint32_t ranked_before(uint64_t key, uint32_t thread) {
+    if constexpr (N == 0) {
+        return 0;
+    } else {
+        const uint32_t lo = dpp<0x120 + N, 0xF>(0u, (uint32_t)key), hi = dpp<0x120 + N, 0xF>(0u, (uint32_t)(key >> 32));
+        const uint64_t other = ((uint64_t)hi << 32) | lo;   // of the lane N below, or 16 - N above
+        return ranked_before<N - 1>(key, thread) + (other > key || (other == key && thread >= (uint32_t)N) ? 1u : 0u);
+    }
 }
 
 // v_exp_f32 and v_rcp_f32 are within a step of their value; arguments are rounded once more on the way to base 2
@@ -337,7 +352,7 @@ struct WinnersArgs {
 };
 
 // Candidates a thread takes at most; a threshold is looked for where k is at most three quarters of the threads.
-constexpr int kHeld = 4;
+constexpr int kHeld = 2;
 template <int THREADS>
 constexpr uint32_t kMostByThreshold = THREADS * 3 / 4;
 
@@ -349,6 +364,7 @@ struct Row {
     using K = std::conditional_t<SHARES, double, float>;
     using U = std::conditional_t<SHARES, uint64_t, uint32_t>;
     static constexpr int C = L::C, Q = R / C;
+    static constexpr int kDrop = SHARES ? 0 : kAlike<T>;
 
     const WinnersArgs& a;
     const T* s_row;
@@ -369,75 +385,160 @@ struct Row {
         return x > -INFINITY && key > -INFINITY ? key + 0.0 : -INFINITY;   // (a NaN of the bias is no key; -0 is 0)
     }
 
-    // keys outside the best groups become -inf; false where slack > 0 and binary32 keys do not tell the groups apart.  slack:
-    // how far a key may be off, beside its own rounding
+    // Which of a thread's keys lie in the best groups, a bit a register.  sure: false where slack > 0 and keys that are off by
+    // slack, beside their own rounding, do not tell the groups apart.
     template <typename F>
-    __device__ __forceinline__ bool keep_groups(F (&key)[R], F slack) {
+    __device__ __forceinline__ uint32_t in_best_groups(const F (&key)[R], F slack, bool& sure) {
+        if constexpr (C == 8) {
+            const uint32_t span = a.group_size / 8;
+            if (a.group_size % 8 == 0 && (span & (span - 1)) == 0 && span <= (uint32_t)Team<THREADS>::kLanes)
+                return in_best_groups_by_lanes(key, slack, span, sure);
+        }
+        return in_best_groups_by_lds(key, slack, sure);
+    }
+    // size: the largest sum of sizes of summed keys; worst and lost: the lowest score that is kept and the highest that is not
+    template <typename F>
+    __device__ __forceinline__ bool told_apart(F size, F worst, F lost, F slack) {
+        size = team.max(size);
+        worst = -team.max(-worst);
+        lost = team.max(lost);
+        // two sums, of two keys each: every one off by slack, and by three roundings of half a step of at most `size`
+        return !(lost > (F)-INFINITY) || worst - lost > 4 * slack + size * (F)0x1p-21;
+    }
+    // Groups of 8 * span ids, span a power of two up to the lanes of the team: each lies in one chunk, with whole registers of
+    // `span` neighbouring lanes.
+    template <typename F>
+    __device__ __forceinline__ uint32_t in_best_groups_by_lanes(const F (&key)[R], F slack, uint32_t span, bool& sure) {
+        const sdrb_winners_spec& w = a.w;
+        const uint32_t per_chunk = THREADS / span, own = thread() / span;
+        F* group = reinterpret_cast<F*>(mine);   // [groups, rounded up to 4]
+        F score[Q], size = 0;
+        uint32_t before[Q];
+        for (uint32_t g = w.groups + thread(); g < (w.groups + 3) / 4 * 4; g += THREADS) group[g] = (F)-INFINITY;
+#pragma unroll
+        for (int q = 0; q < Q; ++q) {
+            F best = key[q * C], next = (F)-INFINITY;
+            const auto meet = [&](F b, F n) {
+                next = fmax(fmin(best, b), fmax(next, n));
+                best = fmax(best, b);
+            };
+#pragma unroll
+            for (int j = 1; j < C; ++j) {
+                next = fmax(next, fmin(best, key[q * C + j]));
+                best = fmax(best, key[q * C + j]);
+            }
+            if (span >= 2) meet(dpp<0xB1, 0xF>(best, best), dpp<0xB1, 0xF>(next, next));
+            if (span >= 4) meet(dpp<0x4E, 0xF>(best, best), dpp<0x4E, 0xF>(next, next));
+            if (span >= 8) meet(dpp<0x141, 0xF>(best, best), dpp<0x141, 0xF>(next, next));
+            if (span >= 16) meet(dpp<0x140, 0xF>(best, best), dpp<0x140, 0xF>(next, next));
+            if constexpr (THREADS >= 64) {
+                if (span >= 32) meet(__shfl_xor(best, 16, 64), __shfl_xor(next, 16, 64));
+                if (span >= 64) meet(__shfl_xor(best, 32, 64), __shfl_xor(next, 32, 64));
+            }
+            const bool two = w.group_top > 1 && next > (F)-INFINITY;
+            score[q] = two ? best + next : best;
+            if (best > (F)-INFINITY) size = fmax(size, fabs(best) + (two ? fabs(next) : (F)0));
+            const uint32_t g = q * per_chunk + own;
+            if ((thread() & (span - 1)) == 0 && g < w.groups) group[g] = score[q];
+            before[q] = 0;
+        }
+        team.sync();
+        for (uint32_t o = 0; o < w.groups; o += 4) {
+            F other[4];
+            __builtin_memcpy(other, group + o, sizeof other);
+#pragma unroll
+            for (int q = 0; q < Q; ++q)
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    before[q] += other[j] > score[q] || (other[j] == score[q] && o + j < q * per_chunk + own) ? 1u : 0u;
+        }
+        F worst = (F)INFINITY, lost = (F)-INFINITY;
+        uint32_t kept = 0;
+#pragma unroll
+        for (int q = 0; q < Q; ++q) {
+            const bool in = score[q] > (F)-INFINITY && before[q] < w.top_groups;
+            if (in) worst = fmin(worst, score[q]);
+            else lost = fmax(lost, score[q]);
+            kept |= in ? 0xFFu << (q * C) : 0u;
+        }
+        team.sync();
+        sure = !(slack > (F)0) || told_apart(size, worst, lost, slack);
+        return kept;
+    }
+    // Any groups: the keys are laid into LDS, and 2^group_lanes_log2 threads look through a group.
+    template <typename F>
+    __device__ __forceinline__ uint32_t in_best_groups_by_lds(const F (&key)[R], F slack, bool& sure) {
         const sdrb_winners_spec& w = a.w;
         F* keys = reinterpret_cast<F*>(mine);
-        F* group = keys + a.n_ids;                                             // [groups]
-        unsigned char* kept = reinterpret_cast<unsigned char*>(group + w.groups);   // [groups]
+        F* group = keys + a.n_ids;                                                  // [groups]
+        unsigned char* best_ones = reinterpret_cast<unsigned char*>(group + w.groups);   // [groups]
 #pragma unroll
         for (int r = 0; r < R; ++r)
             if (L::id(r) < a.n_ids) keys[L::id(r)] = key[r];
         team.sync();
-        // a group's one or two largest keys, by 2^group_lanes_log2 threads a group
         const uint32_t lanes = 1u << a.group_lanes_log2;
-        F size = (F)0;   // of the keys that are summed
+        F size = 0;
         for (uint32_t g0 = 0; g0 < w.groups; g0 += THREADS >> a.group_lanes_log2) {
             const uint32_t g = g0 + (thread() >> a.group_lanes_log2);
             F best = (F)-INFINITY, next = (F)-INFINITY;
             if (g < w.groups)
                 for (uint32_t e = thread() & (lanes - 1); e < a.group_size; e += lanes) {
                     const F k = keys[g * a.group_size + e];
-                    next = k > best ? best : (k > next ? k : next);
-                    best = max_of(best, k);
+                    next = fmax(next, fmin(best, k));
+                    best = fmax(best, k);
                 }
             for (uint32_t d = 1; d < lanes; d <<= 1) {
                 const F b = __shfl_xor(best, (int)d, 64), n = __shfl_xor(next, (int)d, 64);
-                next = b > best ? max_of(best, n) : max_of(next, b);
-                best = max_of(best, b);
+                next = fmax(fmin(best, b), fmax(next, n));
+                best = fmax(best, b);
             }
             const bool two = w.group_top > 1 && next > (F)-INFINITY;
             if (g < w.groups && (thread() & (lanes - 1)) == 0) group[g] = two ? best + next : best;
-            if (best > (F)-INFINITY) size = max_of(size, (best < 0 ? -best : best) + (two ? (next < 0 ? -next : next) : (F)0));
+            if (best > (F)-INFINITY) size = fmax(size, fabs(best) + (two ? fabs(next) : (F)0));
         }
         team.sync();
-        // a group is kept if fewer than top_groups groups stand before it
+        // a group is one of the best if fewer than top_groups stand before it
         F worst = (F)INFINITY, lost = (F)-INFINITY;
         for (uint32_t g = thread(); g < w.groups; g += THREADS) {
             const F score = group[g];
             uint32_t before = 0;
             for (uint32_t o = 0; o < w.groups; ++o) before += group[o] > score || (group[o] == score && o < g) ? 1u : 0u;
             const bool in = score > (F)-INFINITY && before < w.top_groups;
-            kept[g] = in ? 1 : 0;
-            if (in) worst = score < worst ? score : worst;
-            else lost = max_of(lost, score);
+            best_ones[g] = in ? 1 : 0;
+            if (in) worst = fmin(worst, score);
+            else lost = fmax(lost, score);
         }
-        bool sure = true;
-        if (slack > (F)0) {
-            size = team.max(size);
-            worst = -team.max(-worst);
-            lost = team.max(lost);
-            // two sums, of two keys each: every one off by slack and three roundings of at most `size`
-            sure = !(lost > (F)-INFINITY) || worst - lost > 4 * slack + size * (F)0x1p-20;
-        }
+        sure = !(slack > (F)0) || told_apart(size, worst, lost, slack);
         team.sync();
+        uint32_t kept = 0;
 #pragma unroll
         for (int r = 0; r < R; ++r) {
-            const uint32_t g = __umulhi(2 * L::id(r), a.group_magic);   // (ids beyond the row have no key)
-            if (key[r] > (F)-INFINITY && !kept[g]) key[r] = (F)-INFINITY;
+            const uint32_t g = __umulhi(2 * L::id(r), a.group_magic);
+            if (L::id(r) < a.n_ids && best_ones[g]) kept |= 1u << r;
         }
         team.sync();
-        return sure;
+        return kept;
+    }
+    __device__ __forceinline__ void exact_keys(const float (&s)[R], K (&exact)[R]) const {
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            if constexpr (SHARES) exact[r] = L::id(r) < a.n_ids ? exact_key(s[r], L::id(r)) : (double)-INFINITY;
+            else exact[r] = s[r];
+        }
     }
 
     // the winners among keys that the threads hold CH at a time, to LDS
     template <int H, int CH, typename F, typename G>
     __device__ __forceinline__ uint32_t put_winners(const U (&key)[H], F id_of, G score_of) {
         uint32_t won, here[H / CH], place[H / CH];
-        const U none = order_of((K)-INFINITY);
-        const uint32_t found = select_largest<H, CH, THREADS>(key, none, a.w.k, team, won);
+        const U none = order_of((K)-INFINITY) >> kDrop;
+        uint32_t found;
+        if constexpr (H == 1 && THREADS == 16) {
+            won = key[0] > none && ranked_before<15>(key[0], thread()) < a.w.k ? 1u : 0u;
+            found = team.count(won != 0);
+        } else {
+            found = select_largest<H, CH, THREADS>(key, none, a.w.k, team, won);
+        }
 #pragma unroll
         for (int q = 0; q < H / CH; ++q) here[q] = __popc((won >> (q * CH)) & (uint32_t)((1ull << CH) - 1));
         team.places(here, place);
@@ -466,38 +567,52 @@ struct Row {
 #pragma unroll
             for (int r = 0; r < R; ++r) {
                 float k = sig() ? sigmoid(key[r]) : exp_fast(below(key[r], top)) * inv_sum;
-                if (w.bias) k += b[r];
-                key[r] = key[r] > -INFINITY && k > -INFINITY ? k : -INFINITY;
+                if (w.bias) k = fmaxf(k + b[r], -INFINITY);
+                key[r] = key[r] > -INFINITY ? k : -INFINITY;
             }
         }
-        if (w.groups > 1 && !keep_groups<float>(key, slack)) return false;
+        if (w.groups > 1) {
+            bool sure;
+            uint32_t kept = in_best_groups<float>(key, slack, sure);
+            if constexpr (SHARES) {
+                if (!sure) {   // the groups by exact keys
+                    float s[R];
+                    K exact[R];
+                    read_scores<R, THREADS>(s_row, a.n_ids, s);
+                    exact_keys(s, exact);
+                    kept = in_best_groups<K>(exact, (K)0, sure);
+                }
+            }
+#pragma unroll
+            for (int r = 0; r < R; ++r) key[r] = (kept >> r) & 1u ? key[r] : -INFINITY;
+        }
 
         float top_key = key[0];
 #pragma unroll
         for (int r = 1; r < R; ++r) top_key = fmaxf(top_key, key[r]);
-        const uint32_t top_order = order_of(top_key);
+        const uint32_t top_order = order_of(top_key) >> kDrop, none = kOrderOfNone >> kDrop;
         float t = -INFINITY;
-        if (team.count(top_order > kOrderOfNone) >= w.k) {
-            uint32_t lo = team.min(top_order > kOrderOfNone ? top_order : 0xFFFFFFFFu), hi = team.max(top_order) + 1;
-            const uint32_t enough = w.k + w.k / 8 + 1;
-            uint32_t done = 0;
-            while (hi - lo > 1 && !done) {
-                const uint32_t mid = lo + (hi - lo) / 2, c = team.count(top_order >= mid);
+        if (team.count(top_order > none) >= w.k) {
+            uint32_t lo = team.min(top_order > none ? top_order : 0xFFFFFFFFu), hi = team.max(top_order) + 1;
+            uint32_t c = 0;
+            while (hi - lo > 1 && c != w.k) {
+                const uint32_t mid = lo + (hi - lo) / 2;
+                c = team.count(top_order >= mid);
                 if (c >= w.k) lo = mid;
                 else hi = mid;
-                done = c >= w.k && c <= enough;
             }
-            t = key_at(lo);
+            t = key_at(lo << kDrop);
             // k keys are no smaller than t less what a key can be off; a key as large may seem smaller by as much again
-            if (SHARES) t -= 2.0f * slack + fabsf(t) * 0x1p-21f;   // (an infinite t becomes NaN, which nothing reaches)
+            if (SHARES) t -= 2.0f * slack + fabsf(t) * 0x1p-21f;
         }
+        t = fmaxf(t, -3.402823466e38f);   // (every key > -inf; an infinite t has become a NaN, and all are candidates)
         uint32_t bits = 0, here[Q], place[Q];
 #pragma unroll
-        for (int r = 0; r < R; ++r) bits |= key[r] >= t && key[r] > -INFINITY ? 1u << r : 0u;
+        for (int r = 0; r < R; ++r) bits |= key[r] >= t ? 1u << r : 0u;
 #pragma unroll
         for (int q = 0; q < Q; ++q) here[q] = __popc((bits >> (q * C)) & ((1u << C) - 1u));
         const uint32_t n = team.places(here, place);
-        if (n > (uint32_t)THREADS * kHeld || (n < w.k && t != -INFINITY)) return false;
+        if (n > (uint32_t)THREADS * kHeld) return false;
         int32_t* list = reinterpret_cast<int32_t*>(mine);
 #pragma unroll
         for (int q = 0; q < Q; ++q) {
@@ -526,7 +641,7 @@ struct Row {
                 id[j] = list[i];
                 x[j] = to_f32(s_row[id[j]]) + 0.0f;   // -0 is 0
                 if constexpr (SHARES) key[j] = order_of(exact_key(x[j], (uint32_t)id[j]));
-                else key[j] = order_of(x[j]);
+                else key[j] = order_of(x[j]) >> kDrop;
             }
         }
         team.sync();   // the list has been read: winners are put in its place
@@ -538,15 +653,13 @@ struct Row {
         float s[R];
         read_scores<R, THREADS>(s_row, a.n_ids, s);
         K exact[R];
-#pragma unroll
-        for (int r = 0; r < R; ++r) {
-            if constexpr (SHARES) exact[r] = L::id(r) < a.n_ids ? exact_key(s[r], L::id(r)) : (double)-INFINITY;
-            else exact[r] = s[r];
-        }
-        if (a.w.groups > 1) keep_groups<K>(exact, (K)0);
+        exact_keys(s, exact);
+        uint32_t kept = ~0u;
+        bool sure;
+        if (a.w.groups > 1) kept = in_best_groups<K>(exact, (K)0, sure);
         U key[R];
 #pragma unroll
-        for (int r = 0; r < R; ++r) key[r] = order_of(exact[r]);
+        for (int r = 0; r < R; ++r) key[r] = (kept >> r) & 1u ? order_of(exact[r]) >> kDrop : 0;
         return put_winners<R, C>(key, [&](int r) { return (int32_t)L::id(r); }, [&](int r) { return s[r]; });
     }
 };
