@@ -9,15 +9,18 @@
 // A team of threads owns a row and holds its scores in registers, read once: 64 threads, 512 for more than 2048 ids, or 16
 // where there are many short rows (four rows a wave: what a team does once, it does for four rows at a time).  Two steps
 // choose the winners:
-//  1. Candidates.  Of the threads' largest keys a threshold is found that k of them reach (a compare and a count a step), so
-//     at least k keys reach it, and few more: about 62 of 2048 for k = 40.  Keys are binary32 here; where shares enter them
-//     the threshold is lowered by what their arithmetic can be off, so that no winner is lost.
+//  1. Candidates.  Of the threads' largest keys -- two a thread, each of half its registers -- a threshold is found that k of
+//     them reach (a compare and a count a step), so at least k keys reach it, and few more: about 47 of 2048 for k = 40.  Keys
+//     are binary32 here; where shares enter them the threshold is lowered by what their arithmetic can be off, so that no
+//     winner is lost.
 //  2. The candidates' ids go to LDS in ascending order, one a thread from there on; their keys are computed exactly, and the
 //     k-th largest is found by bisection over the keys' order-preserving integers, which ends as soon as exactly k keys lie
 //     at or above the middle.
 // Shares that enter keys are computed in binary64 in the second step: whether an id wins hangs on the difference of two keys,
-// which binary32 exponentials would decide by their own error.  Rows whose candidates are too many (many equal scores, a k
-// near the number of threads) bisect over all their keys instead; groups that binary32 does not tell apart are scored again.
+// which binary32 exponentials would decide by their own error.  Groups that binary32 does not tell apart are scored again
+// exactly; rows whose candidates are too many (many equal scores, or a k above the number of threads) bisect over all their
+// keys.  Both are rolled loops that read the row anew: what runs rarely has to be short, since fetching instructions that no
+// other wave has run costs more than running them (straight-line code of 900 instructions: 15 us).
 // Bound: instruction issue, not memory.
 #include <type_traits>
 
@@ -348,13 +351,15 @@ struct WinnersArgs {
     uint32_t n_ids;
     uint32_t group_size, group_lanes_log2;   // ids of a group; lanes that look at one group together
     uint32_t group_magic;                    // id * group_magic >> 31 is the id's group
+    uint32_t lds_groups;                     // where a row's LDS holds its groups, behind its winners and keys
     uint32_t lds_row;                        // bytes of dynamic LDS a row has
 };
 
-// Candidates a thread takes at most; a threshold is looked for where k is at most three quarters of the threads.
-constexpr int kHeld = 2;
+constexpr int kHeld = 2;   // candidates a thread takes at most
+// The k for which a threshold leaves few enough candidates: with 2 * THREADS largest keys, half of them at most.  Rows of no more
+// ids than the threads hold need none.
 template <int THREADS>
-constexpr uint32_t kMostByThreshold = THREADS * 3 / 4;
+constexpr uint32_t kMostByThreshold = THREADS;
 
 // A row of scores and the steps that choose its winners.  SHARES: keys are shares (+ bias), exactly so in binary64; else the
 // scores.
@@ -385,16 +390,27 @@ struct Row {
         return x > -INFINITY && key > -INFINITY ? key + 0.0 : -INFINITY;   // (a NaN of the bias is no key; -0 is 0)
     }
 
-    // Which of a thread's keys lie in the best groups, a bit a register.  sure: false where slack > 0 and keys that are off by
-    // slack, beside their own rounding, do not tell the groups apart.
-    template <typename F>
-    __device__ __forceinline__ uint32_t in_best_groups(const F (&key)[R], F slack, bool& sure) {
+    // Which of a thread's keys lie in the best groups, a bit a register.  slack: how far a key may be off, beside its own
+    // rounding; where that does not tell the groups apart, they are scored by exact keys.
+    __device__ __forceinline__ uint32_t in_best_groups(const float (&key)[R], float slack) {
+        bool sure;
         if constexpr (C == 8) {
             const uint32_t span = a.group_size / 8;
-            if (a.group_size % 8 == 0 && (span & (span - 1)) == 0 && span <= (uint32_t)Team<THREADS>::kLanes)
-                return in_best_groups_by_lanes(key, slack, span, sure);
+            if (a.group_size % 8 == 0 && (span & (span - 1)) == 0 && span <= (uint32_t)Team<THREADS>::kLanes) {
+                const uint32_t kept = in_best_groups_by_lanes(key, slack, span, sure);
+                if (sure) return kept;
+                find_best_groups<K>([&](uint32_t id) { return exact_key_of(id); }, (K)0, sure);
+                return kept_of_best_ones();
+            }
         }
-        return in_best_groups_by_lds(key, slack, sure);
+        float* keys = reinterpret_cast<float*>(mine);
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+            if (L::id(r) < a.n_ids) keys[L::id(r)] = key[r];
+        team.sync();
+        find_best_groups<float>([&](uint32_t id) { return keys[id]; }, slack, sure);
+        if (!sure) find_best_groups<K>([&](uint32_t id) { return exact_key_of(id); }, (K)0, sure);
+        return kept_of_best_ones();
     }
     // size: the largest sum of sizes of summed keys; worst and lost: the lowest score that is kept and the highest that is not
     template <typename F>
@@ -407,8 +423,8 @@ struct Row {
     }
     // Groups of 8 * span ids, span a power of two up to the lanes of the team: each lies in one chunk, with whole registers of
     // `span` neighbouring lanes.
-    template <typename F>
-    __device__ __forceinline__ uint32_t in_best_groups_by_lanes(const F (&key)[R], F slack, uint32_t span, bool& sure) {
+    __device__ __forceinline__ uint32_t in_best_groups_by_lanes(const float (&key)[R], float slack, uint32_t span, bool& sure) {
+        using F = float;
         const sdrb_winners_spec& w = a.w;
         const uint32_t per_chunk = THREADS / span, own = thread() / span;
         F* group = reinterpret_cast<F*>(mine);   // [groups, rounded up to 4]
@@ -465,28 +481,26 @@ struct Row {
         sure = !(slack > (F)0) || told_apart(size, worst, lost, slack);
         return kept;
     }
-    // Any groups: the keys are laid into LDS, and 2^group_lanes_log2 threads look through a group.
-    template <typename F>
-    __device__ __forceinline__ uint32_t in_best_groups_by_lds(const F (&key)[R], F slack, bool& sure) {
+    // Any groups: 2^group_lanes_log2 threads look through a group; key_of(id) is called in a rolled loop.  A byte a group is left
+    // in LDS: best_ones().
+    __device__ __forceinline__ unsigned char* best_ones() const { return mine + a.lds_groups; }
+    template <typename F, typename G>
+    __device__ __forceinline__ void find_best_groups(G key_of, F slack, bool& sure) {
         const sdrb_winners_spec& w = a.w;
-        F* keys = reinterpret_cast<F*>(mine);
-        F* group = keys + a.n_ids;                                                  // [groups]
-        unsigned char* best_ones = reinterpret_cast<unsigned char*>(group + w.groups);   // [groups]
-#pragma unroll
-        for (int r = 0; r < R; ++r)
-            if (L::id(r) < a.n_ids) keys[L::id(r)] = key[r];
-        team.sync();
+        F* group = reinterpret_cast<F*>(best_ones() + kWinnersMaxGroups);   // [groups]
         const uint32_t lanes = 1u << a.group_lanes_log2;
         F size = 0;
         for (uint32_t g0 = 0; g0 < w.groups; g0 += THREADS >> a.group_lanes_log2) {
             const uint32_t g = g0 + (thread() >> a.group_lanes_log2);
             F best = (F)-INFINITY, next = (F)-INFINITY;
             if (g < w.groups)
+#pragma unroll 1
                 for (uint32_t e = thread() & (lanes - 1); e < a.group_size; e += lanes) {
-                    const F k = keys[g * a.group_size + e];
+                    const F k = key_of(g * a.group_size + e);
                     next = fmax(next, fmin(best, k));
                     best = fmax(best, k);
                 }
+#pragma unroll 1
             for (uint32_t d = 1; d < lanes; d <<= 1) {
                 const F b = __shfl_xor(best, (int)d, 64), n = __shfl_xor(next, (int)d, 64);
                 next = fmax(fmin(best, b), fmax(next, n));
@@ -499,32 +513,33 @@ struct Row {
         team.sync();
         // a group is one of the best if fewer than top_groups stand before it
         F worst = (F)INFINITY, lost = (F)-INFINITY;
+#pragma unroll 1
         for (uint32_t g = thread(); g < w.groups; g += THREADS) {
             const F score = group[g];
             uint32_t before = 0;
+#pragma unroll 1
             for (uint32_t o = 0; o < w.groups; ++o) before += group[o] > score || (group[o] == score && o < g) ? 1u : 0u;
             const bool in = score > (F)-INFINITY && before < w.top_groups;
-            best_ones[g] = in ? 1 : 0;
+            best_ones()[g] = in ? 1 : 0;
             if (in) worst = fmin(worst, score);
             else lost = fmax(lost, score);
         }
         sure = !(slack > (F)0) || told_apart(size, worst, lost, slack);
         team.sync();
+    }
+    __device__ __forceinline__ uint32_t kept_of_best_ones() const {
         uint32_t kept = 0;
 #pragma unroll
         for (int r = 0; r < R; ++r) {
             const uint32_t g = __umulhi(2 * L::id(r), a.group_magic);
-            if (L::id(r) < a.n_ids && best_ones[g]) kept |= 1u << r;
+            if (L::id(r) < a.n_ids && best_ones()[g]) kept |= 1u << r;
         }
-        team.sync();
         return kept;
     }
-    __device__ __forceinline__ void exact_keys(const float (&s)[R], K (&exact)[R]) const {
-#pragma unroll
-        for (int r = 0; r < R; ++r) {
-            if constexpr (SHARES) exact[r] = L::id(r) < a.n_ids ? exact_key(s[r], L::id(r)) : (double)-INFINITY;
-            else exact[r] = s[r];
-        }
+    __device__ __forceinline__ float score_of(uint32_t id) const { return fmaxf(to_f32(s_row[id]) + 0.0f, -INFINITY); }
+    __device__ __forceinline__ K exact_key_of(uint32_t id) const {
+        if constexpr (SHARES) return exact_key(score_of(id), id);
+        else return score_of(id);
     }
 
     // the winners among keys that the threads hold CH at a time, to LDS
@@ -555,7 +570,7 @@ struct Row {
     // the candidates that a threshold leaves, and the winners among them; false where the row needs choose_among_all
     __device__ __forceinline__ bool choose_among_candidates(float (&key)[R], uint32_t& found) {
         const sdrb_winners_spec& w = a.w;
-        if (w.k > kMostByThreshold<THREADS>) return false;
+        if (w.k > kMostByThreshold<THREADS> && a.n_ids > (uint32_t)THREADS * kHeld) return false;
         float slack = 0.0f;
         if constexpr (SHARES) {
             // Off by less than 3.1 * 2^-24 for the sigmoid -- 1.5 |x| + 2 steps in its exponential t, which enter the result
@@ -572,32 +587,35 @@ struct Row {
             }
         }
         if (w.groups > 1) {
-            bool sure;
-            uint32_t kept = in_best_groups<float>(key, slack, sure);
-            if constexpr (SHARES) {
-                if (!sure) {   // the groups by exact keys
-                    float s[R];
-                    K exact[R];
-                    read_scores<R, THREADS>(s_row, a.n_ids, s);
-                    exact_keys(s, exact);
-                    kept = in_best_groups<K>(exact, (K)0, sure);
-                }
-            }
+            const uint32_t kept = in_best_groups(key, slack);
 #pragma unroll
             for (int r = 0; r < R; ++r) key[r] = (kept >> r) & 1u ? key[r] : -INFINITY;
+            team.sync();
         }
 
-        float top_key = key[0];
+        constexpr int kTops = R > 1 ? 2 : 1;
+        uint32_t tops[kTops];
 #pragma unroll
-        for (int r = 1; r < R; ++r) top_key = fmaxf(top_key, key[r]);
-        const uint32_t top_order = order_of(top_key) >> kDrop, none = kOrderOfNone >> kDrop;
+        for (int h = 0; h < kTops; ++h) {
+            float most = key[h * (R / kTops)];
+#pragma unroll
+            for (int r = 1; r < R / kTops; ++r) most = fmaxf(most, key[h * (R / kTops) + r]);
+            tops[h] = order_of(most) >> kDrop;
+        }
+        constexpr uint32_t none = kOrderOfNone >> kDrop;
         float t = -INFINITY;
-        if (team.count(top_order > none) >= w.k) {
-            uint32_t lo = team.min(top_order > none ? top_order : 0xFFFFFFFFu), hi = team.max(top_order) + 1;
+        if (w.k <= kMostByThreshold<THREADS> && team.template count_all<kTops>([&](int h) { return tops[h] > none; }) >= w.k) {
+            uint32_t least = 0xFFFFFFFFu, most = 0;
+#pragma unroll
+            for (int h = 0; h < kTops; ++h) {
+                least = tops[h] > none && tops[h] < least ? tops[h] : least;
+                most = max_u32(most, tops[h]);
+            }
+            uint32_t lo = team.min(least), hi = team.max(most) + 1;
             uint32_t c = 0;
             while (hi - lo > 1 && c != w.k) {
                 const uint32_t mid = lo + (hi - lo) / 2;
-                c = team.count(top_order >= mid);
+                c = team.template count_all<kTops>([&](int h) { return tops[h] >= mid; });
                 if (c >= w.k) lo = mid;
                 else hi = mid;
             }
@@ -648,19 +666,60 @@ struct Row {
         return put_winners<H, 1>(key, [&](int j) { return id[j]; }, [&](int j) { return x[j]; });
     }
 
-    // bisection over all keys, from the scores anew
+    // bisection over all keys, computed anew in every step
     __device__ __forceinline__ uint32_t choose_among_all() {
-        float s[R];
-        read_scores<R, THREADS>(s_row, a.n_ids, s);
-        K exact[R];
-        exact_keys(s, exact);
-        uint32_t kept = ~0u;
+        const sdrb_winners_spec& w = a.w;
         bool sure;
-        if (a.w.groups > 1) kept = in_best_groups<K>(exact, (K)0, sure);
-        U key[R];
-#pragma unroll
-        for (int r = 0; r < R; ++r) key[r] = (kept >> r) & 1u ? order_of(exact[r]) >> kDrop : 0;
-        return put_winners<R, C>(key, [&](int r) { return (int32_t)L::id(r); }, [&](int r) { return s[r]; });
+        if (w.groups > 1) find_best_groups<K>([&](uint32_t id) { return exact_key_of(id); }, (K)0, sure);
+        const U none = order_of((K)-INFINITY) >> kDrop;
+        const auto order_at = [&](uint32_t id) {
+            if (w.groups > 1 && !best_ones()[__umulhi(2 * id, a.group_magic)]) return (U)0;
+            return (U)(order_of(exact_key_of(id)) >> kDrop);
+        };
+        const auto count = [&](U least) {
+            uint32_t c = 0;
+#pragma unroll 1
+            for (uint32_t id = thread(); id < a.n_ids; id += THREADS) c += order_at(id) >= least ? 1u : 0u;
+            return team.sum(c);
+        };
+        // at least min(k, live) keys are >= lo, fewer than k >= hi
+        U lo = none + 1, hi = ~(U)0;
+        uint32_t above = 0;   // keys above lo where the bisection ends on a key
+        uint32_t c = count(lo);
+        if (c > w.k) {
+#pragma unroll 1
+            while (hi - lo > 1 && c != w.k) {
+                const U mid = lo + (hi - lo) / 2;
+                c = count(mid);
+                if (c >= w.k) lo = mid;
+                else hi = mid;
+            }
+            if (c != w.k) above = count(lo + 1);
+        }
+        uint32_t room = w.k - above, found = 0;   // places for keys equal to lo
+        const bool ties = above != 0 || c > w.k || hi - lo <= 1;
+#pragma unroll 1
+        for (uint32_t id0 = 0; id0 < a.n_ids; id0 += THREADS) {
+            const uint32_t id = id0 + thread();
+            const U key = id < a.n_ids ? order_at(id) : (U)0;
+            bool win = key >= lo;
+            uint32_t here[1], place[1];
+            if (ties) {
+                here[0] = key == lo ? 1u : 0u;
+                const uint32_t equal = team.places(here, place);
+                if (here[0] && place[0] >= room) win = false;
+                room -= equal < room ? equal : room;
+            }
+            here[0] = win ? 1u : 0u;
+            const uint32_t wins = team.places(here, place);
+            if (win) {
+                win_ids()[found + place[0]] = (int32_t)id;
+                win_scores()[found + place[0]] = score_of(id);
+            }
+            found += wins;
+        }
+        team.sync();
+        return found;
     }
 };
 
@@ -872,8 +931,9 @@ __global__ __launch_bounds__(block_of(THREADS)) void k_winners_grad(WinnersGradA
     }
 }
 
-// Calls f(R, THREADS) with the smallest layout that holds n ids.  Four rows share a wave where rows are short and enough of them
-// to fill the chip that way (1024 SIMDs, a wave each); with fewer the row's latency counts, and 64 lanes have less to do each.
+// Calls f(R, THREADS) with the smallest layout that holds n ids and chooses k of them by a threshold.  Four rows share a wave
+// where rows are short and enough of them to fill the chip that way (1024 SIMDs, a wave each); with fewer the row's latency
+// counts, and 64 lanes have less to do each.
 template <typename F>
 int with_layout(uint32_t n, uint64_t n_rows, uint32_t k, F&& f) {
     using std::integral_constant;
@@ -887,10 +947,13 @@ int with_layout(uint32_t n, uint64_t n_rows, uint32_t k, F&& f) {
     }
     if (n <= 64) return f(integral_constant<int, 1>{}, wave);
     if (n <= 128) return f(integral_constant<int, 2>{}, wave);
-    if (n <= 256) return f(integral_constant<int, 4>{}, wave);
-    if (n <= 512) return f(integral_constant<int, 8>{}, wave);
-    if (n <= 1024) return f(integral_constant<int, 16>{}, wave);
-    if (n <= 2048) return f(integral_constant<int, 32>{}, wave);
+    if (n <= 2048 && k <= kMostByThreshold<64>) {
+        if (n <= 256) return f(integral_constant<int, 4>{}, wave);
+        if (n <= 512) return f(integral_constant<int, 8>{}, wave);
+        if (n <= 1024) return f(integral_constant<int, 16>{}, wave);
+        return f(integral_constant<int, 32>{}, wave);
+    }
+    if (n <= 1024) return f(integral_constant<int, 2>{}, waves);
     if (n <= 4096) return f(integral_constant<int, 8>{}, waves);
     if (n <= 8192) return f(integral_constant<int, 16>{}, waves);
     return f(integral_constant<int, 32>{}, waves);
@@ -923,11 +986,11 @@ int launch_winners(const sdrb_dense& scores, const sdrb_winners_spec& spec, int3
             using T = decltype(t);
             const auto go = [&](auto s) {
                 constexpr bool SHARES = decltype(s)::value;
-                const size_t of_key = SHARES ? sizeof(double) : sizeof(float);
-                const size_t grouped = spec.groups > 1 ? (a.n_ids + spec.groups) * of_key + spec.groups : 0;
+                const auto up = [](size_t bytes) { return (uint32_t)((bytes + 15) / 16 * 16); };
                 const size_t held = (a.n_ids < (uint32_t)THREADS * kHeld ? a.n_ids : (uint32_t)THREADS * kHeld) * sizeof(int32_t);
-                const size_t listed = spec.k * 8 > held ? spec.k * 8 : held;
-                a.lds_row = (uint32_t)(((grouped > listed ? grouped : listed) + 15) / 16 * 16);
+                const size_t keys = spec.groups > 1 ? a.n_ids * sizeof(float) : 0, won = spec.k * 8;
+                a.lds_groups = up(won > held ? (won > keys ? won : keys) : (held > keys ? held : keys));
+                a.lds_row = a.lds_groups + (spec.groups > 1 ? up(kWinnersMaxGroups + (spec.groups + 3) * (SHARES ? sizeof(double) : sizeof(float))) : 0);
                 const size_t lds = (size_t)a.lds_row * kPerBlock;
                 if (const int rc = allow_lds(&k_winners<R, THREADS, SHARES, T>, lds)) return rc;
                 hipLaunchKernelGGL((k_winners<R, THREADS, SHARES, T>), dim3((uint32_t)((a.n_rows + kPerBlock - 1) / kPerBlock)),
