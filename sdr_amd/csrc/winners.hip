@@ -723,6 +723,7 @@ struct Row {
     }
 };
 
+// (k is at most 16, 128 and 1024 for 16, 64 and 512 threads)
 constexpr uint32_t block_of(int threads) { return threads < 256 ? 256 : threads; }
 
 template <int R, int THREADS, bool SHARES, typename T>
@@ -804,131 +805,117 @@ struct WinnersGradArgs {
     sdrb_winners_spec w;
     uint64_t n_rows, ld, out_ld;
     uint32_t n_ids;
-    uint32_t lds_row;
 };
 
-// d scores of a row, from its winners and their weights' gradient, laid out in LDS: a row of zeros into which the winners'
-// values are put.  Only a softmax over the whole row reads the row; the other gradients read the winners' scores alone.
-// Bound: the write of the result.
+// d scores of a row, from its winners and their weights' gradient.  The row is written as if nothing had won -- zeros, or a
+// softmax's share of what is taken from every score -- and the winners' values are stored over it, once those stores have
+// arrived; only a softmax over the whole row reads it, the other gradients read the winners' scores alone.  No LDS: what
+// bounds it is latency (ids, then their scores) over the waves in flight, and the write of the result.
 template <int R, int THREADS, bool WHOLE, typename T, typename O>
 __global__ __launch_bounds__(block_of(THREADS)) void k_winners_grad(WinnersGradArgs a, const T* __restrict__ scores,
                                                                     const int32_t* __restrict__ ids_in,
-                                                                    const float* __restrict__ grad_in, O* __restrict__ out) {
+                                                                    const float* __restrict__ grad_in, O* out) {
     using L = Layout<R, THREADS>;
     constexpr int C = L::C, kWaves = THREADS > 64 ? THREADS / 64 : 1;
-    extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
     __shared__ double slots[2 * kWaves];
-    const uint32_t in_block = threadIdx.x / THREADS;
-    const uint64_t row = (uint64_t)blockIdx.x * (block_of(THREADS) / THREADS) + in_block;
+    const uint64_t row = (uint64_t)blockIdx.x * (block_of(THREADS) / THREADS) + threadIdx.x / THREADS;
     if (row >= a.n_rows) return;
-    float* line = reinterpret_cast<float*>(lds + in_block * a.lds_row);   // [L::kIds]
     Team<THREADS> team{slots, nullptr, 0};
     const uint32_t thread = team.thread();
     const T* s_row = scores + row * a.ld;
-    const int32_t* ids = ids_in + row * a.w.k;
-    const float* grad = grad_in + row * a.w.k;
+    O* to = out + row * a.out_ld;
     const sdrb_winners_spec& w = a.w;
     const bool sig = w.score == SDRB_SCORE_SIGMOID;
+    // a thread's winners (the layouts give it at most two); -1 where it has none: a NaN or -inf never won
+    constexpr int H = 2;
+    int32_t id[H];
+    float x[H], g[H];
+#pragma unroll
+    for (int h = 0; h < H; ++h) {
+        const uint32_t i = h * THREADS + thread;
+        id[h] = i < w.k ? ids_in[row * w.k + i] : -1;
+        g[h] = i < w.k ? grad_in[row * w.k + i] : 0.0f;
+    }
     float s[WHOLE ? R : 1];
-    if constexpr (WHOLE) read_scores<R, THREADS>(s_row, a.n_ids, s);
-    const float zeros[C] = {};
-#pragma unroll
-    for (int q = 0; q < R / C; ++q) store_n<C>(line + L::id(q * C), zeros);
-    team.sync();
-    // a thread's winners: the score of place i, -inf where it holds none
-    const auto score_at = [&](uint32_t i, int32_t& id) {
-        id = ids[i];
-        if (id < 0 || (uint32_t)id >= a.n_ids) return -INFINITY;
-        const float x = to_f32(s_row[id]);
-        return x > -INFINITY ? x : -INFINITY;   // (a NaN never won)
-    };
     if constexpr (WHOLE) {
-        for (uint32_t i = thread; i < w.k; i += THREADS) {
-            int32_t id;
-            if (score_at(i, id) > -INFINITY) line[id] = grad[i];
-        }
-        team.sync();
-        float m = -INFINITY;
-#pragma unroll
-        for (int r = 0; r < R; ++r) m = fmaxf(m, s[r]);
-        m = team.max(m);
-        float g[R], sum = 0.0f, dot = 0.0f;
-#pragma unroll
-        for (int q = 0; q < R / C; ++q) {
-            float part[C];
-            load_n<C>(line + L::id(q * C), part);
-#pragma unroll
-            for (int j = 0; j < C; ++j) g[q * C + j] = part[j];
-        }
-#pragma unroll
-        for (int r = 0; r < R; ++r) {
-            s[r] = s[r] > -INFINITY ? exp_fast(below(s[r], m)) : 0.0f;
-            sum += s[r];
-            dot = fmaf(s[r], g[r], dot);
-        }
-        const float inv = rcp_fast(team.sum(sum));
-        dot = team.sum(dot) * inv;
-        const float scale = w.scale * inv;
-#pragma unroll
-        for (int r = 0; r < R; ++r) s[r] = s[r] > 0.0f ? scale * s[r] * (g[r] - dot) : 0.0f;
-#pragma unroll
-        for (int q = 0; q < R / C; ++q) {
-            const uint32_t first = L::id(q * C);
-            O* to = out + row * a.out_ld + first;
-            if (first + C <= a.n_ids) {
-                float part[C];
-#pragma unroll
-                for (int j = 0; j < C; ++j) part[j] = s[q * C + j];
-                store_n<C>(to, part);
-            } else {
-#pragma unroll
-                for (int j = 0; j < C; ++j)
-                    if (first + j < a.n_ids) to[j] = from_f32<O>(s[q * C + j]);
-            }
-        }
+        read_scores<R, THREADS>(s_row, a.n_ids, s);
     } else {
-        float shift = 0.0f, inv = 1.0f, dot = 0.0f;
-        const auto part_of = [&](float x) { return sig ? sigmoid_over(x, shift) : exp_fast(below(x, shift)); };
-        if (w.renormalise) {
-            float m = -INFINITY, sum = 0.0f;
-            int32_t id;
-            for (uint32_t i = thread; i < w.k; i += THREADS) m = max_of(m, score_at(i, id));
-            shift = team.max(m);
-            if (sig) shift = shift < 0.0f ? shift : 0.0f;
-            for (uint32_t i = thread; i < w.k; i += THREADS) {
-                const float x = score_at(i, id);
-                if (x > -INFINITY) {
-                    const float p = part_of(x);
-                    sum += p;
-                    dot = fmaf(p, grad[i], dot);
-                }
-            }
-            inv = rcp_fast(team.sum(sum));
-            dot = team.sum(dot) * inv;
-        }
-        for (uint32_t i = thread; i < w.k; i += THREADS) {
-            int32_t id;
-            const float x = score_at(i, id);
-            if (x > -INFINITY) {
-                float d = w.renormalise ? part_of(x) * inv * (grad[i] - dot) : grad[i] * sigmoid(x);
-                if (sig) d *= sigmoid(-x);
-                line[id] = w.scale * d;
-            }
-        }
-        team.sync();
-        constexpr int V = 16 / sizeof(O);   // 16 bytes of the result a lane
+        constexpr int V = 16 / sizeof(O);
+        const float zeros[V] = {};
         for (uint32_t first = thread * V; first < a.n_ids; first += THREADS * V) {
-            float part[V];
-            load_n<V>(line + first, part);
-            O* to = out + row * a.out_ld + first;
             if (first + V <= a.n_ids) {
-                store_n<V>(to, part);
+                store_n<V>(to + first, zeros);
             } else {
-                for (int j = 0; j < V; ++j)
-                    if (first + j < a.n_ids) to[j] = from_f32<O>(part[j]);
+                for (uint32_t j = first; j < a.n_ids; ++j) to[j] = from_f32<O>(0.0f);
             }
         }
     }
+#pragma unroll
+    for (int h = 0; h < H; ++h) {
+        x[h] = id[h] >= 0 && (uint32_t)id[h] < a.n_ids ? to_f32(s_row[id[h]]) : -INFINITY;
+        if (!(x[h] > -INFINITY)) id[h] = -1;
+    }
+    // the part of the softmax that the sum runs over; `shift` is its largest argument
+    float shift = 0.0f, inv = 1.0f, dot = 0.0f;
+    const auto part_of = [&](float v) { return sig ? sigmoid_over(v, shift) : exp_fast(below(v, shift)); };
+    if (WHOLE || w.renormalise) {
+        float m = -INFINITY, sum = 0.0f;
+        if constexpr (WHOLE) {
+#pragma unroll
+            for (int r = 0; r < R; ++r) m = fmaxf(m, s[r]);
+        } else {
+#pragma unroll
+            for (int h = 0; h < H; ++h)
+                if (id[h] >= 0) m = fmaxf(m, x[h]);
+        }
+        shift = team.max(m);
+        if (sig) shift = shift < 0.0f ? shift : 0.0f;
+        if constexpr (WHOLE) {
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                s[r] = s[r] > -INFINITY ? exp_fast(below(s[r], shift)) : 0.0f;
+                sum += s[r];
+            }
+        }
+#pragma unroll
+        for (int h = 0; h < H; ++h)
+            if (id[h] >= 0) {
+                const float p = part_of(x[h]);
+                if (!WHOLE) sum += p;
+                dot = fmaf(p, g[h], dot);
+            }
+        inv = rcp_fast(team.sum(sum));
+        dot = team.sum(dot) * inv;
+    }
+    if constexpr (WHOLE) {
+        const float scale = -w.scale * inv * dot;
+#pragma unroll
+        for (int q = 0; q < R / C; ++q) {
+            const uint32_t first = L::id(q * C);
+            float part[C];
+#pragma unroll
+            for (int j = 0; j < C; ++j) part[j] = s[q * C + j] > 0.0f ? scale * s[q * C + j] : 0.0f;   // (a row without live scores has inv = inf)
+            if (first + C <= a.n_ids) {
+                store_n<C>(to + first, part);
+            } else {
+#pragma unroll
+                for (int j = 0; j < C; ++j)
+                    if (first + j < a.n_ids) to[first + j] = from_f32<O>(part[j]);
+            }
+        }
+    }
+    // the stores above come from other lanes: they have arrived before the ones below set out
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(0x0F70);   // vmcnt(0)
+    if constexpr (kWaves > 1) __syncthreads();
+    asm volatile("" ::: "memory");
+#pragma unroll
+    for (int h = 0; h < H; ++h)
+        if (id[h] >= 0) {
+            float d = WHOLE || w.renormalise ? part_of(x[h]) * inv * (g[h] - dot) : g[h] * sigmoid(x[h]);
+            if (sig) d *= sigmoid(-x[h]);
+            to[id[h]] = from_f32<O>(w.scale * d);
+        }
 }
 
 // Calls f(R, THREADS) with the smallest layout that holds n ids and chooses k of them by a threshold.  Four rows share a wave
@@ -1015,17 +1002,14 @@ int launch_winners_grad(const sdrb_dense& scores, const sdrb_winners_spec& spec,
     return with_layout(a.n_ids, a.n_rows, spec.k, [&](auto r, auto n_threads) {
         constexpr int R = decltype(r)::value, THREADS = decltype(n_threads)::value;
         constexpr uint32_t kPerBlock = block_of(THREADS) / THREADS;
-        a.lds_row = (uint32_t)(Layout<R, THREADS>::kIds + 8) * sizeof(float);   // (16 bytes of result are read at a time)
-        const size_t lds = (size_t)a.lds_row * kPerBlock;
         return with_type(scores.type, [&](auto t) {
             return with_type(out.type, [&](auto o) {
                 using T = decltype(t);
                 using O = decltype(o);
                 const auto go = [&](auto all) {
                     constexpr bool WHOLE = decltype(all)::value;
-                    if (const int rc = allow_lds(&k_winners_grad<R, THREADS, WHOLE, T, O>, lds)) return rc;
                     hipLaunchKernelGGL((k_winners_grad<R, THREADS, WHOLE, T, O>), dim3((uint32_t)((a.n_rows + kPerBlock - 1) / kPerBlock)),
-                                       dim3(block_of(THREADS)), lds, stream, a, static_cast<const T*>(scores.data), ids, grad_weights,
+                                       dim3(block_of(THREADS)), 0, stream, a, static_cast<const T*>(scores.data), ids, grad_weights,
                                        static_cast<O*>(out.data));
                     SDRB_HIP(hipGetLastError());
                     return SDRB_OK;
