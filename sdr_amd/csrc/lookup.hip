@@ -1,10 +1,18 @@
 // Ragged gather-sums over a dense matrix: out[s, :] = scale * sum of weight[p] * src[index[p], :] over a segment's
 // elements p.  A lookup runs it over the rows of a batch, the table's gradient over the elements sorted by id.
 //
-// A group of lanes owns one segment and one slice of the columns, 16 bytes of src a lane, and adds the segment's
-// elements in order into binary32 registers; the sum is scaled and rounded once to the output's type.  A segment of
-// more than `chunk` elements would keep its group busy long after the others: its elements are summed by groups that
-// own a chunk of the element list each (k_gather_chunks), and the segment's own group adds those sums up in order.
+// A group of L lanes owns one segment and a slice of the columns, V * SL columns a lane, and adds the segment's elements into
+// binary32 registers; the sum is scaled and rounded once to the output's type.  The group's lanes read L elements at a time,
+// one each, turn ids into byte offsets, and pass these around by ds_bpermute, so that an element costs its lanes one
+// addition, the load, and an fma a column.  Rows of src are read by buffer loads, which yield 0 beyond the matrix: an element
+// that contributes nothing has an offset there and a weight of 0, and needs no branch.  (Matrices beyond 2 GiB, or not aligned
+// to 4 bytes, are read by address.)
+// Short segments (tokens): whole waves, four slices at once, one element a turn: a copy, bound by HBM.
+// Long segments (codes): L = 8, 128 bytes of a row.  A table's slice of 128 bytes times its rows fits the 4 MiB of an XCD's L2
+// where the whole does not, so each XCD (block number modulo 8) works through the slices of its own, one after another.
+// S groups share a segment where there are too few of them to fill the chip, and join their sums in LDS.
+// A segment of more than `chunk` elements would keep its group busy long after the others: its elements are summed by groups
+// that own a chunk of the element list each (k_gather_chunks), and the segment's own group adds those sums up in order.
 // Every order of additions follows from the shapes and offsets alone: results repeat bit for bit.
 #include <algorithm>
 
@@ -14,17 +22,28 @@ namespace sdrb {
 
 namespace {
 
+constexpr uint32_t kThreads = 256;
+constexpr uint32_t kNowhere = 0x80000000u;   // an offset beyond every matrix that is read by buffer loads
+
 struct GatherArgs {
     uint64_t n_segments, n_elems, src_rows, src_ld, out_ld;
     const uint32_t* start;
+    const void* index;
     const float* weight;
     float* partials;
+    uint32_t row_bytes;      // of src, where it is read by buffer loads
+    uint32_t src_bytes;      // its end
     float scale;
-    uint32_t row_len;       // where start is null
+    uint32_t row_len;        // where start is null
     uint32_t dim;
-    uint32_t chunk;         // longer segments come from `partials` (0: there are none)
-    uint32_t lanes_log2;    // lanes of a group
-    uint32_t slices;        // of the columns
+    uint32_t chunk;          // longer segments come from `partials` (0: there are none)
+    uint32_t lanes_log2;     // L
+    uint32_t split_log2;     // S
+    uint32_t slices;         // of the columns
+    uint32_t xcd_slices;     // 1: a block's slice follows from its XCD
+    uint32_t blocks;         // of a slice
+    uint32_t wide_index;     // 64-bit indexes
+    uint32_t accumulate;
 };
 
 // the elements [lo, hi) of a segment; offsets that run backwards or past the list are cut to it
@@ -40,80 +59,191 @@ __device__ __forceinline__ void segment_of(const GatherArgs& a, uint64_t s, uint
     }
 }
 
-template <int V, typename T, typename Id, bool WEIGHTED>
-__device__ __forceinline__ void add_elements(const GatherArgs& a, const Id* __restrict__ index, const T* __restrict__ src,
-                                             uint64_t lo, uint64_t hi, uint32_t col, float (&acc)[V]) {
-    for (uint64_t p = lo; p < hi; ++p) {
-        const Id id = index[p];
-        if (id < 0 || (uint64_t)id >= a.src_rows) continue;
-        float v[V];
-        load_n<V>(src + (uint64_t)id * a.src_ld + col, v);
-        const float w = WEIGHTED ? a.weight[p] : 1.0f;
-#pragma unroll
-        for (int k = 0; k < V; ++k) acc[k] = WEIGHTED ? fmaf(w, v[k], acc[k]) : acc[k] + v[k];
-    }
+__device__ __forceinline__ uint32_t from_lane(uint32_t v, uint32_t lane) {
+    return (uint32_t)__builtin_amdgcn_ds_bpermute((int)(lane * 4), (int)v);
 }
 
-// Where a group stands: its segment (or chunk) and the first column of this lane.  A lane whose columns would run past
-// the end reads the last V columns instead and stores only what is its own (from `col_own`).
+// Where a group stands: its segment (or chunk), its part of the segment, and its lane's columns.  A lane whose columns would run
+// past the end reads the last V columns instead and stores only what is its own (from `own`).
+template <int V, int SL>
 struct Place {
     uint64_t item;
-    uint32_t slice, col, col_own;
+    uint32_t lane, part;
+    uint32_t col[SL], own[SL];
     bool live;
+
+    __device__ __forceinline__ Place(const GatherArgs& a, uint64_t n_items) {
+        const uint32_t lanes = 1u << a.lanes_log2, group = threadIdx.x >> a.lanes_log2;
+        const uint32_t items = (kThreads >> a.lanes_log2) >> a.split_log2;   // of a block
+        lane = threadIdx.x & (lanes - 1);
+        part = group & ((1u << a.split_log2) - 1);
+        uint32_t slice;
+        uint64_t block;
+        if (a.xcd_slices) {
+            // XCD x takes the slices x, x + 8, ..., one after another over all segments (slices: a multiple of 8), or its share
+            // of one slice's segments (slices: 1, 2 or 4)
+            const uint32_t xcd = blockIdx.x & 7, turn = blockIdx.x >> 3;
+            if (a.slices >= 8) {
+                slice = xcd + 8 * (turn / a.blocks);
+                block = turn % a.blocks;
+            } else {
+                slice = xcd & (a.slices - 1);
+                block = (uint64_t)turn * (8 / a.slices) + xcd / a.slices;
+            }
+        } else {
+            slice = blockIdx.x % a.slices;
+            block = blockIdx.x / a.slices;
+        }
+        item = block * items + (group >> a.split_log2);
+        live = item < n_items && slice < a.slices;
+#pragma unroll
+        for (int j = 0; j < SL; ++j) {
+            own[j] = (((slice * SL + j) << a.lanes_log2) + lane) * V;
+            col[j] = own[j] + V <= a.dim ? own[j] : a.dim - V;
+        }
+    }
+    __device__ __forceinline__ bool stores(const GatherArgs& a, int j) const { return own[j] < a.dim; }
 };
-template <int V>
-__device__ __forceinline__ Place place_of(const GatherArgs& a, uint64_t n_items) {
-    Place p;
-    const uint32_t groups = 256u >> a.lanes_log2, group = threadIdx.x >> a.lanes_log2;
-    const uint32_t lane = threadIdx.x & ((1u << a.lanes_log2) - 1u);
-    p.slice = blockIdx.x % a.slices;
-    p.item = (uint64_t)(blockIdx.x / a.slices) * groups + group;
-    p.col_own = ((p.slice << a.lanes_log2) + lane) * V;
-    p.live = p.item < n_items && p.col_own < a.dim;
-    p.col = p.col_own + V <= a.dim ? p.col_own : a.dim - V;
-    return p;
+
+using i32x2 = __attribute__((ext_vector_type(2))) int32_t;
+using i32x4 = __attribute__((ext_vector_type(4))) int32_t;
+
+// V elements at a byte offset of the matrix; beyond it zeros
+template <int V, typename T>
+__device__ __forceinline__ void load_at(__amdgpu_buffer_rsrc_t src, uint32_t offset, float (&v)[V]) {
+    constexpr int kBytes = V * sizeof(T);
+    static_assert(kBytes == 16 || kBytes == 8 || kBytes == 4);
+    T t[V];
+    if constexpr (kBytes == 16) {
+        const i32x4 raw = __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(src, (int)offset, 0, 0));
+        __builtin_memcpy(t, &raw, sizeof t);
+    } else if constexpr (kBytes == 8) {
+        const i32x2 raw = __builtin_bit_cast(i32x2, __builtin_amdgcn_raw_buffer_load_b64(src, (int)offset, 0, 0));
+        __builtin_memcpy(t, &raw, sizeof t);
+    } else {
+        const int32_t raw = __builtin_bit_cast(int32_t, __builtin_amdgcn_raw_buffer_load_b32(src, (int)offset, 0, 0));
+        __builtin_memcpy(t, &raw, sizeof t);
+    }
+#pragma unroll
+    for (int k = 0; k < V; ++k) v[k] = to_f32(t[k]);
 }
 
-template <int V, typename T, typename O, typename Id, bool WEIGHTED, bool ACCUMULATE>
-__global__ __launch_bounds__(256) void k_gather_rows(GatherArgs a, const Id* __restrict__ index, const T* __restrict__ src,
-                                                     O* __restrict__ out) {
-    const Place at = place_of<V>(a, a.n_segments);
-    if (!at.live) return;
-    uint64_t lo, hi;
-    segment_of(a, at.item, lo, hi);
-    if (ACCUMULATE && lo == hi) return;
-    float acc[V];
+// acc += the elements [lo, hi) of the list, as far as this part of the segment goes.  U elements a turn.
+template <int V, int SL, int U, bool BUFFER, typename T>
+__device__ __forceinline__ void add_elements(const GatherArgs& a, const Place<V, SL>& at, const T* __restrict__ src, uint64_t lo,
+                                             uint64_t hi, float (&acc)[SL][V]) {
+    const uint32_t lanes = 1u << a.lanes_log2, first = threadIdx.x & 63 & ~(lanes - 1);   // of the group
+    const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(src), 0, (int)a.src_bytes, 0x00020000);
+    for (uint64_t p0 = lo + ((uint64_t)at.part << a.lanes_log2); p0 < hi; p0 += (uint64_t)lanes << a.split_log2) {
+        const uint64_t p = p0 + at.lane;
+        uint64_t id = ~0ull;
+        if (p < hi) id = a.wide_index ? static_cast<const uint64_t*>(a.index)[p] : (uint64_t)(int64_t) static_cast<const int32_t*>(a.index)[p];
+        const bool in = id < a.src_rows;   // (a negative id is a large one)
+        float w = 0.0f;
+        if (in) w = a.weight ? a.weight[p] : 1.0f;
+        const uint32_t offset = BUFFER ? (in ? (uint32_t)id * a.row_bytes : kNowhere) : (in ? (uint32_t)id : kNowhere);
+        const uint32_t n = hi - p0 < lanes ? (uint32_t)(hi - p0) : lanes;
+        for (uint32_t u = 0; u < n; u += U) {
+            float v[U][SL][V], wu[U];
 #pragma unroll
-    for (int k = 0; k < V; ++k) acc[k] = 0.0f;
+            for (int j = 0; j < U; ++j) {
+                // (lanes beyond n, and beyond the group where U is larger, hold no element)
+                const uint32_t from = first + (U > 1 && u + j >= lanes ? lanes - 1 : u + j);
+                uint32_t o = from_lane(offset, from);
+                wu[j] = __builtin_bit_cast(float, from_lane(__builtin_bit_cast(uint32_t, w), from));
+                if (U > 1 && u + j >= lanes) {
+                    o = kNowhere;
+                    wu[j] = 0.0f;
+                }
+#pragma unroll
+                for (int k = 0; k < SL; ++k) {
+                    if constexpr (BUFFER) {
+                        load_at<V, T>(rsrc, o + at.col[k] * (uint32_t)sizeof(T), v[j][k]);
+                    } else {
+#pragma unroll
+                        for (int c = 0; c < V; ++c) v[j][k][c] = 0.0f;
+                        if (o != kNowhere) load_n<V>(src + (uint64_t)o * a.src_ld + at.col[k], v[j][k]);
+                    }
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < U; ++j)
+#pragma unroll
+                for (int k = 0; k < SL; ++k)
+#pragma unroll
+                    for (int c = 0; c < V; ++c) acc[k][c] = fmaf(wu[j], v[j][k][c], acc[k][c]);
+        }
+    }
+}
+
+// The parts' sums, added up in order by the first of them.
+template <int V, int SL>
+__device__ __forceinline__ void join_parts(const GatherArgs& a, uint32_t part, float (&acc)[SL][V], float* shared) {
+    const uint32_t parts = 1u << a.split_log2;
+    if (parts == 1) return;
+#pragma unroll
+    for (int k = 0; k < SL; ++k) {
+        if (k) __syncthreads();
+#pragma unroll
+        for (int c = 0; c < V; ++c) shared[c * kThreads + threadIdx.x] = acc[k][c];
+        __syncthreads();
+        if (part == 0)
+            for (uint32_t s = 1; s < parts; ++s)
+#pragma unroll
+                for (int c = 0; c < V; ++c) acc[k][c] += shared[c * kThreads + threadIdx.x + (s << a.lanes_log2)];
+    }
+}
+
+template <int V, int SL, int U, bool BUFFER, typename T, typename O>
+__global__ __launch_bounds__(kThreads) void k_gather_rows(GatherArgs a, const T* __restrict__ src, O* __restrict__ out) {
+    __shared__ float shared[V * kThreads];
+    const Place<V, SL> at(a, a.n_segments);
+    uint64_t lo = 0, hi = 0;
+    if (at.live) segment_of(a, at.item, lo, hi);
+    float acc[SL][V];
+#pragma unroll
+    for (int k = 0; k < SL; ++k)
+#pragma unroll
+        for (int c = 0; c < V; ++c) acc[k][c] = 0.0f;
     if (a.chunk && hi - lo > a.chunk) {
         // chunk c of the element list keeps two sums: of the segment its first element lies in, and of the one its last
-        for (uint64_t c = lo / a.chunk; c * a.chunk < hi; ++c) {
-            const float* part = a.partials + (2 * c + (c * a.chunk < lo ? 1 : 0)) * a.dim + at.col;
-            float v[V];
-            load_n<V>(part, v);
+        if (at.part == 0)
+            for (uint64_t c = lo / a.chunk; c * a.chunk < hi; ++c) {
+                const float* part = a.partials + (2 * c + (c * a.chunk < lo ? 1 : 0)) * a.dim;
 #pragma unroll
-            for (int k = 0; k < V; ++k) acc[k] += v[k];
-        }
+                for (int k = 0; k < SL; ++k) {
+                    float v[V];
+                    load_n<V>(part + at.col[k], v);
+#pragma unroll
+                    for (int j = 0; j < V; ++j) acc[k][j] += v[j];
+                }
+            }
     } else {
-        add_elements<V, T, Id, WEIGHTED>(a, index, src, lo, hi, at.col, acc);
+        add_elements<V, SL, U, BUFFER>(a, at, src, lo, hi, acc);
     }
-    O* to = out + at.item * a.out_ld + at.col;
-    if (at.col == at.col_own) {
-        if (ACCUMULATE) {
-            float old[V];
-            load_n<V>(to, old);
+    join_parts<V, SL>(a, at.part, acc, shared);
+    if (!at.live || at.part != 0 || (a.accumulate && lo == hi)) return;
 #pragma unroll
-            for (int k = 0; k < V; ++k) acc[k] = fmaf(a.scale, acc[k], old[k]);
+    for (int k = 0; k < SL; ++k) {
+        if (!at.stores(a, k)) break;
+        O* to = out + at.item * a.out_ld + at.col[k];
+        if (at.col[k] == at.own[k]) {
+            if (a.accumulate) {
+                float old[V];
+                load_n<V>(to, old);
+#pragma unroll
+                for (int c = 0; c < V; ++c) acc[k][c] = fmaf(a.scale, acc[k][c], old[c]);
+            } else {
+#pragma unroll
+                for (int c = 0; c < V; ++c) acc[k][c] *= a.scale;
+            }
+            store_n<V>(to, acc[k]);
         } else {
+            const uint32_t skip = at.own[k] - at.col[k];
 #pragma unroll
-            for (int k = 0; k < V; ++k) acc[k] *= a.scale;
+            for (int c = 0; c < V; ++c)
+                if ((uint32_t)c >= skip) to[c] = from_f32<O>(a.accumulate ? fmaf(a.scale, acc[k][c], to_f32(to[c])) : acc[k][c] * a.scale);
         }
-        store_n<V>(to, acc);
-    } else {
-        const uint32_t skip = at.col_own - at.col;
-#pragma unroll
-        for (int k = 0; k < V; ++k)
-            if ((uint32_t)k >= skip) to[k] = from_f32<O>(ACCUMULATE ? fmaf(a.scale, acc[k], to_f32(to[k])) : acc[k] * a.scale);
     }
 }
 
@@ -129,74 +259,127 @@ __device__ __forceinline__ uint64_t segment_at(const uint32_t* __restrict__ star
 }
 
 // the sums that chunk c of the element list contributes to segments longer than a chunk
-template <int V, typename T, typename Id, bool WEIGHTED>
-__global__ __launch_bounds__(256) void k_gather_chunks(GatherArgs a, const Id* __restrict__ index, const T* __restrict__ src,
-                                                       uint64_t n_chunks) {
-    const Place at = place_of<V>(a, n_chunks);
-    if (!at.live) return;
+template <int V, int SL, int U, bool BUFFER, typename T>
+__global__ __launch_bounds__(kThreads) void k_gather_chunks(GatherArgs a, const T* __restrict__ src, uint64_t n_chunks) {
+    __shared__ float shared[V * kThreads];
+    const Place<V, SL> at(a, n_chunks);
     const uint64_t c_lo = at.item * a.chunk, c_hi = c_lo + a.chunk < a.n_elems ? c_lo + a.chunk : a.n_elems;
-#pragma unroll
+#pragma unroll 1
     for (int end = 0; end < 2; ++end) {
-        uint64_t lo, hi;
-        if (a.start) {
-            segment_of(a, segment_at(a.start, a.n_segments, end ? c_hi - 1 : c_lo), lo, hi);
-        } else {
-            lo = (end ? c_hi - 1 : c_lo) / a.row_len * a.row_len;
-            hi = lo + a.row_len;
+        uint64_t lo = 0, hi = 0;
+        if (at.live) {
+            if (a.start) {
+                segment_of(a, segment_at(a.start, a.n_segments, end ? c_hi - 1 : c_lo), lo, hi);
+            } else {
+                lo = (end ? c_hi - 1 : c_lo) / a.row_len * a.row_len;
+                hi = lo + a.row_len;
+            }
+            if (hi - lo <= a.chunk || (end && lo <= c_lo)) lo = hi = 0;   // short, or the first element's segment once more
         }
-        if (hi - lo <= a.chunk) continue;
-        if (end && lo <= c_lo) continue;   // the first element's segment once more
-        float acc[V];
+        const bool any = lo < hi;
+        float acc[SL][V];
 #pragma unroll
-        for (int k = 0; k < V; ++k) acc[k] = 0.0f;
-        add_elements<V, T, Id, WEIGHTED>(a, index, src, lo > c_lo ? lo : c_lo, hi < c_hi ? hi : c_hi, at.col, acc);
-        float* to = a.partials + (2 * at.item + end) * a.dim + at.col;
-        if (at.col == at.col_own) {
-            store_n<V>(to, acc);
-        } else {
-            const uint32_t skip = at.col_own - at.col;
+        for (int k = 0; k < SL; ++k)
 #pragma unroll
-            for (int k = 0; k < V; ++k)
-                if ((uint32_t)k >= skip) to[k] = acc[k];
+            for (int c = 0; c < V; ++c) acc[k][c] = 0.0f;
+        if (a.split_log2 ? __syncthreads_or(any) : any) {
+            if (any) add_elements<V, SL, U, BUFFER>(a, at, src, lo > c_lo ? lo : c_lo, hi < c_hi ? hi : c_hi, acc);
+            join_parts<V, SL>(a, at.part, acc, shared);
+            if (any && at.part == 0)
+#pragma unroll
+                for (int k = 0; k < SL; ++k) {
+                    if (!at.stores(a, k)) break;
+                    float* to = a.partials + (2 * at.item + end) * a.dim + at.col[k];
+                    if (at.col[k] == at.own[k]) {
+                        store_n<V>(to, acc[k]);
+                    } else {
+                        const uint32_t skip = at.own[k] - at.col[k];
+#pragma unroll
+                        for (int c = 0; c < V; ++c)
+                            if ((uint32_t)c >= skip) to[c] = acc[k][c];
+                    }
+                }
+            if (a.split_log2) __syncthreads();
         }
     }
 }
 
-// the longest run of elements that one group of lanes sums by itself
+// The longest run of elements that one group of lanes sums by itself: long enough that few segments need a second step, short
+// enough that the longest does not outlast the rest.
 uint32_t chunk_of(uint64_t n_segments, uint64_t n_elems) {
     const uint64_t mean = n_elems / (n_segments ? n_segments : 1);
-    uint32_t chunk = 128;
+    uint32_t chunk = 64;
     while (chunk < 4 * mean && chunk < 1024) chunk *= 2;
     return chunk;
 }
 
-template <int V, typename T, typename O, typename Id, bool WEIGHTED>
-int launch_typed(const GatherSum& g, GatherArgs a, hipStream_t stream) {
-    const Id* index = static_cast<const Id*>(g.index);
+uint32_t log2_of(uint64_t v) {
+    uint32_t l = 0;
+    while ((2ull << l) <= v) ++l;
+    return l;
+}
+
+template <int V, int SL, int U, bool BUFFER, typename T, typename O>
+int launch_shaped(const GatherSum& g, GatherArgs a, uint64_t mean, hipStream_t stream) {
     const T* src = static_cast<const T*>(g.src);
-    uint32_t lanes_log2 = 0;
-    while (lanes_log2 < 6 && ((uint64_t)V << lanes_log2) < a.dim) ++lanes_log2;
-    a.lanes_log2 = lanes_log2;
-    a.slices = (uint32_t)((a.dim + ((uint64_t)V << lanes_log2) - 1) / ((uint64_t)V << lanes_log2));
-    const uint64_t per_block = 256u >> lanes_log2;
-    const auto blocks = [&](uint64_t items) { return (items + per_block - 1) / per_block * a.slices; };
-    if (blocks(g.n_segments) > 0x7FFFFFFFull) {
-        set_error("too many rows and columns for one launch");
-        return SDRB_ERR_OVERFLOW;
-    }
+    const uint64_t vectors = (a.dim + V - 1) / V;
+    // lanes of a group: a wave, or 128 bytes of a row for long segments; no more than the row has vectors
+    a.lanes_log2 = std::min<uint32_t>(U == 1 ? 6 : 3, log2_of(vectors > 1 ? 2 * vectors - 1 : 1));
+    const uint64_t a_slice = (uint64_t)SL << a.lanes_log2;
+    a.slices = (uint32_t)((vectors + a_slice - 1) / a_slice);
+    const auto run = [&](auto kernel, GatherArgs b, uint64_t items, uint64_t each, auto... more) {
+        // S: waves for the whole chip, eight a SIMD, as long as every part has elements to add
+        const uint64_t groups = items * b.slices, enough = (uint64_t)1024 * 8 * (64u >> b.lanes_log2);
+        b.split_log2 = 0;
+        while ((kThreads >> b.lanes_log2 >> b.split_log2) > 1 && (groups << b.split_log2) < enough && (1ull << b.split_log2) << b.lanes_log2 < each)
+            ++b.split_log2;
+        const uint64_t per_block = kThreads >> b.lanes_log2 >> b.split_log2, blocks = (items + per_block - 1) / per_block;
+        uint64_t grid = blocks * b.slices;
+        b.xcd_slices = 0;
+        b.blocks = (uint32_t)blocks;
+        if (U > 1 && blocks >= 8) {
+            if (b.slices >= 8) {
+                b.xcd_slices = 1;
+                grid = blocks * ((b.slices + 7) / 8 * 8);
+            } else if ((b.slices & (b.slices - 1)) == 0) {
+                b.xcd_slices = 1;
+                grid = (blocks + 8 / b.slices - 1) / (8 / b.slices) * 8;
+            }
+        }
+        if (grid > 0x7FFFFFFFull) {
+            set_error("too many rows and columns for one launch");
+            return SDRB_ERR_OVERFLOW;
+        }
+        hipLaunchKernelGGL(kernel, dim3((uint32_t)grid), dim3(kThreads), 0, stream, b, src, more...);
+        SDRB_HIP(hipGetLastError());
+        return SDRB_OK;
+    };
     if (a.chunk) {
         const uint64_t n_chunks = (g.n_elems + a.chunk - 1) / a.chunk;
-        hipLaunchKernelGGL((k_gather_chunks<V, T, Id, WEIGHTED>), dim3((uint32_t)blocks(n_chunks)), dim3(256), 0, stream, a,
-                           index, src, n_chunks);
-        SDRB_HIP(hipGetLastError());
+        if (const int rc = run(k_gather_chunks<V, SL, U, BUFFER, T>, a, n_chunks, (uint64_t)a.chunk, n_chunks)) return rc;
     }
-    const dim3 grid((uint32_t)blocks(g.n_segments));
-    if (g.accumulate)
-        hipLaunchKernelGGL((k_gather_rows<V, T, O, Id, WEIGHTED, true>), grid, dim3(256), 0, stream, a, index, src, static_cast<O*>(g.out));
-    else
-        hipLaunchKernelGGL((k_gather_rows<V, T, O, Id, WEIGHTED, false>), grid, dim3(256), 0, stream, a, index, src, static_cast<O*>(g.out));
-    SDRB_HIP(hipGetLastError());
-    return SDRB_OK;
+    return run(k_gather_rows<V, SL, U, BUFFER, T, O>, a, g.n_segments, mean, static_cast<O*>(g.out));
+}
+
+template <typename T, typename O>
+int launch_typed(const GatherSum& g, GatherArgs a, hipStream_t stream) {
+    constexpr int kWide = 16 / sizeof(T), kEven = 16 / (sizeof(T) > sizeof(O) ? sizeof(T) : sizeof(O));
+    const uint64_t mean = g.n_elems / g.n_segments;
+    const uint64_t bytes = g.src_rows ? ((g.src_rows - 1) * g.src_ld + a.dim) * sizeof(T) : 0;
+    const bool buffer = bytes < kNowhere && reinterpret_cast<uintptr_t>(g.src) % 4 == 0 && g.src_ld * sizeof(T) % 4 == 0 && a.dim >= (uint32_t)kWide &&
+                        a.dim * sizeof(T) % 4 == 0;
+    a.row_bytes = (uint32_t)(g.src_ld * sizeof(T));
+    a.src_bytes = (uint32_t)bytes;
+    if (buffer) {
+        // long segments read more than they write: 16 bytes a load; short ones: 16 bytes at most a load or store
+        if (mean >= 3) return launch_shaped<kWide, 1, 4, true, T, O>(g, a, mean, stream);
+        return launch_shaped<kEven, 4, 1, true, T, O>(g, a, mean, stream);
+    }
+    if (a.dim >= (uint32_t)kWide) {
+        if (mean >= 3) return launch_shaped<kWide, 1, 4, false, T, O>(g, a, mean, stream);
+        return launch_shaped<kEven, 4, 1, false, T, O>(g, a, mean, stream);
+    }
+    return launch_shaped<1, 1, 1, false, T, O>(g, a, mean, stream);
 }
 
 }  // namespace
@@ -218,25 +401,17 @@ int launch_gather_sum(const GatherSum& g, hipStream_t stream) {
     a.src_ld = g.src_ld;
     a.out_ld = g.out_ld;
     a.start = g.start;
+    a.index = g.index;
+    a.wide_index = g.index_bits == 64;
     a.weight = g.weight;
     a.partials = g.partials;
     a.scale = g.scale;
     a.row_len = g.start ? 0u : (uint32_t)(g.n_elems / g.n_segments);
     a.dim = g.dim;
     a.chunk = g.partials ? chunk_of(g.n_segments, g.n_elems) : 0u;
+    a.accumulate = g.accumulate ? 1u : 0u;
     return with_type(g.src_type, [&](auto t) {
-        return with_type(g.out_type, [&](auto o) {
-            using T = decltype(t);
-            using O = decltype(o);
-            constexpr int V = 16 / sizeof(T);
-            const auto go = [&](auto id, auto weighted) {
-                using Id = decltype(id);
-                constexpr bool W = decltype(weighted)::value;
-                return a.dim >= (uint32_t)V ? launch_typed<V, T, O, Id, W>(g, a, stream) : launch_typed<1, T, O, Id, W>(g, a, stream);
-            };
-            if (g.index_bits == 64) return g.weight ? go(int64_t{}, std::true_type{}) : go(int64_t{}, std::false_type{});
-            return g.weight ? go(int32_t{}, std::true_type{}) : go(int32_t{}, std::false_type{});
-        });
+        return with_type(g.out_type, [&](auto o) { return launch_typed<decltype(t), decltype(o)>(g, a, stream); });
     });
 }
 
