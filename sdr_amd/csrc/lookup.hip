@@ -8,7 +8,7 @@
 // that contributes nothing has an offset there and a weight of 0, and needs no branch.  (Matrices beyond 2 GiB, or not aligned
 // to 4 bytes, are read by address.)
 // Short segments (tokens): whole waves, four slices at once, one element a turn: a copy, bound by HBM.
-// Long segments (codes): L = 8, 128 bytes of a row.  A table's slice of 128 bytes times its rows fits the 4 MiB of an XCD's L2
+// Long segments (codes): L = 8, 128 bytes of a row, eight elements in flight.  A table's slice of 128 bytes times its rows fits the 4 MiB of an XCD's L2
 // where the whole does not, so each XCD (block number modulo 8) works through the slices of its own, one after another.
 // S groups share a segment where there are too few of them to fill the chip, and join their sums in LDS.
 // A segment of more than `chunk` elements would keep its group busy long after the others: its elements are summed by groups
@@ -65,23 +65,38 @@ __device__ __forceinline__ uint32_t from_lane(uint32_t v, uint32_t lane) {
 
 // Where a group stands: its segment (or chunk), its part of the segment, and its lane's columns.  A lane whose columns would run
 // past the end reads the last V columns instead and stores only what is its own (from `own`).
-template <int V, int SL>
+// LANES: L where it is known at compile time, else 0
+template <int LANES>
+__device__ __forceinline__ uint32_t lanes_log2(const GatherArgs& a) {
+    if constexpr (LANES == 8) return 3;
+    if constexpr (LANES == 64) return 6;
+    return a.lanes_log2;
+}
+template <int V, int SL, int LANES>
 struct Place {
     uint64_t item;
     uint32_t lane, part;
     uint32_t col[SL], own[SL];
     bool live;
 
-    __device__ __forceinline__ Place(const GatherArgs& a, uint64_t n_items) {
-        const uint32_t lanes = 1u << a.lanes_log2, group = threadIdx.x >> a.lanes_log2;
-        const uint32_t items = (kThreads >> a.lanes_log2) >> a.split_log2;   // of a block
-        lane = threadIdx.x & (lanes - 1);
-        part = group & ((1u << a.split_log2) - 1);
+    __device__ __forceinline__ Place(const GatherArgs& a, uint32_t slice, uint64_t of) : item(of), live(slice < a.slices) {
+        const uint32_t l = lanes_log2<LANES>(a);
+        lane = threadIdx.x & ((1u << l) - 1);
+        part = (threadIdx.x >> l) & ((1u << a.split_log2) - 1);
+#pragma unroll
+        for (int j = 0; j < SL; ++j) {
+            own[j] = (((slice * SL + j) << l) + lane) * V;
+            col[j] = own[j] + V <= a.dim ? own[j] : a.dim - V;
+        }
+    }
+    // of the segments' groups: blocks of one slice each
+    __device__ __forceinline__ static Place of_segments(const GatherArgs& a) {
+        const uint32_t l = lanes_log2<LANES>(a), items = kThreads >> l >> a.split_log2;   // of a block
         uint32_t slice;
         uint64_t block;
         if (a.xcd_slices) {
-            // XCD x takes the slices x, x + 8, ..., one after another over all segments (slices: a multiple of 8), or its share
-            // of one slice's segments (slices: 1, 2 or 4)
+            // XCD x takes the slices x, x + 8, ..., one after another over all segments (slices: 8 or more), or its share of
+            // one slice's segments (slices: 1, 2 or 4)
             const uint32_t xcd = blockIdx.x & 7, turn = blockIdx.x >> 3;
             if (a.slices >= 8) {
                 slice = xcd + 8 * (turn / a.blocks);
@@ -94,13 +109,9 @@ struct Place {
             slice = blockIdx.x % a.slices;
             block = blockIdx.x / a.slices;
         }
-        item = block * items + (group >> a.split_log2);
-        live = item < n_items && slice < a.slices;
-#pragma unroll
-        for (int j = 0; j < SL; ++j) {
-            own[j] = (((slice * SL + j) << a.lanes_log2) + lane) * V;
-            col[j] = own[j] + V <= a.dim ? own[j] : a.dim - V;
-        }
+        Place p(a, slice, block * items + (threadIdx.x >> l >> a.split_log2));
+        p.live = p.live && p.item < a.n_segments;
+        return p;
     }
     __device__ __forceinline__ bool stores(const GatherArgs& a, int j) const { return own[j] < a.dim; }
 };
@@ -128,30 +139,37 @@ __device__ __forceinline__ void load_at(__amdgpu_buffer_rsrc_t src, uint32_t off
     for (int k = 0; k < V; ++k) v[k] = to_f32(t[k]);
 }
 
-// acc += the elements [lo, hi) of the list, as far as this part of the segment goes.  U elements a turn.
-template <int V, int SL, int U, bool BUFFER, typename T>
-__device__ __forceinline__ void add_elements(const GatherArgs& a, const Place<V, SL>& at, const T* __restrict__ src, uint64_t lo,
+// acc += the elements [lo, hi) of the list, as far as this part of the segment goes.  U elements a turn (U divides L, or L
+// is smaller); the ids of the next L elements are on their way while these are added.
+template <int V, int SL, int LANES, int U, bool BUFFER, typename T>
+__device__ __forceinline__ void add_elements(const GatherArgs& a, const Place<V, SL, LANES>& at, const T* __restrict__ src, uint64_t lo,
                                              uint64_t hi, float (&acc)[SL][V]) {
-    const uint32_t lanes = 1u << a.lanes_log2, first = threadIdx.x & 63 & ~(lanes - 1);   // of the group
+    const uint32_t l = lanes_log2<LANES>(a), lanes = 1u << l, first = threadIdx.x & 63 & ~(lanes - 1);   // of the group
     const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(src), 0, (int)a.src_bytes, 0x00020000);
-    for (uint64_t p0 = lo + ((uint64_t)at.part << a.lanes_log2); p0 < hi; p0 += (uint64_t)lanes << a.split_log2) {
-        const uint64_t p = p0 + at.lane;
-        uint64_t id = ~0ull;
-        if (p < hi) id = a.wide_index ? static_cast<const uint64_t*>(a.index)[p] : (uint64_t)(int64_t) static_cast<const int32_t*>(a.index)[p];
+    const auto id_at = [&](uint64_t p) {
+        return a.wide_index ? static_cast<const uint64_t*>(a.index)[p] : (uint64_t)(int64_t) static_cast<const int32_t*>(a.index)[p];
+    };
+    const uint64_t step = (uint64_t)lanes << a.split_log2;
+    uint64_t p = lo + ((uint64_t)at.part << l) + at.lane;
+    uint64_t id = p < hi ? id_at(p) : ~0ull;
+    float weight = a.weight && p < hi ? a.weight[p] : 1.0f;
+    for (uint64_t p0 = p - at.lane; p0 < hi; p0 += step) {
         const bool in = id < a.src_rows;   // (a negative id is a large one)
-        float w = 0.0f;
-        if (in) w = a.weight ? a.weight[p] : 1.0f;
-        const uint32_t offset = BUFFER ? (in ? (uint32_t)id * a.row_bytes : kNowhere) : (in ? (uint32_t)id : kNowhere);
+        const uint32_t offset = in ? (BUFFER ? (uint32_t)id * a.row_bytes : (uint32_t)id) : kNowhere;
+        const float w = in ? weight : 0.0f;
+        p += step;
+        id = p < hi ? id_at(p) : ~0ull;
+        if (a.weight) weight = p < hi ? a.weight[p] : 0.0f;
         const uint32_t n = hi - p0 < lanes ? (uint32_t)(hi - p0) : lanes;
         for (uint32_t u = 0; u < n; u += U) {
             float v[U][SL][V], wu[U];
 #pragma unroll
             for (int j = 0; j < U; ++j) {
-                // (lanes beyond n, and beyond the group where U is larger, hold no element)
-                const uint32_t from = first + (U > 1 && u + j >= lanes ? lanes - 1 : u + j);
+                const bool over = LANES == 0 && U > 1 && u + j >= lanes;   // (a group of fewer lanes than U)
+                const uint32_t from = over ? first : first + u + j;
                 uint32_t o = from_lane(offset, from);
                 wu[j] = __builtin_bit_cast(float, from_lane(__builtin_bit_cast(uint32_t, w), from));
-                if (U > 1 && u + j >= lanes) {
+                if (over) {
                     o = kNowhere;
                     wu[j] = 0.0f;
                 }
@@ -177,7 +195,7 @@ __device__ __forceinline__ void add_elements(const GatherArgs& a, const Place<V,
 }
 
 // The parts' sums, added up in order by the first of them.
-template <int V, int SL>
+template <int V, int SL, int LANES>
 __device__ __forceinline__ void join_parts(const GatherArgs& a, uint32_t part, float (&acc)[SL][V], float* shared) {
     const uint32_t parts = 1u << a.split_log2;
     if (parts == 1) return;
@@ -190,14 +208,14 @@ __device__ __forceinline__ void join_parts(const GatherArgs& a, uint32_t part, f
         if (part == 0)
             for (uint32_t s = 1; s < parts; ++s)
 #pragma unroll
-                for (int c = 0; c < V; ++c) acc[k][c] += shared[c * kThreads + threadIdx.x + (s << a.lanes_log2)];
+                for (int c = 0; c < V; ++c) acc[k][c] += shared[c * kThreads + threadIdx.x + (s << lanes_log2<LANES>(a))];
     }
 }
 
-template <int V, int SL, int U, bool BUFFER, typename T, typename O>
+template <int V, int SL, int LANES, int U, bool BUFFER, typename T, typename O>
 __global__ __launch_bounds__(kThreads) void k_gather_rows(GatherArgs a, const T* __restrict__ src, O* __restrict__ out) {
     __shared__ float shared[V * kThreads];
-    const Place<V, SL> at(a, a.n_segments);
+    const Place<V, SL, LANES> at = Place<V, SL, LANES>::of_segments(a);
     uint64_t lo = 0, hi = 0;
     if (at.live) segment_of(a, at.item, lo, hi);
     float acc[SL][V];
@@ -219,9 +237,9 @@ __global__ __launch_bounds__(kThreads) void k_gather_rows(GatherArgs a, const T*
                 }
             }
     } else {
-        add_elements<V, SL, U, BUFFER>(a, at, src, lo, hi, acc);
+        add_elements<V, SL, LANES, U, BUFFER>(a, at, src, lo, hi, acc);
     }
-    join_parts<V, SL>(a, at.part, acc, shared);
+    join_parts<V, SL, LANES>(a, at.part, acc, shared);
     if (!at.live || at.part != 0 || (a.accumulate && lo == hi)) return;
 #pragma unroll
     for (int k = 0; k < SL; ++k) {
@@ -247,60 +265,57 @@ __global__ __launch_bounds__(kThreads) void k_gather_rows(GatherArgs a, const T*
     }
 }
 
-// last segment whose first element is at or before p (p < n_elems): the one that holds p, empty segments being passed over
+// The segment that holds element p (p < n_elems) is the last one whose first element is at or before p.  A wave looks at 64
+// segments a step.
 __device__ __forceinline__ uint64_t segment_at(const uint32_t* __restrict__ start, uint64_t n_segments, uint64_t p) {
-    uint64_t lo = 0, hi = n_segments;
-    while (hi - lo > 1) {
-        const uint64_t mid = (lo + hi) >> 1;
-        if (start[mid] <= p) lo = mid;
-        else hi = mid;
+    uint64_t lo = 0, n = n_segments;   // it is one of [lo, lo + n)
+    while (n > 1) {
+        const uint64_t stride = (n + 63) / 64, at = lo + (threadIdx.x & 63) * stride;
+        const bool reached = at < lo + n && start[at] <= p;
+        const uint64_t last = (uint64_t)__builtin_popcountll(__builtin_amdgcn_ballot_w64(reached));   // lane 0 always, unless p is before all
+        const uint64_t step = last ? (last - 1) * stride : 0;
+        n = n - step < stride ? n - step : stride;
+        lo += step;
     }
     return lo;
 }
 
-// the sums that chunk c of the element list contributes to segments longer than a chunk
-template <int V, int SL, int U, bool BUFFER, typename T>
-__global__ __launch_bounds__(kThreads) void k_gather_chunks(GatherArgs a, const T* __restrict__ src, uint64_t n_chunks) {
+// The sums that chunk c of the element list contributes to segments longer than a chunk.  A block takes a chunk and
+// some of the slices; its groups of 8 lanes are parts of the chunk.  Where no segment is long, it finds that and ends.
+template <int V, int LANES, int U, bool BUFFER, typename T>
+__global__ __launch_bounds__(kThreads) void k_gather_chunks(GatherArgs a, const T* __restrict__ src) {
     __shared__ float shared[V * kThreads];
-    const Place<V, SL> at(a, n_chunks);
-    const uint64_t c_lo = at.item * a.chunk, c_hi = c_lo + a.chunk < a.n_elems ? c_lo + a.chunk : a.n_elems;
+    const uint32_t l = lanes_log2<LANES>(a), group = threadIdx.x >> l, per_block = kThreads >> l >> a.split_log2;   // slices
+    const uint64_t c = blockIdx.x / a.blocks;
+    const Place<V, 1, LANES> at(a, (blockIdx.x % a.blocks) * per_block + (group >> a.split_log2), c);
+    const uint64_t c_lo = c * a.chunk, c_hi = c_lo + a.chunk < a.n_elems ? c_lo + a.chunk : a.n_elems;
 #pragma unroll 1
     for (int end = 0; end < 2; ++end) {
-        uint64_t lo = 0, hi = 0;
-        if (at.live) {
-            if (a.start) {
-                segment_of(a, segment_at(a.start, a.n_segments, end ? c_hi - 1 : c_lo), lo, hi);
+        uint64_t lo, hi;
+        if (a.start) {
+            segment_of(a, segment_at(a.start, a.n_segments, end ? c_hi - 1 : c_lo), lo, hi);
+        } else {
+            lo = (end ? c_hi - 1 : c_lo) / a.row_len * a.row_len;
+            hi = lo + a.row_len;
+        }
+        if (hi - lo <= a.chunk || (end && lo <= c_lo)) continue;   // short, or the first element's segment once more
+        float acc[1][V];
+#pragma unroll
+        for (int k = 0; k < V; ++k) acc[0][k] = 0.0f;
+        if (at.live) add_elements<V, 1, LANES, U, BUFFER>(a, at, src, lo > c_lo ? lo : c_lo, hi < c_hi ? hi : c_hi, acc);
+        join_parts<V, 1, LANES>(a, at.part, acc, shared);
+        if (at.part == 0 && at.stores(a, 0)) {
+            float* to = a.partials + (2 * c + end) * a.dim + at.col[0];
+            if (at.col[0] == at.own[0]) {
+                store_n<V>(to, acc[0]);
             } else {
-                lo = (end ? c_hi - 1 : c_lo) / a.row_len * a.row_len;
-                hi = lo + a.row_len;
+                const uint32_t skip = at.own[0] - at.col[0];
+#pragma unroll
+                for (int k = 0; k < V; ++k)
+                    if ((uint32_t)k >= skip) to[k] = acc[0][k];
             }
-            if (hi - lo <= a.chunk || (end && lo <= c_lo)) lo = hi = 0;   // short, or the first element's segment once more
         }
-        const bool any = lo < hi;
-        float acc[SL][V];
-#pragma unroll
-        for (int k = 0; k < SL; ++k)
-#pragma unroll
-            for (int c = 0; c < V; ++c) acc[k][c] = 0.0f;
-        if (a.split_log2 ? __syncthreads_or(any) : any) {
-            if (any) add_elements<V, SL, U, BUFFER>(a, at, src, lo > c_lo ? lo : c_lo, hi < c_hi ? hi : c_hi, acc);
-            join_parts<V, SL>(a, at.part, acc, shared);
-            if (any && at.part == 0)
-#pragma unroll
-                for (int k = 0; k < SL; ++k) {
-                    if (!at.stores(a, k)) break;
-                    float* to = a.partials + (2 * at.item + end) * a.dim + at.col[k];
-                    if (at.col[k] == at.own[k]) {
-                        store_n<V>(to, acc[k]);
-                    } else {
-                        const uint32_t skip = at.own[k] - at.col[k];
-#pragma unroll
-                        for (int c = 0; c < V; ++c)
-                            if ((uint32_t)c >= skip) to[c] = acc[k][c];
-                    }
-                }
-            if (a.split_log2) __syncthreads();
-        }
+        __syncthreads();
     }
 }
 
@@ -319,67 +334,80 @@ uint32_t log2_of(uint64_t v) {
     return l;
 }
 
-template <int V, int SL, int U, bool BUFFER, typename T, typename O>
-int launch_shaped(const GatherSum& g, GatherArgs a, uint64_t mean, hipStream_t stream) {
-    const T* src = static_cast<const T*>(g.src);
-    const uint64_t vectors = (a.dim + V - 1) / V;
-    // lanes of a group: a wave, or 128 bytes of a row for long segments; no more than the row has vectors
-    a.lanes_log2 = std::min<uint32_t>(U == 1 ? 6 : 3, log2_of(vectors > 1 ? 2 * vectors - 1 : 1));
-    const uint64_t a_slice = (uint64_t)SL << a.lanes_log2;
-    a.slices = (uint32_t)((vectors + a_slice - 1) / a_slice);
-    const auto run = [&](auto kernel, GatherArgs b, uint64_t items, uint64_t each, auto... more) {
-        // S: waves for the whole chip, eight a SIMD, as long as every part has elements to add
-        const uint64_t groups = items * b.slices, enough = (uint64_t)1024 * 8 * (64u >> b.lanes_log2);
-        b.split_log2 = 0;
-        while ((kThreads >> b.lanes_log2 >> b.split_log2) > 1 && (groups << b.split_log2) < enough && (1ull << b.split_log2) << b.lanes_log2 < each)
-            ++b.split_log2;
-        const uint64_t per_block = kThreads >> b.lanes_log2 >> b.split_log2, blocks = (items + per_block - 1) / per_block;
-        uint64_t grid = blocks * b.slices;
-        b.xcd_slices = 0;
-        b.blocks = (uint32_t)blocks;
-        if (U > 1 && blocks >= 8) {
-            if (b.slices >= 8) {
-                b.xcd_slices = 1;
-                grid = blocks * ((b.slices + 7) / 8 * 8);
-            } else if ((b.slices & (b.slices - 1)) == 0) {
-                b.xcd_slices = 1;
-                grid = (blocks + 8 / b.slices - 1) / (8 / b.slices) * 8;
-            }
-        }
-        if (grid > 0x7FFFFFFFull) {
-            set_error("too many rows and columns for one launch");
-            return SDRB_ERR_OVERFLOW;
-        }
-        hipLaunchKernelGGL(kernel, dim3((uint32_t)grid), dim3(kThreads), 0, stream, b, src, more...);
-        SDRB_HIP(hipGetLastError());
-        return SDRB_OK;
-    };
-    if (a.chunk) {
-        const uint64_t n_chunks = (g.n_elems + a.chunk - 1) / a.chunk;
-        if (const int rc = run(k_gather_chunks<V, SL, U, BUFFER, T>, a, n_chunks, (uint64_t)a.chunk, n_chunks)) return rc;
+// lanes of a group: `most`, but no more than the row has vectors
+uint32_t group_log2(uint32_t most, uint64_t vectors) { return std::min<uint32_t>(most, log2_of(vectors > 1 ? 2 * vectors - 1 : 1)); }
+
+template <int V, int LANES, bool BUFFER, typename T>
+int launch_chunks(const GatherSum& g, GatherArgs a, hipStream_t stream) {
+    const uint64_t n_chunks = (g.n_elems + a.chunk - 1) / a.chunk, vectors = (a.dim + V - 1) / V;
+    a.lanes_log2 = group_log2(3, vectors);
+    const uint32_t groups = kThreads >> a.lanes_log2;
+    a.split_log2 = std::min<uint32_t>(log2_of(groups), log2_of(std::max<uint32_t>(a.chunk >> a.lanes_log2, 1)));
+    a.slices = (uint32_t)((vectors + (1u << a.lanes_log2) - 1) >> a.lanes_log2);
+    while (a.split_log2 > 2 && (groups >> a.split_log2) < a.slices) --a.split_log2;
+    const uint32_t per_block = groups >> a.split_log2;
+    a.blocks = (a.slices + per_block - 1) / per_block;   // of a chunk
+    a.xcd_slices = 0;
+    if (n_chunks * a.blocks > 0x7FFFFFFFull) {
+        set_error("too many elements and columns for one launch");
+        return SDRB_ERR_OVERFLOW;
     }
-    return run(k_gather_rows<V, SL, U, BUFFER, T, O>, a, g.n_segments, mean, static_cast<O*>(g.out));
+    hipLaunchKernelGGL((k_gather_chunks<V, LANES, 8, BUFFER, T>), dim3((uint32_t)(n_chunks * a.blocks)), dim3(kThreads), 0, stream, a,
+                       static_cast<const T*>(g.src));
+    SDRB_HIP(hipGetLastError());
+    return SDRB_OK;
 }
 
-template <typename T, typename O>
+template <int V, int SL, int LANES, int U, bool BUFFER, typename T, typename O>
+int launch_rows(const GatherSum& g, GatherArgs a, uint64_t mean, hipStream_t stream) {
+    const uint64_t vectors = (a.dim + V - 1) / V;
+    a.lanes_log2 = LANES ? log2_of(LANES) : group_log2(U == 1 ? 6 : 3, vectors);
+    const uint64_t a_slice = (uint64_t)SL << a.lanes_log2;
+    a.slices = (uint32_t)((vectors + a_slice - 1) / a_slice);
+    // S: waves for the whole chip, eight a SIMD, as long as every part has elements to add
+    const uint64_t groups = g.n_segments * a.slices, enough = (uint64_t)1024 * 8 * (64u >> a.lanes_log2);
+    a.split_log2 = 0;
+    while ((kThreads >> a.lanes_log2 >> a.split_log2) > 1 && (groups << a.split_log2) < enough && (1ull << a.split_log2) << a.lanes_log2 < mean)
+        ++a.split_log2;
+    const uint64_t per_block = kThreads >> a.lanes_log2 >> a.split_log2, blocks = (g.n_segments + per_block - 1) / per_block;
+    uint64_t grid = blocks * a.slices;
+    a.xcd_slices = 0;
+    a.blocks = (uint32_t)blocks;
+    if (U > 1 && blocks >= 8) {
+        if (a.slices >= 8) {
+            a.xcd_slices = 1;
+            grid = blocks * ((a.slices + 7) / 8 * 8);
+        } else if ((a.slices & (a.slices - 1)) == 0) {
+            a.xcd_slices = 1;
+            grid = (blocks + 8 / a.slices - 1) / (8 / a.slices) * 8;
+        }
+    }
+    if (grid > 0x7FFFFFFFull) {
+        set_error("too many rows and columns for one launch");
+        return SDRB_ERR_OVERFLOW;
+    }
+    hipLaunchKernelGGL((k_gather_rows<V, SL, LANES, U, BUFFER, T, O>), dim3((uint32_t)grid), dim3(kThreads), 0, stream, a,
+                       static_cast<const T*>(g.src), static_cast<O*>(g.out));
+    SDRB_HIP(hipGetLastError());
+    return SDRB_OK;
+}
+
+template <bool BUFFER, typename T, typename O>
 int launch_typed(const GatherSum& g, GatherArgs a, hipStream_t stream) {
+    // long segments read more than they write: 16 bytes a load; short ones: 16 bytes at most a load or store
     constexpr int kWide = 16 / sizeof(T), kEven = 16 / (sizeof(T) > sizeof(O) ? sizeof(T) : sizeof(O));
     const uint64_t mean = g.n_elems / g.n_segments;
-    const uint64_t bytes = g.src_rows ? ((g.src_rows - 1) * g.src_ld + a.dim) * sizeof(T) : 0;
-    const bool buffer = bytes < kNowhere && reinterpret_cast<uintptr_t>(g.src) % 4 == 0 && g.src_ld * sizeof(T) % 4 == 0 && a.dim >= (uint32_t)kWide &&
-                        a.dim * sizeof(T) % 4 == 0;
-    a.row_bytes = (uint32_t)(g.src_ld * sizeof(T));
-    a.src_bytes = (uint32_t)bytes;
-    if (buffer) {
-        // long segments read more than they write: 16 bytes a load; short ones: 16 bytes at most a load or store
-        if (mean >= 3) return launch_shaped<kWide, 1, 4, true, T, O>(g, a, mean, stream);
-        return launch_shaped<kEven, 4, 1, true, T, O>(g, a, mean, stream);
+    const bool full = a.dim >= 8u * kWide;   // eight lanes have vectors
+    if (a.chunk) {
+        const int rc = full ? launch_chunks<kWide, 8, BUFFER, T>(g, a, stream) : launch_chunks<kWide, 0, BUFFER, T>(g, a, stream);
+        if (rc != SDRB_OK) return rc;
     }
-    if (a.dim >= (uint32_t)kWide) {
-        if (mean >= 3) return launch_shaped<kWide, 1, 4, false, T, O>(g, a, mean, stream);
-        return launch_shaped<kEven, 4, 1, false, T, O>(g, a, mean, stream);
+    if (mean >= 3) {
+        if (full) return launch_rows<kWide, 1, 8, 8, BUFFER, T, O>(g, a, mean, stream);
+        return launch_rows<kWide, 1, 0, 4, BUFFER, T, O>(g, a, mean, stream);
     }
-    return launch_shaped<1, 1, 1, false, T, O>(g, a, mean, stream);
+    if (a.dim >= 64u * kEven) return launch_rows<kEven, 4, 64, 1, BUFFER, T, O>(g, a, mean, stream);
+    return launch_rows<kEven, 1, 0, 1, BUFFER, T, O>(g, a, mean, stream);
 }
 
 }  // namespace
@@ -411,7 +439,22 @@ int launch_gather_sum(const GatherSum& g, hipStream_t stream) {
     a.chunk = g.partials ? chunk_of(g.n_segments, g.n_elems) : 0u;
     a.accumulate = g.accumulate ? 1u : 0u;
     return with_type(g.src_type, [&](auto t) {
-        return with_type(g.out_type, [&](auto o) { return launch_typed<decltype(t), decltype(o)>(g, a, stream); });
+        return with_type(g.out_type, [&](auto o) {
+            using T = decltype(t);
+            using O = decltype(o);
+            constexpr uint32_t kWide = 16 / sizeof(T);
+            const uint64_t bytes = g.src_rows ? ((g.src_rows - 1) * g.src_ld + a.dim) * sizeof(T) : 0;
+            const bool by_words = reinterpret_cast<uintptr_t>(g.src) % 4 == 0 && g.src_ld * sizeof(T) % 4 == 0 && a.dim * sizeof(T) % 4 == 0;
+            if (a.dim < kWide) {   // narrower than a load: a column a lane
+                if (a.chunk)
+                    if (const int rc = launch_chunks<1, 0, false, T>(g, a, stream)) return rc;
+                return launch_rows<1, 1, 0, 1, false, T, O>(g, a, g.n_elems / g.n_segments, stream);
+            }
+            if (bytes >= kNowhere || !by_words) return launch_typed<false, T, O>(g, a, stream);
+            a.row_bytes = (uint32_t)(g.src_ld * sizeof(T));
+            a.src_bytes = (uint32_t)bytes;
+            return launch_typed<true, T, O>(g, a, stream);
+        });
     });
 }
 
