@@ -44,6 +44,13 @@ int with_type(int type, F&& f) {
         default: return f(float{});
     }
 }
+// more than 64 KiB of LDS, all in all, has to be asked for
+template <typename F>
+int allow_lds(F* kernel, size_t dynamic_bytes) {
+    if (dynamic_bytes > 49152)
+        SDRB_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)dynamic_bytes));
+    return SDRB_OK;
+}
 inline size_t type_size(int type) { return type == SDRB_F32 ? 4 : 2; }
 
 // A ragged sum: out[s, :] (+)= scale * sum over p in [start[s], start[s+1]) of weight[p] * src[index[p], :].
@@ -72,7 +79,7 @@ size_t gather_partial_bytes(uint64_t n_segments, uint64_t n_elems, bool ragged, 
 int launch_gather_sum(const GatherSum& g, hipStream_t stream);
 
 // lookup_grad.hip
-size_t table_grad_scratch_bytes(uint64_t n_elems, uint64_t n_table_rows, uint32_t dim);
+size_t table_grad_scratch_bytes(uint64_t n_elems, uint64_t n_table_rows, bool weighted, uint32_t dim);
 int launch_table_grad(int device, const sdrb_rows& rows, const sdrb_dense& grad, float scale, bool accumulate,
                       const sdrb_dense& out, void* scratch, hipStream_t stream);
 int launch_weight_grad(const sdrb_rows& rows, const sdrb_dense& grad, const sdrb_dense& table, float scale, float* out,

@@ -8,8 +8,10 @@
 // that contributes nothing has an offset there and a weight of 0, and needs no branch.  (Matrices beyond 2 GiB, or not aligned
 // to 4 bytes, are read by address.)
 // Short segments (tokens): whole waves, four slices at once, one element a turn: a copy, bound by HBM.
-// Long segments (codes): L = 8, 128 bytes of a row, eight elements in flight.  A table's slice of 128 bytes times its rows fits the 4 MiB of an XCD's L2
-// where the whole does not, so each XCD (block number modulo 8) works through the slices of its own, one after another.
+// Long segments (codes): L = 16, two slices of 256 bytes a lane's turn, four elements in flight: bound by L2.  Each XCD (block
+// number modulo 8) works through slices of its own, one after another: 512 bytes of every row of a table are what its L2 has
+// to hold at a time, not the whole table.  Measured on 4096 rows of 328 of 16384 ids, 1024 bf16 columns (2.75 GB read):
+// 126 us = 22 TB/s; slices of 128 bytes 175 us, 256 bytes 138 us, one slice of 1 KiB for all XCDs 226 us.
 // S groups share a segment where there are too few of them to fill the chip, and join their sums in LDS.
 // A segment of more than `chunk` elements would keep its group busy long after the others: its elements are summed by groups
 // that own a chunk of the element list each (k_gather_chunks), and the segment's own group adds those sums up in order.
@@ -69,6 +71,7 @@ __device__ __forceinline__ uint32_t from_lane(uint32_t v, uint32_t lane) {
 template <int LANES>
 __device__ __forceinline__ uint32_t lanes_log2(const GatherArgs& a) {
     if constexpr (LANES == 8) return 3;
+    if constexpr (LANES == 16) return 4;
     if constexpr (LANES == 64) return 6;
     return a.lanes_log2;
 }
@@ -361,7 +364,7 @@ int launch_chunks(const GatherSum& g, GatherArgs a, hipStream_t stream) {
 template <int V, int SL, int LANES, int U, bool BUFFER, typename T, typename O>
 int launch_rows(const GatherSum& g, GatherArgs a, uint64_t mean, hipStream_t stream) {
     const uint64_t vectors = (a.dim + V - 1) / V;
-    a.lanes_log2 = LANES ? log2_of(LANES) : group_log2(U == 1 ? 6 : 3, vectors);
+    a.lanes_log2 = LANES ? log2_of(LANES) : group_log2(U == 1 ? 6 : 4, vectors);
     const uint64_t a_slice = (uint64_t)SL << a.lanes_log2;
     a.slices = (uint32_t)((vectors + a_slice - 1) / a_slice);
     // S: waves for the whole chip, eight a SIMD, as long as every part has elements to add
@@ -397,13 +400,13 @@ int launch_typed(const GatherSum& g, GatherArgs a, hipStream_t stream) {
     // long segments read more than they write: 16 bytes a load; short ones: 16 bytes at most a load or store
     constexpr int kWide = 16 / sizeof(T), kEven = 16 / (sizeof(T) > sizeof(O) ? sizeof(T) : sizeof(O));
     const uint64_t mean = g.n_elems / g.n_segments;
-    const bool full = a.dim >= 8u * kWide;   // eight lanes have vectors
     if (a.chunk) {
-        const int rc = full ? launch_chunks<kWide, 8, BUFFER, T>(g, a, stream) : launch_chunks<kWide, 0, BUFFER, T>(g, a, stream);
+        const int rc = a.dim >= 8u * kWide ? launch_chunks<kWide, 8, BUFFER, T>(g, a, stream) : launch_chunks<kWide, 0, BUFFER, T>(g, a, stream);
         if (rc != SDRB_OK) return rc;
     }
     if (mean >= 3) {
-        if (full) return launch_rows<kWide, 1, 8, 8, BUFFER, T, O>(g, a, mean, stream);
+        if (a.dim >= 32u * kWide) return launch_rows<kWide, 2, 16, 4, BUFFER, T, O>(g, a, mean, stream);
+        if (a.dim >= 16u * kWide) return launch_rows<kWide, 1, 16, 8, BUFFER, T, O>(g, a, mean, stream);
         return launch_rows<kWide, 1, 0, 4, BUFFER, T, O>(g, a, mean, stream);
     }
     if (a.dim >= 64u * kEven) return launch_rows<kEven, 4, 64, 1, BUFFER, T, O>(g, a, mean, stream);

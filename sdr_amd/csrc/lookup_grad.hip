@@ -5,17 +5,41 @@
 // sorted list like a lookup whose rows are the ids (lookup.hip): no atomic addition, the same bits every time, and the
 // work of an id that many rows hold is shared out.
 // To the weights: d w[e] = scale * <d out[row(e), :], table[id[e], :]>, a dot product an element.
+#include <algorithm>
+
 #include "dense_rows.h"
 
 namespace sdrb {
 
 namespace {
 
-constexpr uint32_t kTile = 2048, kDigitBits = 8, kDigits = 1u << kDigitBits, kWaves = 4, kPerWave = kTile / kWaves;
+// ---- sorting elements by id ---------------------------------------------------------------------------------------------
+// Keys are ids, or n_table_rows for an element that contributes nothing (an id outside the table, or an element that no row
+// holds), so they take bits(n_table_rows).  A pass sorts by a digit of them, stably: the 64 elements of a wave's turn find
+// the others of their digit by a ballot a digit bit, and a wave counts in LDS what its earlier turns have seen of each digit.
+//
+// Up to 16384 elements one block does it all in LDS (k_sort_small), 8 bits a pass, the elements in registers between passes:
+// every further launch costs more than a pass.  More elements take three launches a pass: digits counted by tile, the
+// counts summed over tiles, and the elements sent to their places.  Digits have up to 12 bits there, so that ids below
+// 4096 -- the widths of sparse codes -- need one pass, and then the counts are the segments' starts too.
 
+struct SortArgs {
+    const void* ids;
+    const uint32_t* off;     // row offsets, or null: rows of row_len
+    const float* weight;     // or null
+    uint64_t n, n_keys, n_rows;
+    uint32_t row_len, wide;  // wide: 64-bit ids
+    uint32_t key_bits;
+};
+
+__device__ __forceinline__ uint32_t key_of(const SortArgs& a, uint64_t e) {
+    const uint64_t id = a.wide ? static_cast<const uint64_t*>(a.ids)[e] : (uint64_t)(int64_t) static_cast<const int32_t*>(a.ids)[e];
+    const bool in = id < a.n_keys && (!a.off || (e >= a.off[0] && e < a.off[a.n_rows]));   // (a negative id is a large one)
+    return in ? (uint32_t)id : (uint32_t)a.n_keys;
+}
 // the row of element e
 __device__ __forceinline__ uint32_t row_of(const uint32_t* __restrict__ off, uint64_t n_rows, uint32_t row_len, uint64_t e) {
-    if (!off) return (uint32_t)(e / row_len);
+    if (!off) return (uint32_t)e / row_len;
     uint64_t lo = 0, hi = n_rows;   // last row that starts at or before e
     while (hi - lo > 1) {
         const uint64_t mid = (lo + hi) >> 1;
@@ -24,101 +48,239 @@ __device__ __forceinline__ uint32_t row_of(const uint32_t* __restrict__ off, uin
     }
     return (uint32_t)lo;
 }
-
-// Elements as sort keys: the id, or n_table_rows for an element that contributes nothing (an id outside the table, or an
-// element behind the last row).
-template <typename Id>
-__global__ __launch_bounds__(256) void k_keys(const Id* __restrict__ ids, uint64_t n, uint64_t n_table_rows,
-                                              const uint32_t* __restrict__ off, uint64_t n_rows, uint32_t* __restrict__ keys,
-                                              uint32_t* __restrict__ elems) {
-    const uint64_t e = (uint64_t)blockIdx.x * 256 + threadIdx.x;
-    if (e >= n) return;
-    const Id id = ids[e];
-    const bool in = id >= 0 && (uint64_t)id < n_table_rows && (!off || (e >= off[0] && e < off[n_rows]));
-    keys[e] = in ? (uint32_t)id : (uint32_t)n_table_rows;
-    elems[e] = (uint32_t)e;
+__device__ __forceinline__ uint32_t lanes_below(unsigned long long mask) {
+    return __builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0u));
 }
-
-// counts[digit * n_tiles + tile]: keys of the tile whose digit is `digit`
-__global__ __launch_bounds__(256) void k_count(const uint32_t* __restrict__ keys, uint64_t n, uint32_t shift, uint32_t n_tiles,
-                                               uint32_t* __restrict__ counts) {
-    __shared__ uint32_t h[kDigits];
-    h[threadIdx.x] = 0;
-    __syncthreads();
-    const uint64_t t0 = (uint64_t)blockIdx.x * kTile;
-    for (uint32_t i = threadIdx.x; i < kTile && t0 + i < n; i += 256) atomicAdd(&h[(keys[t0 + i] >> shift) & (kDigits - 1)], 1u);
-    __syncthreads();
-    counts[(uint64_t)threadIdx.x * n_tiles + blockIdx.x] = h[threadIdx.x];
+// the lanes of the wave that hold the same digit, of those that are live
+__device__ __forceinline__ unsigned long long same_digit(uint32_t digit, uint32_t bits, bool live) {
+    unsigned long long same = __builtin_amdgcn_ballot_w64(live);
+    for (uint32_t b = 0; b < bits; ++b) {
+        const bool set = (digit >> b) & 1u;
+        const unsigned long long with = __builtin_amdgcn_ballot_w64(set);
+        same &= set ? with : ~with;
+    }
+    return same;
 }
-
-// in-place exclusive prefix sum by one block
-__global__ __launch_bounds__(1024) void k_scan(uint32_t* __restrict__ data, uint64_t n) {
-    __shared__ uint32_t waves[16];
-    uint32_t carry = 0;
-    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    for (uint64_t base = 0; base < n; base += 1024) {
-        const uint64_t i = base + threadIdx.x;
-        const uint32_t v = i < n ? data[i] : 0u;
-        uint32_t sum = v;
+// Of equal digits, what the wave's earlier turns and the lower lanes hold; counter[digit] goes up by this turn's.
+__device__ __forceinline__ uint32_t rank_in_wave(uint32_t* counter, uint32_t digit, uint32_t bits, bool live) {
+    const unsigned long long same = same_digit(digit, bits, live);
+    const uint32_t below = lanes_below(same);
+    uint32_t before = 0;
+    if (live) before = counter[digit];
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");   // all have read before the first of them writes
+    __builtin_amdgcn_wave_barrier();
+    if (live && below == 0) counter[digit] = before + (uint32_t)__builtin_popcountll(same);
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    return before + below;
+}
+// inclusive sums over the lanes of a wave
+__device__ __forceinline__ uint32_t scan_lanes(uint32_t v) {
+    const uint32_t lane = threadIdx.x & 63;
 #pragma unroll
-        for (uint32_t s = 1; s < 64; s <<= 1) {
-            const uint32_t below = (uint32_t)__shfl_up((int)sum, s, 64);
-            if (lane >= s) sum += below;
+    for (uint32_t s = 1; s < 64; s <<= 1) {
+        const uint32_t below = (uint32_t)__shfl_up((int)v, s, 64);
+        if (lane >= s) v += below;
+    }
+    return v;
+}
+
+constexpr uint32_t kSmall = 16384, kSmallThreads = 1024, kSmallWaves = kSmallThreads / 64, kSmallTurns = kSmall / kSmallThreads;
+constexpr uint64_t kStartsInSort = 4096;   // up to so many keys the one block finds their starts as well, four a thread
+
+__global__ __launch_bounds__(kSmallThreads) void k_sort_small(SortArgs a, uint32_t* __restrict__ keys_out, int32_t* __restrict__ row_out,
+                                                              float* __restrict__ weight_out, uint32_t* __restrict__ start) {
+    __shared__ uint32_t key_at[kSmall];
+    __shared__ uint16_t elem_at[kSmall];
+    __shared__ uint32_t counter[kSmallWaves][256];
+    __shared__ uint32_t digit_waves[4];
+    const uint32_t n = (uint32_t)a.n, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const uint32_t turns = (n + kSmallThreads - 1) / kSmallThreads;   // a wave owns turns * 64 neighbouring elements
+    uint32_t key[kSmallTurns], elem[kSmallTurns], place[kSmallTurns];
+#pragma unroll
+    for (uint32_t t = 0; t < kSmallTurns; ++t) {
+        elem[t] = (wave * turns + t) * 64 + lane;
+        key[t] = t < turns && elem[t] < n ? key_of(a, elem[t]) : 0u;
+    }
+    for (uint32_t shift = 0; shift < a.key_bits; shift += 8) {
+        const uint32_t bits = a.key_bits - shift < 8 ? a.key_bits - shift : 8;
+        for (uint32_t k = threadIdx.x; k < kSmallWaves * 256; k += kSmallThreads) counter[k >> 8][k & 255] = 0;
+        __syncthreads();
+#pragma unroll
+        for (uint32_t t = 0; t < kSmallTurns; ++t) {
+            if (t >= turns) break;
+            // (positions, not elements, say which lanes are live: after the first pass the last ones are the largest keys)
+            const bool live = (wave * turns + t) * 64 + lane < n;
+            place[t] = rank_in_wave(counter[wave], (key[t] >> shift) & 255u, bits, live);
         }
+        __syncthreads();
+        if (threadIdx.x < 256) {   // a digit a thread: sums over the waves, then over the digits
+            uint32_t total = 0;
+            for (uint32_t w = 0; w < kSmallWaves; ++w) {
+                const uint32_t here = counter[w][threadIdx.x];
+                counter[w][threadIdx.x] = total;
+                total += here;
+            }
+            const uint32_t sum = scan_lanes(total);
+            if (lane == 63) digit_waves[wave] = sum;
+            key_at[threadIdx.x] = sum - total;   // (its contents have been read)
+        }
+        __syncthreads();
+        if (threadIdx.x < 256) {
+            uint32_t before = key_at[threadIdx.x];
+            for (uint32_t w = 0; w < wave; ++w) before += digit_waves[w];
+            for (uint32_t w = 0; w < kSmallWaves; ++w) counter[w][threadIdx.x] += before;
+        }
+        __syncthreads();
+#pragma unroll
+        for (uint32_t t = 0; t < kSmallTurns; ++t) {
+            if (t >= turns) break;
+            if ((wave * turns + t) * 64 + lane < n) {
+                const uint32_t to = counter[wave][(key[t] >> shift) & 255u] + place[t];
+                key_at[to] = key[t];
+                elem_at[to] = (uint16_t)elem[t];
+            }
+        }
+        __syncthreads();
+#pragma unroll
+        for (uint32_t t = 0; t < kSmallTurns; ++t) {
+            if (t >= turns) break;
+            const uint32_t p = (wave * turns + t) * 64 + lane;
+            if (p < n) {
+                key[t] = key_at[p];
+                elem[t] = elem_at[p];
+            }
+        }
+        __syncthreads();
+    }
+#pragma unroll
+    for (uint32_t t = 0; t < kSmallTurns; ++t) {
+        if (t >= turns) break;
+        const uint32_t p = (wave * turns + t) * 64 + lane;
+        if (p < n) {
+            keys_out[p] = key[t];
+            row_out[p] = (int32_t)row_of(a.off, a.n_rows, a.row_len, elem[t]);
+            if (a.weight) weight_out[p] = a.weight[elem[t]];
+            key_at[p] = key[t];
+        }
+    }
+    if (a.n_keys > kStartsInSort) return;
+    __syncthreads();
+    for (uint32_t v = threadIdx.x; v <= a.n_keys; v += kSmallThreads) {
+        uint32_t lo = 0, hi = n;
+        while (lo < hi) {
+            const uint32_t mid = (lo + hi) >> 1;
+            if (key_at[mid] < v) lo = mid + 1;
+            else hi = mid;
+        }
+        start[v] = lo;
+    }
+}
+
+constexpr uint32_t kTileWaves = 4, kMostDigits = 4096;   // of a tile of the sort of many elements
+
+struct PassArgs {
+    const uint32_t* keys;    // null in the first pass: the ids themselves
+    const uint32_t* elems;
+    uint32_t* counts;        // [tile][digit]
+    uint32_t* totals;        // [digit]
+    uint32_t shift, bits, turns, n_tiles;   // turns: of 64 elements a wave
+    uint32_t last;
+    uint32_t* keys_out;
+    uint32_t* elems_out;
+    int32_t* row_out;        // in the last pass
+    float* weight_out;
+    uint32_t* start;         // in the only pass
+};
+__device__ __forceinline__ uint32_t pass_key(const SortArgs& a, const PassArgs& s, uint64_t p) { return s.keys ? s.keys[p] : key_of(a, p); }
+
+__global__ __launch_bounds__(256) void k_count(SortArgs a, PassArgs s) {
+    __shared__ uint32_t h[kMostDigits];
+    const uint32_t digits = 1u << s.bits;
+    for (uint32_t d = threadIdx.x; d < digits; d += 256) h[d] = 0;
+    __syncthreads();
+    const uint64_t tile = (uint64_t)kTileWaves * s.turns * 64, t0 = blockIdx.x * tile;
+    for (uint64_t i = threadIdx.x; i < tile && t0 + i < a.n; i += 256)
+        atomicAdd(&h[(pass_key(a, s, t0 + i) >> s.shift) & (digits - 1)], 1u);   // (a count does not depend on their order)
+    __syncthreads();
+    for (uint32_t d = threadIdx.x; d < digits; d += 256) s.counts[(uint64_t)blockIdx.x * digits + d] = h[d];
+}
+
+// counts[tile][digit] become what the tiles before hold of the digit; totals[digit] what all do
+__global__ __launch_bounds__(64) void k_sum_tiles(PassArgs s) {
+    const uint32_t digits = 1u << s.bits, d = blockIdx.x * 64 + threadIdx.x;
+    if (d >= digits) return;
+    uint32_t total = 0;
+    uint32_t* at = s.counts + d;
+    uint32_t t = 0;
+    for (; t + 8 <= s.n_tiles; t += 8) {   // eight reads in flight
+        uint32_t c[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) c[k] = at[(uint64_t)(t + k) * digits];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            at[(uint64_t)(t + k) * digits] = total;
+            total += c[k];
+        }
+    }
+    for (; t < s.n_tiles; ++t) {
+        const uint32_t c = at[(uint64_t)t * digits];
+        at[(uint64_t)t * digits] = total;
+        total += c;
+    }
+    s.totals[d] = total;
+}
+
+__global__ __launch_bounds__(256) void k_scatter(SortArgs a, PassArgs s) {
+    extern __shared__ uint32_t lds[];   // [kTileWaves][digits]
+    __shared__ uint32_t waves[4];
+    const uint32_t digits = 1u << s.bits, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    for (uint32_t k = threadIdx.x; k < kTileWaves * digits; k += 256) lds[k] = 0;
+    __syncthreads();
+    const uint64_t w0 = ((uint64_t)blockIdx.x * kTileWaves + wave) * s.turns * 64;
+    for (uint32_t t = 0; t < s.turns; ++t) {
+        const uint64_t p = w0 + t * 64 + lane;
+        if (p < a.n) atomicAdd(&lds[wave * digits + ((pass_key(a, s, p) >> s.shift) & (digits - 1))], 1u);
+    }
+    __syncthreads();
+    // a digit's first place: the digits before it, the tiles before this one, the waves before
+    uint32_t carry = 0;
+    for (uint32_t d0 = 0; d0 < digits; d0 += 256) {
+        const uint32_t d = d0 + threadIdx.x;
+        const uint32_t total = d < digits ? s.totals[d] : 0u;
+        const uint32_t sum = scan_lanes(total);
         if (lane == 63) waves[wave] = sum;
         __syncthreads();
-        uint32_t before = 0, total = 0;
-        for (uint32_t k = 0; k < 16; ++k) {
-            before += k < wave ? waves[k] : 0u;
-            total += waves[k];
+        uint32_t first = carry + sum - total;
+        for (uint32_t w = 0; w < 4; ++w) {
+            first += w < wave ? waves[w] : 0u;
+            carry += waves[w];
         }
-        if (i < n) data[i] = carry + before + sum - v;
-        carry += total;
+        if (d < digits) {
+            if (s.start && blockIdx.x == 0 && d <= a.n_keys) s.start[d] = first;
+            uint32_t at = first + s.counts[(uint64_t)blockIdx.x * digits + d];
+            for (uint32_t w = 0; w < kTileWaves; ++w) {
+                const uint32_t here = lds[w * digits + d];
+                lds[w * digits + d] = at;
+                at += here;
+            }
+        }
         __syncthreads();
     }
-}
-
-// Sends the tile's pairs to their digits' places, in order.  Within a wave the 64 elements of a turn find the others of
-// their digit by a ballot a key bit; a wave's first place of a digit is the tile's plus what the waves before it hold.
-__global__ __launch_bounds__(256) void k_scatter(const uint32_t* __restrict__ keys, const uint32_t* __restrict__ elems, uint64_t n,
-                                                 uint32_t shift, uint32_t n_tiles, const uint32_t* __restrict__ starts,
-                                                 uint32_t* __restrict__ keys_out, uint32_t* __restrict__ elems_out) {
-    __shared__ uint32_t next[kWaves][kDigits];
-    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    for (uint32_t k = 0; k < kWaves; ++k) next[k][threadIdx.x] = 0;
-    __syncthreads();
-    const uint64_t w0 = (uint64_t)blockIdx.x * kTile + wave * kPerWave;
-    for (uint32_t i = lane; i < kPerWave && w0 + i < n; i += 64) atomicAdd(&next[wave][(keys[w0 + i] >> shift) & (kDigits - 1)], 1u);
-    __syncthreads();
-    {
-        uint32_t at = starts[(uint64_t)threadIdx.x * n_tiles + blockIdx.x];
-        for (uint32_t k = 0; k < kWaves; ++k) {
-            const uint32_t here = next[k][threadIdx.x];
-            next[k][threadIdx.x] = at;
-            at += here;
+    for (uint32_t t = 0; t < s.turns; ++t) {
+        const uint64_t p = w0 + t * 64 + lane;
+        const bool live = p < a.n;
+        const uint32_t key = live ? pass_key(a, s, p) : 0u;
+        const uint32_t to = rank_in_wave(lds + wave * digits, (key >> s.shift) & (digits - 1), s.bits, live);
+        if (!live) continue;
+        const uint32_t e = s.elems ? s.elems[p] : (uint32_t)p;
+        if (s.last) {
+            s.row_out[to] = (int32_t)row_of(a.off, a.n_rows, a.row_len, e);
+            if (a.weight) s.weight_out[to] = a.weight[e];
+        } else {
+            s.elems_out[to] = e;
         }
-    }
-    __syncthreads();
-    for (uint32_t i0 = 0; i0 < kPerWave; i0 += 64) {   // the same number of turns for every wave
-        const uint64_t p = w0 + i0 + lane;
-        const bool live = p < n;
-        const uint32_t key = live ? keys[p] : 0u, elem = live ? elems[p] : 0u;
-        const uint32_t digit = (key >> shift) & (kDigits - 1);
-        unsigned long long same = __builtin_amdgcn_ballot_w64(live);
-#pragma unroll
-        for (uint32_t b = 0; b < kDigitBits; ++b) {
-            const unsigned long long set = __builtin_amdgcn_ballot_w64((digit >> b) & 1u);
-            same &= ((digit >> b) & 1u) ? set : ~set;
-        }
-        const uint32_t rank = (uint32_t)__builtin_popcountll(same & ((1ull << lane) - 1ull));
-        const uint32_t place = live ? next[wave][digit] + rank : 0u;
-        __syncthreads();   // all have read their digit's place
-        if (live && rank == 0) next[wave][digit] += (uint32_t)__builtin_popcountll(same);
-        __syncthreads();
-        if (live) {
-            keys_out[place] = key;
-            elems_out[place] = elem;
-        }
+        if (s.keys_out) s.keys_out[to] = key;
     }
 }
 
@@ -136,108 +298,210 @@ __global__ __launch_bounds__(256) void k_starts(const uint32_t* __restrict__ key
     start[v] = (uint32_t)lo;
 }
 
-// the sorted elements' rows and weights
-__global__ __launch_bounds__(256) void k_rows(const uint32_t* __restrict__ elems, uint64_t n, const uint32_t* __restrict__ off,
-                                              uint64_t n_rows, uint32_t row_len, const float* __restrict__ weight,
-                                              int32_t* __restrict__ row, float* __restrict__ row_weight) {
-    const uint64_t p = (uint64_t)blockIdx.x * 256 + threadIdx.x;
-    if (p >= n) return;
-    const uint32_t e = elems[p];
-    row[p] = (int32_t)row_of(off, n_rows, row_len, e);
-    if (weight) row_weight[p] = weight[e];
-}
-
-// one wave per element: the dot product of its row's gradient and its table row
-template <typename T, typename G, typename Id>
-__global__ __launch_bounds__(256) void k_weight_grad(const Id* __restrict__ ids, uint64_t n, const uint32_t* __restrict__ off,
-                                                     uint64_t n_rows, uint32_t row_len, const G* __restrict__ grad, uint64_t grad_ld,
-                                                     const T* __restrict__ table, uint64_t table_rows, uint64_t table_ld, uint32_t dim,
-                                                     float scale, float* __restrict__ out) {
-    const uint64_t e = (uint64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+// ---- the gradient to the weights ------------------------------------------------------------------------------------------
+// A wave takes 64 elements, a lane finding the row and the table row of each, and works through them B at a time: every lane
+// loads 16 bytes of the B rows of grad and table, column after column, and the B sums over the lanes are formed together: in
+// three steps eight values a lane become one value an eighth of the lanes, half of the values changing sides each time.
+template <typename T, typename G>
+__global__ __launch_bounds__(256) void k_weight_grad(SortArgs a, const G* __restrict__ grad, uint64_t grad_ld, const T* __restrict__ table,
+                                                     uint64_t table_ld, uint32_t dim, float scale, float* __restrict__ out) {
+    constexpr int V = 16 / (sizeof(T) > sizeof(G) ? sizeof(T) : sizeof(G)), B = 8;
+    const uint64_t e0 = ((uint64_t)blockIdx.x * 4 + (threadIdx.x >> 6)) * 64;
     const uint32_t lane = threadIdx.x & 63;
-    if (e >= n) return;
-    const Id id = ids[e];
-    float sum = 0.0f;
-    const bool in = id >= 0 && (uint64_t)id < table_rows && (!off || (e >= off[0] && e < off[n_rows]));
-    if (in) {
-        const G* g = grad + (uint64_t)row_of(off, n_rows, row_len, e) * grad_ld;
-        const T* t = table + (uint64_t)id * table_ld;
-        for (uint32_t c = lane; c < dim; c += 64) sum = fmaf(to_f32(g[c]), to_f32(t[c]), sum);
+    if (e0 >= a.n) return;
+    uint32_t id = (uint32_t)a.n_keys, row = 0;
+    if (e0 + lane < a.n) {
+        id = key_of(a, e0 + lane);
+        row = row_of(a.off, a.n_rows, a.row_len, e0 + lane);
     }
+    float mine = 0.0f;   // of the lane's own element
+    const uint32_t n = a.n - e0 < 64 ? (uint32_t)(a.n - e0) : 64;
+    for (uint32_t u = 0; u < n; u += B) {
+        float sum[B];
+        const T* t[B];
+        const G* g[B];
+        uint32_t live = 0;
 #pragma unroll
-    for (int s = 32; s >= 1; s >>= 1) sum += __shfl_xor(sum, s, 64);
-    if (lane == 0) out[e] = in ? scale * sum : 0.0f;
+        for (int j = 0; j < B; ++j) {
+            const uint32_t of_id = (uint32_t)__builtin_amdgcn_readlane((int)id, (int)(u + j)), of_row = (uint32_t)__builtin_amdgcn_readlane((int)row, (int)(u + j));
+            if (of_id < a.n_keys) live |= 1u << j;
+            t[j] = table + (uint64_t)(of_id < a.n_keys ? of_id : 0u) * table_ld;
+            g[j] = grad + (uint64_t)of_row * grad_ld;
+            sum[j] = 0.0f;
+        }
+        if (live == 0) continue;
+        const bool one_row = g[0] == g[1] && g[0] == g[2] && g[0] == g[3] && g[0] == g[4] && g[0] == g[5] && g[0] == g[6] && g[0] == g[7];
+        for (uint32_t c = lane * V; c < dim; c += 64 * V) {
+            if (c + V <= dim) {
+                float x[B][V], y[B][V];
+#pragma unroll
+                for (int j = 0; j < B; ++j) load_n<V>(t[j] + c, x[j]);
+                if (one_row) {
+                    load_n<V>(g[0] + c, y[0]);
+#pragma unroll
+                    for (int j = 0; j < B; ++j)
+#pragma unroll
+                        for (int k = 0; k < V; ++k) sum[j] = fmaf(x[j][k], y[0][k], sum[j]);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < B; ++j) load_n<V>(g[j] + c, y[j]);
+#pragma unroll
+                    for (int j = 0; j < B; ++j)
+#pragma unroll
+                        for (int k = 0; k < V; ++k) sum[j] = fmaf(x[j][k], y[j][k], sum[j]);
+                }
+            } else {
+                for (uint32_t k = c; k < dim; ++k)
+#pragma unroll
+                    for (int j = 0; j < B; ++j) sum[j] = fmaf(to_f32(t[j][k]), to_f32(g[j][k]), sum[j]);
+            }
+        }
+        // lane bits 0, 1, 2 choose which half of the values a lane keeps; what is left is that of element lane & 7
+        const auto halve = [&](auto count, int bit) {
+            constexpr int kHalf = decltype(count)::value / 2;
+            const bool high = (lane >> bit) & 1u;
+#pragma unroll
+            for (int j = 0; j < kHalf; ++j) {
+                const float keep = high ? sum[2 * j + 1] : sum[2 * j], give = high ? sum[2 * j] : sum[2 * j + 1];
+                sum[j] = keep + __shfl_xor(give, 1 << bit, 64);
+            }
+        };
+        halve(std::integral_constant<int, 8>{}, 0);
+        halve(std::integral_constant<int, 4>{}, 1);
+        halve(std::integral_constant<int, 2>{}, 2);
+#pragma unroll
+        for (int s = 8; s < 64; s <<= 1) sum[0] += __shfl_xor(sum[0], s, 64);
+        if (lane >= u && lane < u + B && ((live >> (lane - u)) & 1u)) mine = scale * sum[0];   // (u is a multiple of 8)
+    }
+    if (e0 + lane < a.n) out[e0 + lane] = mine;
 }
 
 size_t up(size_t bytes) { return (bytes + 255) / 256 * 256; }
 
+uint32_t bits_of(uint64_t v) {
+    uint32_t b = 1;
+    while (v >> b) ++b;
+    return b;
+}
+
+// How many elements are sorted by more than one block: turns of 64 a wave, so that the tiles are some 500 at most, and passes.
+struct Passes {
+    uint32_t turns, n_tiles, count, bits;
+    Passes(uint64_t n, uint32_t key_bits) {
+        turns = 8;
+        while (turns < 64 && n > (uint64_t)512 * kTileWaves * turns * 64) turns *= 2;
+        n_tiles = (uint32_t)((n + kTileWaves * turns * 64 - 1) / (kTileWaves * turns * 64));
+        count = (key_bits + 11) / 12;
+        bits = (key_bits + count - 1) / count;
+    }
+};
+
+SortArgs sort_args(const sdrb_rows& rows, uint64_t n_table_rows) {
+    SortArgs a{};
+    a.ids = rows.ids;
+    a.off = rows.row_offsets;
+    a.weight = rows.weights;
+    a.n = rows.n_elems;
+    a.n_keys = n_table_rows;
+    a.n_rows = rows.n_rows;
+    a.row_len = rows.row_offsets || !rows.n_rows ? 1u : (uint32_t)(rows.n_elems / rows.n_rows);
+    a.wide = rows.id_bits == 64;
+    a.key_bits = bits_of(n_table_rows);
+    return a;
+}
+
+// what a sort and the sums after it keep in the caller's scratch
+struct Scratch {
+    uint32_t *keys[2], *elems[2], *counts, *totals, *start;
+    int32_t* row;
+    float* weight;
+    float* partials;
+    size_t bytes;
+    Scratch(void* base, uint64_t n, uint64_t n_keys, bool weighted, uint32_t dim) {
+        size_t at = 0;
+        const auto take = [&](size_t count) {
+            char* p = static_cast<char*>(base) + (base ? at : 0);
+            at += up(count * 4);
+            return reinterpret_cast<uint32_t*>(p);
+        };
+        const Passes p(n, bits_of(n_keys));
+        const bool small = n <= kSmall;
+        row = reinterpret_cast<int32_t*>(take(n));
+        weight = reinterpret_cast<float*>(take(weighted ? n : 0));
+        for (int k = 0; k < 2; ++k) {   // as many as the passes write: k_starts reads the keys of more than one
+            keys[k] = take(small ? (k ? 0 : n) : p.count > 1 ? n : 0);
+            elems[k] = take(!small && p.count > 1u + k ? n : 0);
+        }
+        counts = take(small ? 0 : (size_t)p.n_tiles << p.bits);
+        totals = take(small ? 0 : (size_t)1 << p.bits);
+        start = take(n_keys + 1);
+        partials = gather_partial_bytes(n_keys, n, true, dim) ? reinterpret_cast<float*>(take(0)) : nullptr;
+        bytes = at + gather_partial_bytes(n_keys, n, true, dim);
+    }
+};
+
+int sort_by_id(const SortArgs& a, const Scratch& s, hipStream_t stream) {
+    const uint32_t* sorted = nullptr;   // keys whose starts are still to be found
+    if (a.n <= kSmall) {
+        hipLaunchKernelGGL(k_sort_small, dim3(1), dim3(kSmallThreads), 0, stream, a, s.keys[0], s.row, s.weight, s.start);
+        SDRB_HIP(hipGetLastError());
+        if (a.n_keys > kStartsInSort) sorted = s.keys[0];
+    } else {
+        const Passes passes(a.n, a.key_bits);
+        for (uint32_t k = 0; k < passes.count; ++k) {
+            PassArgs p{};
+            p.keys = k ? s.keys[(k - 1) & 1] : nullptr;
+            p.elems = k ? s.elems[(k - 1) & 1] : nullptr;
+            p.counts = s.counts;
+            p.totals = s.totals;
+            p.shift = k * passes.bits;
+            p.bits = passes.bits;
+            p.turns = passes.turns;
+            p.n_tiles = passes.n_tiles;
+            p.last = k + 1 == passes.count;
+            p.keys_out = passes.count > 1 ? s.keys[k & 1] : nullptr;
+            p.elems_out = p.last ? nullptr : s.elems[k & 1];
+            p.row_out = s.row;
+            p.weight_out = s.weight;
+            p.start = passes.count == 1 ? s.start : nullptr;
+            hipLaunchKernelGGL(k_count, dim3(passes.n_tiles), dim3(256), 0, stream, a, p);
+            SDRB_HIP(hipGetLastError());
+            hipLaunchKernelGGL(k_sum_tiles, dim3(((1u << passes.bits) + 63) / 64), dim3(64), 0, stream, p);
+            SDRB_HIP(hipGetLastError());
+            const size_t lds = ((size_t)kTileWaves << passes.bits) * sizeof(uint32_t);
+            if (const int rc = allow_lds(&k_scatter, lds)) return rc;
+            hipLaunchKernelGGL(k_scatter, dim3(passes.n_tiles), dim3(256), lds, stream, a, p);
+            SDRB_HIP(hipGetLastError());
+        }
+        if (passes.count > 1) sorted = s.keys[(passes.count - 1) & 1];
+    }
+    if (sorted) {
+        hipLaunchKernelGGL(k_starts, dim3((uint32_t)(a.n_keys / 256 + 1)), dim3(256), 0, stream, sorted, a.n, a.n_keys, s.start);
+        SDRB_HIP(hipGetLastError());
+    }
+    return SDRB_OK;
+}
+
 }  // namespace
 
-size_t table_grad_scratch_bytes(uint64_t n_elems, uint64_t n_table_rows, uint32_t dim) {
-    const size_t list = up(n_elems * sizeof(uint32_t));
-    const size_t n_tiles = (n_elems + kTile - 1) / kTile;
-    return 4 * list + up(n_tiles * kDigits * sizeof(uint32_t)) + up((n_table_rows + 1) * sizeof(uint32_t)) +
-           gather_partial_bytes(n_table_rows, n_elems, true, dim);
+size_t table_grad_scratch_bytes(uint64_t n_elems, uint64_t n_table_rows, bool weighted, uint32_t dim) {
+    return Scratch(nullptr, n_elems, n_table_rows, weighted, dim).bytes;
 }
 
 int launch_table_grad(int device, const sdrb_rows& rows, const sdrb_dense& grad, float scale, bool accumulate, const sdrb_dense& out,
                       void* scratch, hipStream_t stream) {
-    const uint64_t n = rows.n_elems, v = out.n_rows;
-    const uint32_t dim = (uint32_t)out.n_cols, row_len = rows.row_offsets || !rows.n_rows ? 1u : (uint32_t)(n / rows.n_rows);
-    const uint32_t n_tiles = (uint32_t)((n + kTile - 1) / kTile);
-    char* ws = static_cast<char*>(scratch);
-    const auto take = [&](size_t bytes) {
-        char* p = ws;
-        ws += up(bytes);
-        return p;
-    };
-    uint32_t* keys[2];
-    uint32_t* elems[2];
-    for (int k = 0; k < 2; ++k) {
-        keys[k] = reinterpret_cast<uint32_t*>(take(n * sizeof(uint32_t)));
-        elems[k] = reinterpret_cast<uint32_t*>(take(n * sizeof(uint32_t)));
-    }
-    uint32_t* counts = reinterpret_cast<uint32_t*>(take((size_t)n_tiles * kDigits * sizeof(uint32_t)));
-    uint32_t* start = reinterpret_cast<uint32_t*>(take((v + 1) * sizeof(uint32_t)));
-    float* partials = gather_partial_bytes(v, n, true, dim) ? reinterpret_cast<float*>(ws) : nullptr;
-    const dim3 per_elem((uint32_t)((n + 255) / 256));
-    int now = 0;
-    if (n) {
-        if (rows.id_bits == 64)
-            hipLaunchKernelGGL((k_keys<int64_t>), per_elem, dim3(256), 0, stream, static_cast<const int64_t*>(rows.ids), n, v,
-                               rows.row_offsets, rows.n_rows, keys[0], elems[0]);
-        else
-            hipLaunchKernelGGL((k_keys<int32_t>), per_elem, dim3(256), 0, stream, static_cast<const int32_t*>(rows.ids), n, v,
-                               rows.row_offsets, rows.n_rows, keys[0], elems[0]);
-        SDRB_HIP(hipGetLastError());
-        for (uint32_t shift = 0; shift < 32 && (v >> shift) != 0; shift += kDigitBits) {   // the largest key is v
-            hipLaunchKernelGGL(k_count, dim3(n_tiles), dim3(256), 0, stream, keys[now], n, shift, n_tiles, counts);
-            SDRB_HIP(hipGetLastError());
-            hipLaunchKernelGGL(k_scan, dim3(1), dim3(1024), 0, stream, counts, (uint64_t)n_tiles * kDigits);
-            SDRB_HIP(hipGetLastError());
-            hipLaunchKernelGGL(k_scatter, dim3(n_tiles), dim3(256), 0, stream, keys[now], elems[now], n, shift, n_tiles, counts,
-                               keys[now ^ 1], elems[now ^ 1]);
-            SDRB_HIP(hipGetLastError());
-            now ^= 1;
-        }
-    }
-    hipLaunchKernelGGL(k_starts, dim3((uint32_t)(v / 256 + 1)), dim3(256), 0, stream, keys[now], n, v, start);
-    SDRB_HIP(hipGetLastError());
-    int32_t* row = reinterpret_cast<int32_t*>(keys[now ^ 1]);
-    float* weight = rows.weights ? reinterpret_cast<float*>(elems[now ^ 1]) : nullptr;
-    if (n) {
-        hipLaunchKernelGGL(k_rows, per_elem, dim3(256), 0, stream, elems[now], n, rows.row_offsets, rows.n_rows, row_len, rows.weights,
-                           row, weight);
-        SDRB_HIP(hipGetLastError());
-    }
+    const uint32_t dim = (uint32_t)out.n_cols;
+    const Scratch s(scratch, rows.n_elems, out.n_rows, rows.weights != nullptr, dim);
+    const SortArgs a = sort_args(rows, out.n_rows);
+    if (const int rc = sort_by_id(a, s, stream)) return rc;
     GatherSum g{};
     g.device = device;
-    g.n_segments = v;
-    g.n_elems = n;
-    g.start = start;
-    g.index = row;
+    g.n_segments = out.n_rows;
+    g.n_elems = rows.n_elems;
+    g.start = s.start;
+    g.index = s.row;
     g.index_bits = 32;
-    g.weight = weight;
+    g.weight = rows.weights ? s.weight : nullptr;
     g.src = grad.data;
     g.src_type = grad.type;
     g.src_rows = grad.n_rows;
@@ -248,29 +512,23 @@ int launch_table_grad(int device, const sdrb_rows& rows, const sdrb_dense& grad,
     g.out_ld = out.ld;
     g.scale = scale;
     g.accumulate = accumulate;
-    g.partials = partials;
+    g.partials = s.partials;
     return launch_gather_sum(g, stream);
 }
 
 int launch_weight_grad(const sdrb_rows& rows, const sdrb_dense& grad, const sdrb_dense& table, float scale, float* out,
                        hipStream_t stream) {
-    const uint64_t n = rows.n_elems;
-    if (n == 0) return SDRB_OK;
-    const uint32_t row_len = rows.row_offsets || !rows.n_rows ? 1u : (uint32_t)(n / rows.n_rows);
+    if (rows.n_elems == 0) return SDRB_OK;
+    const SortArgs a = sort_args(rows, table.n_rows);
     return with_type(table.type, [&](auto t) {
         return with_type(grad.type, [&](auto g) {
             using T = decltype(t);
             using G = decltype(g);
-            const auto go = [&](auto id) {
-                using Id = decltype(id);
-                hipLaunchKernelGGL((k_weight_grad<T, G, Id>), dim3((uint32_t)((n + 3) / 4)), dim3(256), 0, stream,
-                                   static_cast<const Id*>(rows.ids), n, rows.row_offsets, rows.n_rows, row_len,
-                                   static_cast<const G*>(grad.data), grad.ld, static_cast<const T*>(table.data), table.n_rows, table.ld,
-                                   (uint32_t)table.n_cols, scale, out);
-                SDRB_HIP(hipGetLastError());
-                return SDRB_OK;
-            };
-            return rows.id_bits == 64 ? go(int64_t{}) : go(int32_t{});
+            hipLaunchKernelGGL((k_weight_grad<T, G>), dim3((uint32_t)((a.n + 255) / 256)), dim3(256), 0, stream, a,
+                               static_cast<const G*>(grad.data), grad.ld, static_cast<const T*>(table.data), table.ld, (uint32_t)table.n_cols,
+                               scale, out);
+            SDRB_HIP(hipGetLastError());
+            return SDRB_OK;
         });
     });
 }

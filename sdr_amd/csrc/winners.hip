@@ -946,13 +946,6 @@ int with_layout(uint32_t n, uint64_t n_rows, uint32_t k, F&& f) {
     return f(integral_constant<int, 32>{}, waves);
 }
 
-// more than 64 KiB of dynamic LDS has to be asked for
-template <typename F>
-int allow_lds(F* kernel, size_t bytes) {
-    if (bytes > 65536) SDRB_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
-    return SDRB_OK;
-}
-
 }  // namespace
 
 int launch_winners(const sdrb_dense& scores, const sdrb_winners_spec& spec, int32_t* ids, float* weights, hipStream_t stream) {

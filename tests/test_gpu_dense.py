@@ -148,19 +148,35 @@ def test_lookup_grad_table(form, grad, out, dim, n, n_table):
     plain.assert_sum(into.cpu()[on], (want[0] + before.cpu().double())[on], (want[1] + before.cpu().double().abs())[on], want[2][on] + 1, form)
 
 
-@pytest.mark.parametrize("n", [1, 63, 64, 65, 2047, 2048, 2049, 5000, 20_000])
+@pytest.mark.parametrize("n", [1, 63, 64, 65, 1023, 1025, 2049, 16_384, 16_385, 40_000])
 @pytest.mark.parametrize("ids_of", ["one", "two", "all_padding", "distinct", "skewed"])
-def test_lookup_grad_table_of_shared_ids(n, ids_of):
+@pytest.mark.parametrize("n_table", [None, 100, 70_000])
+def test_lookup_grad_table_of_shared_ids(n, ids_of, n_table):
     """ids that many rows hold, and the order of additions: integers in fp32 add exactly"""
     import sdr_amd
     g = rng(n)
-    n_table = max(n, 9)
+    n_table = max(n, 9) if n_table is None else n_table
     ids = {"one": torch.full((n,), 7), "two": torch.arange(n) % 2 * 5 + 2, "all_padding": torch.full((n,), -1), "distinct": torch.randperm(n, generator=g),
            "skewed": (torch.rand(n, generator=g) ** 8 * n).long()}[ids_of].cuda()
+    ids = torch.where(ids < n_table, ids, -1)
     go = torch.randint(-50, 50, (n, 12), generator=g).float().cuda()
     want = torch.zeros(n_table + 1, 12).index_add_(0, torch.where(ids < 0, n_table, ids).cpu(), go.cpu())[:-1]
     assert torch.equal(sdr_amd.lookup_grad_table(ids, go, n_table).cpu(), want)
     assert torch.equal(sdr_amd.lookup_grad_table(ids.int(), go, n_table, scale=2.0).cpu(), want * 2)
+
+
+def test_lookup_grad_table_of_many_ids():
+    """more than 2^24 ids: three passes of the sort of many elements"""
+    import sdr_amd
+    g = rng(24)
+    n, n_table = 30_000, 2 ** 24 + 5
+    ids = torch.randint(0, n_table, (n,), generator=g).cuda()
+    ids[::7] = 2 ** 24 + 4
+    ids[1::7] = 3
+    go = torch.randint(-50, 50, (n, 3), generator=g).float().cuda()
+    want = torch.zeros(n_table, 3, device="cuda").index_add_(0, ids, go)
+    assert torch.equal(sdr_amd.lookup_grad_table(ids, go, n_table), want)
+    assert torch.equal(sdr_amd.lookup_grad_table(ids[:9000], go[:9000], n_table), torch.zeros(n_table, 3, device="cuda").index_add_(0, ids[:9000], go[:9000]))
 
 
 @pytest.mark.parametrize("form", ["tokens", "fives", "ragged"])
