@@ -35,6 +35,35 @@ __device__ __forceinline__ void store_n(T* p, const float (&v)[N]) {
     __builtin_memcpy(p, t, sizeof t);
 }
 
+// ---- values moved between the lanes of a wave, without LDS ----
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t dpp(uint32_t other, uint32_t v) {
+    return (uint32_t)__builtin_amdgcn_update_dpp((int)other, (int)v, CTRL, ROWS, 0xF, false);
+}
+template <int CTRL, int ROWS>
+__device__ __forceinline__ float dpp(float other, float v) {
+    return __builtin_bit_cast(float, dpp<CTRL, ROWS>(__builtin_bit_cast(uint32_t, other), __builtin_bit_cast(uint32_t, v)));
+}
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double dpp(double other, double v) {
+    const uint64_t o = __builtin_bit_cast(uint64_t, other), x = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = dpp<CTRL, ROWS>((uint32_t)o, (uint32_t)x), hi = dpp<CTRL, ROWS>((uint32_t)(o >> 32), (uint32_t)(x >> 32));
+    return __builtin_bit_cast(double, ((uint64_t)hi << 32) | lo);
+}
+// inclusive sums over the lanes of a wave, or of each row of 16
+template <int LANES>
+__device__ __forceinline__ uint32_t scan_lanes(uint32_t v) {
+    v += dpp<0x111, 0xF>(0u, v);   // one lane up in a row of 16, two, four, eight
+    v += dpp<0x112, 0xF>(0u, v);
+    v += dpp<0x114, 0xF>(0u, v);
+    v += dpp<0x118, 0xF>(0u, v);
+    if constexpr (LANES == 64) {
+        v += dpp<0x142, 0xA>(0u, v);   // lane 15 of the row of 16 below, into rows 1 and 3
+        v += dpp<0x143, 0xC>(0u, v);   // lane 31, into rows 2 and 3
+    }
+    return v;
+}
+
 // Calls f(T{}) with the element type named by `type` (checked by the caller).
 template <typename F>
 int with_type(int type, F&& f) {

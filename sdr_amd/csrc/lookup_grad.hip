@@ -52,18 +52,23 @@ __device__ __forceinline__ uint32_t lanes_below(unsigned long long mask) {
     return __builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0u));
 }
 // the lanes of the wave that hold the same digit, of those that are live
-__device__ __forceinline__ unsigned long long same_digit(uint32_t digit, uint32_t bits, bool live) {
-    unsigned long long same = __builtin_amdgcn_ballot_w64(live);
-    for (uint32_t b = 0; b < bits; ++b) {
-        const bool set = (digit >> b) & 1u;
-        const unsigned long long with = __builtin_amdgcn_ballot_w64(set);
-        same &= set ? with : ~with;
+template <int BITS>
+__device__ __forceinline__ unsigned long long same_digit(uint32_t digit, bool live) {
+    const unsigned long long on = __builtin_amdgcn_ballot_w64(live);
+    uint32_t lo = (uint32_t)on, hi = (uint32_t)(on >> 32);
+#pragma unroll
+    for (int b = 0; b < BITS; ++b) {
+        const uint32_t set = (uint32_t)((int32_t)(digit << (31 - b)) >> 31);   // all ones or none
+        const unsigned long long with = __builtin_amdgcn_ballot_w64(set != 0);
+        lo &= ~((uint32_t)with ^ set);
+        hi &= ~((uint32_t)(with >> 32) ^ set);
     }
-    return same;
+    return ((unsigned long long)hi << 32) | lo;
 }
 // Of equal digits, what the wave's earlier turns and the lower lanes hold; counter[digit] goes up by this turn's.
-__device__ __forceinline__ uint32_t rank_in_wave(uint32_t* counter, uint32_t digit, uint32_t bits, bool live) {
-    const unsigned long long same = same_digit(digit, bits, live);
+template <int BITS>
+__device__ __forceinline__ uint32_t rank_in_wave(uint32_t* counter, uint32_t digit, bool live) {
+    const unsigned long long same = same_digit<BITS>(digit, live);
     const uint32_t below = lanes_below(same);
     uint32_t before = 0;
     if (live) before = counter[digit];
@@ -74,17 +79,6 @@ __device__ __forceinline__ uint32_t rank_in_wave(uint32_t* counter, uint32_t dig
     __builtin_amdgcn_wave_barrier();
     return before + below;
 }
-// inclusive sums over the lanes of a wave
-__device__ __forceinline__ uint32_t scan_lanes(uint32_t v) {
-    const uint32_t lane = threadIdx.x & 63;
-#pragma unroll
-    for (uint32_t s = 1; s < 64; s <<= 1) {
-        const uint32_t below = (uint32_t)__shfl_up((int)v, s, 64);
-        if (lane >= s) v += below;
-    }
-    return v;
-}
-
 constexpr uint32_t kSmall = 16384, kSmallThreads = 1024, kSmallWaves = kSmallThreads / 64, kSmallTurns = kSmall / kSmallThreads;
 constexpr uint64_t kStartsInSort = 4096;   // up to so many keys the one block finds their starts as well, four a thread
 
@@ -103,15 +97,14 @@ __global__ __launch_bounds__(kSmallThreads) void k_sort_small(SortArgs a, uint32
         key[t] = t < turns && elem[t] < n ? key_of(a, elem[t]) : 0u;
     }
     for (uint32_t shift = 0; shift < a.key_bits; shift += 8) {
-        const uint32_t bits = a.key_bits - shift < 8 ? a.key_bits - shift : 8;
         for (uint32_t k = threadIdx.x; k < kSmallWaves * 256; k += kSmallThreads) counter[k >> 8][k & 255] = 0;
         __syncthreads();
 #pragma unroll
         for (uint32_t t = 0; t < kSmallTurns; ++t) {
-            if (t >= turns) break;
+            if (t >= turns) continue;
             // (positions, not elements, say which lanes are live: after the first pass the last ones are the largest keys)
             const bool live = (wave * turns + t) * 64 + lane < n;
-            place[t] = rank_in_wave(counter[wave], (key[t] >> shift) & 255u, bits, live);
+            place[t] = rank_in_wave<8>(counter[wave], (key[t] >> shift) & 255u, live);
         }
         __syncthreads();
         if (threadIdx.x < 256) {   // a digit a thread: sums over the waves, then over the digits
@@ -121,7 +114,7 @@ __global__ __launch_bounds__(kSmallThreads) void k_sort_small(SortArgs a, uint32
                 counter[w][threadIdx.x] = total;
                 total += here;
             }
-            const uint32_t sum = scan_lanes(total);
+            const uint32_t sum = scan_lanes<64>(total);
             if (lane == 63) digit_waves[wave] = sum;
             key_at[threadIdx.x] = sum - total;   // (its contents have been read)
         }
@@ -134,7 +127,7 @@ __global__ __launch_bounds__(kSmallThreads) void k_sort_small(SortArgs a, uint32
         __syncthreads();
 #pragma unroll
         for (uint32_t t = 0; t < kSmallTurns; ++t) {
-            if (t >= turns) break;
+            if (t >= turns) continue;
             if ((wave * turns + t) * 64 + lane < n) {
                 const uint32_t to = counter[wave][(key[t] >> shift) & 255u] + place[t];
                 key_at[to] = key[t];
@@ -144,7 +137,7 @@ __global__ __launch_bounds__(kSmallThreads) void k_sort_small(SortArgs a, uint32
         __syncthreads();
 #pragma unroll
         for (uint32_t t = 0; t < kSmallTurns; ++t) {
-            if (t >= turns) break;
+            if (t >= turns) continue;
             const uint32_t p = (wave * turns + t) * 64 + lane;
             if (p < n) {
                 key[t] = key_at[p];
@@ -155,7 +148,7 @@ __global__ __launch_bounds__(kSmallThreads) void k_sort_small(SortArgs a, uint32
     }
 #pragma unroll
     for (uint32_t t = 0; t < kSmallTurns; ++t) {
-        if (t >= turns) break;
+        if (t >= turns) continue;
         const uint32_t p = (wave * turns + t) * 64 + lane;
         if (p < n) {
             keys_out[p] = key[t];
@@ -212,66 +205,74 @@ __global__ __launch_bounds__(64) void k_sum_tiles(PassArgs s) {
     if (d >= digits) return;
     uint32_t total = 0;
     uint32_t* at = s.counts + d;
-    uint32_t t = 0;
-    for (; t + 8 <= s.n_tiles; t += 8) {   // eight reads in flight
-        uint32_t c[8];
+    constexpr uint32_t kAhead = 32;   // reads in flight
+    for (uint32_t t = 0; t < s.n_tiles; t += kAhead) {
+        uint32_t c[kAhead];
 #pragma unroll
-        for (int k = 0; k < 8; ++k) c[k] = at[(uint64_t)(t + k) * digits];
+        for (uint32_t k = 0; k < kAhead; ++k) c[k] = t + k < s.n_tiles ? at[(uint64_t)(t + k) * digits] : 0u;
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-            at[(uint64_t)(t + k) * digits] = total;
+        for (uint32_t k = 0; k < kAhead; ++k) {
+            if (t + k < s.n_tiles) at[(uint64_t)(t + k) * digits] = total;
             total += c[k];
         }
-    }
-    for (; t < s.n_tiles; ++t) {
-        const uint32_t c = at[(uint64_t)t * digits];
-        at[(uint64_t)t * digits] = total;
-        total += c;
     }
     s.totals[d] = total;
 }
 
+template <int BITS>
 __global__ __launch_bounds__(256) void k_scatter(SortArgs a, PassArgs s) {
-    extern __shared__ uint32_t lds[];   // [kTileWaves][digits]
-    __shared__ uint32_t waves[4];
-    const uint32_t digits = 1u << s.bits, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    for (uint32_t k = threadIdx.x; k < kTileWaves * digits; k += 256) lds[k] = 0;
+    constexpr uint32_t kDigits = 1u << BITS, kEach = (kDigits + 255) / 256;   // digits of a thread
+    __shared__ uint32_t next[kTileWaves][kDigits];
+    __shared__ uint32_t sums[kEach * 4];
+    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    uint32_t total[kEach], tiles_before[kEach];
+#pragma unroll
+    for (uint32_t i = 0; i < kEach; ++i) {   // on their way while the tile's own digits are counted
+        const uint32_t d = i * 256 + threadIdx.x;
+        total[i] = d < kDigits ? s.totals[d] : 0u;
+        tiles_before[i] = d < kDigits ? s.counts[(uint64_t)blockIdx.x * kDigits + d] : 0u;
+    }
+    for (uint32_t k = threadIdx.x; k < kTileWaves * kDigits; k += 256) next[k >> BITS][k & (kDigits - 1)] = 0;
     __syncthreads();
     const uint64_t w0 = ((uint64_t)blockIdx.x * kTileWaves + wave) * s.turns * 64;
     for (uint32_t t = 0; t < s.turns; ++t) {
         const uint64_t p = w0 + t * 64 + lane;
-        if (p < a.n) atomicAdd(&lds[wave * digits + ((pass_key(a, s, p) >> s.shift) & (digits - 1))], 1u);
+        if (p < a.n) atomicAdd(&next[wave][(pass_key(a, s, p) >> s.shift) & (kDigits - 1)], 1u);
+    }
+    // a digit's first place: the digits before it, the tiles before this one, the waves before
+    uint32_t first[kEach];
+#pragma unroll
+    for (uint32_t i = 0; i < kEach; ++i) {
+        const uint32_t sum = scan_lanes<64>(total[i]);
+        if (lane == 63) sums[i * 4 + wave] = sum;
+        first[i] = sum - total[i];
     }
     __syncthreads();
-    // a digit's first place: the digits before it, the tiles before this one, the waves before
-    uint32_t carry = 0;
-    for (uint32_t d0 = 0; d0 < digits; d0 += 256) {
-        const uint32_t d = d0 + threadIdx.x;
-        const uint32_t total = d < digits ? s.totals[d] : 0u;
-        const uint32_t sum = scan_lanes(total);
-        if (lane == 63) waves[wave] = sum;
-        __syncthreads();
-        uint32_t first = carry + sum - total;
-        for (uint32_t w = 0; w < 4; ++w) {
-            first += w < wave ? waves[w] : 0u;
-            carry += waves[w];
-        }
-        if (d < digits) {
-            if (s.start && blockIdx.x == 0 && d <= a.n_keys) s.start[d] = first;
-            uint32_t at = first + s.counts[(uint64_t)blockIdx.x * digits + d];
-            for (uint32_t w = 0; w < kTileWaves; ++w) {
-                const uint32_t here = lds[w * digits + d];
-                lds[w * digits + d] = at;
-                at += here;
-            }
-        }
-        __syncthreads();
+    if (wave == 0) {   // the sums of 64 digits each, at most 64 of them
+        const uint32_t here = lane < kEach * 4 ? sums[lane] : 0u, sum = scan_lanes<64>(here);
+        if (lane < kEach * 4) sums[lane] = sum - here;
     }
+    __syncthreads();
+#pragma unroll
+    for (uint32_t i = 0; i < kEach; ++i) {
+        const uint32_t d = i * 256 + threadIdx.x;
+        if (d >= kDigits) continue;
+        first[i] += sums[i * 4 + wave];
+        if (s.start && blockIdx.x == 0 && d <= a.n_keys) s.start[d] = first[i];
+        uint32_t at = first[i] + tiles_before[i];
+#pragma unroll
+        for (uint32_t w = 0; w < kTileWaves; ++w) {
+            const uint32_t here = next[w][d];
+            next[w][d] = at;
+            at += here;
+        }
+    }
+    __syncthreads();
     for (uint32_t t = 0; t < s.turns; ++t) {
         const uint64_t p = w0 + t * 64 + lane;
         const bool live = p < a.n;
         const uint32_t key = live ? pass_key(a, s, p) : 0u;
-        const uint32_t to = rank_in_wave(lds + wave * digits, (key >> s.shift) & (digits - 1), s.bits, live);
+        const uint32_t to = rank_in_wave<BITS>(next[wave], (key >> s.shift) & (kDigits - 1), live);
         if (!live) continue;
         const uint32_t e = s.elems ? s.elems[p] : (uint32_t)p;
         if (s.last) {
@@ -392,7 +393,7 @@ struct Passes {
         while (turns < 64 && n > (uint64_t)512 * kTileWaves * turns * 64) turns *= 2;
         n_tiles = (uint32_t)((n + kTileWaves * turns * 64 - 1) / (kTileWaves * turns * 64));
         count = (key_bits + 11) / 12;
-        bits = (key_bits + count - 1) / count;
+        bits = std::max((key_bits + count - 1) / count, 8u);
     }
 };
 
@@ -468,9 +469,8 @@ int sort_by_id(const SortArgs& a, const Scratch& s, hipStream_t stream) {
             SDRB_HIP(hipGetLastError());
             hipLaunchKernelGGL(k_sum_tiles, dim3(((1u << passes.bits) + 63) / 64), dim3(64), 0, stream, p);
             SDRB_HIP(hipGetLastError());
-            const size_t lds = ((size_t)kTileWaves << passes.bits) * sizeof(uint32_t);
-            if (const int rc = allow_lds(&k_scatter, lds)) return rc;
-            hipLaunchKernelGGL(k_scatter, dim3(passes.n_tiles), dim3(256), lds, stream, a, p);
+            const auto scatter = passes.bits == 12 ? &k_scatter<12> : passes.bits == 11 ? &k_scatter<11> : passes.bits == 10 ? &k_scatter<10> : passes.bits == 9 ? &k_scatter<9> : &k_scatter<8>;
+            hipLaunchKernelGGL(scatter, dim3(passes.n_tiles), dim3(256), 0, stream, a, p);
             SDRB_HIP(hipGetLastError());
         }
         if (passes.count > 1) sorted = s.keys[(passes.count - 1) & 1];

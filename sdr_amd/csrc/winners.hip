@@ -30,21 +30,7 @@ namespace sdrb {
 
 namespace {
 
-// ---- values moved between the lanes of a wave, without LDS ----
-template <int CTRL, int ROWS>
-__device__ __forceinline__ uint32_t dpp(uint32_t other, uint32_t v) {
-    return (uint32_t)__builtin_amdgcn_update_dpp((int)other, (int)v, CTRL, ROWS, 0xF, false);
-}
-template <int CTRL, int ROWS>
-__device__ __forceinline__ float dpp(float other, float v) {
-    return __builtin_bit_cast(float, dpp<CTRL, ROWS>(__builtin_bit_cast(uint32_t, other), __builtin_bit_cast(uint32_t, v)));
-}
-template <int CTRL, int ROWS>
-__device__ __forceinline__ double dpp(double other, double v) {
-    const uint64_t o = __builtin_bit_cast(uint64_t, other), x = __builtin_bit_cast(uint64_t, v);
-    const uint32_t lo = dpp<CTRL, ROWS>((uint32_t)o, (uint32_t)x), hi = dpp<CTRL, ROWS>((uint32_t)(o >> 32), (uint32_t)(x >> 32));
-    return __builtin_bit_cast(double, ((uint64_t)hi << 32) | lo);
-}
+// ---- a wave's reductions ----
 __device__ __forceinline__ uint32_t last_lane(uint32_t v) { return (uint32_t)__builtin_amdgcn_readlane((int)v, 63); }
 __device__ __forceinline__ float last_lane(float v) { return __builtin_bit_cast(float, last_lane(__builtin_bit_cast(uint32_t, v))); }
 __device__ __forceinline__ double last_lane(double v) {
@@ -166,18 +152,9 @@ struct Team {
 #pragma unroll
         for (int p = 0; p < (Q + 1) / 2; ++p) {   // two chunks a register: at most 512 a wave in each
             packed[p] = here[2 * p] | (2 * p + 1 < Q ? here[2 * p + 1] << 16 : 0u);
-            uint32_t v = packed[p];
-            v += dpp<0x111, 0xF>(0u, v);   // one lane up in a row of 16, two, four, eight
-            v += dpp<0x112, 0xF>(0u, v);
-            v += dpp<0x114, 0xF>(0u, v);
-            v += dpp<0x118, 0xF>(0u, v);
-            if constexpr (kWaves == 0) {
-                ends[p] = dpp<0x15F, 0xF>(v, v);   // lane 15 of the row
-            } else {
-                v += dpp<0x142, 0xA>(0u, v);
-                v += dpp<0x143, 0xC>(0u, v);
-                ends[p] = last_lane(v);
-            }
+            const uint32_t v = scan_lanes<kLanes>(packed[p]);
+            if constexpr (kWaves == 0) ends[p] = dpp<0x15F, 0xF>(v, v);   // lane 15 of the row
+            else ends[p] = last_lane(v);
             sums[p] = v;
         }
 #pragma unroll
