@@ -89,7 +89,7 @@ int sdrb_lookup_scratch(const sdrb_rows* rows, uint64_t n_cols, size_t* bytes) {
     const char* what = "sdrb_lookup_scratch";
     if (const int rc = check_rows(what, rows)) return rc;
     if (!bytes || n_cols > kMaxCols) return refuse(SDRB_ERR_INVALID_ARG, what, "bytes is null or n_cols above 2^24");
-    *bytes = gather_partial_bytes(rows->n_rows, rows->n_elems, rows->row_offsets != nullptr, (uint32_t)n_cols);
+    *bytes = partial_bytes(segment_chunk(rows->n_rows, rows->n_elems, rows->row_offsets != nullptr), rows->n_elems, (uint32_t)n_cols);
     return SDRB_OK;
 }
 
@@ -103,7 +103,8 @@ int sdrb_lookup(int device, const sdrb_rows* rows, const sdrb_dense* table, floa
     if (out->n_rows != rows->n_rows || out->n_cols != table->n_cols)
         return refuse(SDRB_ERR_INVALID_ARG, what, "out must have a row for every row and the table's columns");
     if (out->n_rows == 0 || out->n_cols == 0) return SDRB_OK;
-    const size_t need = gather_partial_bytes(rows->n_rows, rows->n_elems, rows->row_offsets != nullptr, (uint32_t)out->n_cols);
+    const uint32_t chunk = segment_chunk(rows->n_rows, rows->n_elems, rows->row_offsets != nullptr);
+    const size_t need = partial_bytes(chunk, rows->n_elems, (uint32_t)out->n_cols);
     if (const int rc = check_scratch(what, need, scratch, scratch_bytes)) return rc;
     DeviceGuard guard(device);
     if (!guard.ok) return no_device(device);
@@ -123,7 +124,8 @@ int sdrb_lookup(int device, const sdrb_rows* rows, const sdrb_dense* table, floa
     g.out_type = out->type;
     g.out_ld = out->ld;
     g.scale = scale;
-    g.partials = need ? static_cast<float*>(scratch) : nullptr;
+    g.chunk = chunk;
+    g.partials = static_cast<float*>(scratch);
     return launch_gather_sum(g, static_cast<hipStream_t>(stream));
 }
 
@@ -150,7 +152,7 @@ int sdrb_lookup_grad_table(int device, const sdrb_rows* rows, const sdrb_dense* 
     if (const int rc = check_scratch(what, need, scratch, scratch_bytes)) return rc;
     DeviceGuard guard(device);
     if (!guard.ok) return no_device(device);
-    return launch_table_grad(device, *rows, *grad, scale, accumulate != 0, *out, scratch, static_cast<hipStream_t>(stream));
+    return launch_table_grad(*rows, *grad, scale, accumulate != 0, *out, scratch, static_cast<hipStream_t>(stream));
 }
 
 int sdrb_lookup_grad_weights(int device, const sdrb_rows* rows, const sdrb_dense* grad, const sdrb_dense* table, float scale,

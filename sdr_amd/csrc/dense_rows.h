@@ -1,6 +1,8 @@
 // Sparse rows of ids against dense matrices: what the kernels of lookup.hip, lookup_grad.hip and winners.hip share.
 #pragma once
 
+#include <type_traits>
+
 #include "sdrb_internal.h"
 
 namespace sdrb {
@@ -18,12 +20,32 @@ __device__ __forceinline__ T from_f32(float v) {
     return (T)v;
 }
 
-// N consecutive elements starting at any multiple of the element's own size (the unaligned access mode of the target
-// makes these single wide loads and stores)
+// 16, 8 and 4 bytes at any multiple of two: the unaligned access mode of the target makes each one load or store
+using Bytes16 = uint32_t __attribute__((ext_vector_type(4), aligned(2)));
+using Bytes8 = uint32_t __attribute__((ext_vector_type(2), aligned(2)));
+using Bytes4 = uint32_t __attribute__((ext_vector_type(1), aligned(2)));
+template <int BYTES>
+using Bytes = std::conditional_t<BYTES % 16 == 0, Bytes16, std::conditional_t<BYTES % 8 == 0, Bytes8, Bytes4>>;
+
+// N consecutive elements starting at any multiple of the element's own size
 template <int N, typename T>
+__device__ __forceinline__ void load_n(const T* p, T (&t)[N]) {
+    if constexpr (N * sizeof(T) % 4 == 0) {
+        using B = Bytes<(int)(N * sizeof(T))>;
+#pragma unroll
+        for (size_t k = 0; k < N * sizeof(T) / sizeof(B); ++k) {
+            const B raw = reinterpret_cast<const B*>(p)[k];
+            __builtin_memcpy(reinterpret_cast<char*>(t) + k * sizeof(B), &raw, sizeof(B));
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < N; ++k) t[k] = p[k];
+    }
+}
+template <int N, typename T, std::enable_if_t<!std::is_same_v<T, float>, int> = 0>
 __device__ __forceinline__ void load_n(const T* p, float (&v)[N]) {
     T t[N];
-    __builtin_memcpy(t, p, sizeof t);
+    load_n<N>(p, t);
 #pragma unroll
     for (int k = 0; k < N; ++k) v[k] = to_f32(t[k]);
 }
@@ -32,7 +54,18 @@ __device__ __forceinline__ void store_n(T* p, const float (&v)[N]) {
     T t[N];
 #pragma unroll
     for (int k = 0; k < N; ++k) t[k] = from_f32<T>(v[k]);
-    __builtin_memcpy(p, t, sizeof t);
+    if constexpr (N * sizeof(T) % 4 == 0) {
+        using B = Bytes<(int)(N * sizeof(T))>;
+#pragma unroll
+        for (size_t k = 0; k < N * sizeof(T) / sizeof(B); ++k) {
+            B raw;
+            __builtin_memcpy(&raw, reinterpret_cast<const char*>(t) + k * sizeof(B), sizeof(B));
+            reinterpret_cast<B*>(p)[k] = raw;
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < N; ++k) p[k] = t[k];
+    }
 }
 
 // ---- values moved between the lanes of a wave, without LDS ----
@@ -82,13 +115,16 @@ int allow_lds(F* kernel, size_t dynamic_bytes) {
 }
 inline size_t type_size(int type) { return type == SDRB_F32 ? 4 : 2; }
 
-// A ragged sum: out[s, :] (+)= scale * sum over p in [start[s], start[s+1]) of weight[p] * src[index[p], :].
+// A ragged sum: out[s, :] (+)= scale * sum over the elements p of segment s of weight[p] * src[index[p], :].
 // lookup.hip runs it over a batch's rows, lookup_grad.hip over the elements sorted by id.
 struct GatherSum {
-    int device;
     uint64_t n_segments;
     uint64_t n_elems;
     const uint32_t* start;     // [n_segments + 1], or null: every segment holds n_elems / n_segments elements
+    // or, with keys given: segments are the runs of equal keys of a sorted list, n_segments is n_elems, and a run's sum goes to
+    // the row of out that its key names (a key of out_rows or more: none); a run's first element and the one after its last
+    const uint32_t *keys, *begin, *end;
+    uint64_t out_rows;
     const void* index;         // [n_elems]
     int index_bits;            // 32 or 64; an index outside [0, src_rows) contributes nothing
     const float* weight;       // [n_elems] or null: 1
@@ -101,15 +137,20 @@ struct GatherSum {
     uint64_t out_ld;
     float scale;
     bool accumulate;           // segments without elements are then left as they are
-    float* partials;           // gather_partial_bytes(...) of scratch, null where none is needed
+    uint32_t chunk;            // segments longer than this are summed in two steps (0: there are none) ...
+    float* partials;           // ... the first of which leaves its sums here: partial_bytes(...)
 };
-// Scratch for the sums of segments too long for one group of lanes: 0 when no segment can be that long.
-size_t gather_partial_bytes(uint64_t n_segments, uint64_t n_elems, bool ragged, uint32_t dim);
+// A chunk for segments of any length, 0 where none can be longer.
+uint32_t segment_chunk(uint64_t n_segments, uint64_t n_elems, bool ragged);
+uint32_t run_chunk(uint64_t n_elems);
+inline size_t partial_bytes(uint32_t chunk, uint64_t n_elems, uint32_t dim) {
+    return chunk ? (size_t)((n_elems + chunk - 1) / chunk) * 2 * dim * sizeof(float) : 0;
+}
 int launch_gather_sum(const GatherSum& g, hipStream_t stream);
 
 // lookup_grad.hip
 size_t table_grad_scratch_bytes(uint64_t n_elems, uint64_t n_table_rows, bool weighted, uint32_t dim);
-int launch_table_grad(int device, const sdrb_rows& rows, const sdrb_dense& grad, float scale, bool accumulate,
+int launch_table_grad(const sdrb_rows& rows, const sdrb_dense& grad, float scale, bool accumulate,
                       const sdrb_dense& out, void* scratch, hipStream_t stream);
 int launch_weight_grad(const sdrb_rows& rows, const sdrb_dense& grad, const sdrb_dense& table, float scale, float* out,
                        hipStream_t stream);

@@ -28,8 +28,9 @@ constexpr uint32_t kThreads = 256;
 constexpr uint32_t kNowhere = 0x80000000u;   // an offset beyond every matrix that is read by buffer loads
 
 struct GatherArgs {
-    uint64_t n_segments, n_elems, src_rows, src_ld, out_ld;
+    uint64_t n_segments, n_elems, src_rows, src_ld, out_rows, out_ld;
     const uint32_t* start;
+    const uint32_t *keys, *begin, *end;
     const void* index;
     const float* weight;
     float* partials;
@@ -48,8 +49,16 @@ struct GatherArgs {
     uint32_t accumulate;
 };
 
-// the elements [lo, hi) of a segment; offsets that run backwards or past the list are cut to it
-__device__ __forceinline__ void segment_of(const GatherArgs& a, uint64_t s, uint64_t& lo, uint64_t& hi) {
+// The elements [lo, hi) of a segment and the row its sum goes to; false where it has none.  Offsets that run backwards or past
+// the list are cut to it.
+__device__ __forceinline__ bool segment_of(const GatherArgs& a, uint64_t s, uint64_t& lo, uint64_t& hi, uint64_t& row) {
+    row = s;
+    if (a.keys) {
+        row = a.keys[s];
+        lo = a.begin[s];
+        hi = a.end[s];
+        return lo == s && row < a.out_rows;   // the run's first element speaks for it
+    }
     if (a.start) {
         lo = a.start[s];
         hi = a.start[s + 1];
@@ -59,6 +68,7 @@ __device__ __forceinline__ void segment_of(const GatherArgs& a, uint64_t s, uint
         lo = s * a.row_len;
         hi = lo + a.row_len;
     }
+    return true;
 }
 
 __device__ __forceinline__ uint32_t from_lane(uint32_t v, uint32_t lane) {
@@ -218,9 +228,10 @@ __device__ __forceinline__ void join_parts(const GatherArgs& a, uint32_t part, f
 template <int V, int SL, int LANES, int U, bool BUFFER, typename T, typename O>
 __global__ __launch_bounds__(kThreads) void k_gather_rows(GatherArgs a, const T* __restrict__ src, O* __restrict__ out) {
     __shared__ float shared[V * kThreads];
-    const Place<V, SL, LANES> at = Place<V, SL, LANES>::of_segments(a);
-    uint64_t lo = 0, hi = 0;
-    if (at.live) segment_of(a, at.item, lo, hi);
+    Place<V, SL, LANES> at = Place<V, SL, LANES>::of_segments(a);
+    uint64_t lo = 0, hi = 0, row = 0;
+    if (at.live) at.live = segment_of(a, at.item, lo, hi, row);
+    if (!at.live) lo = hi = 0;
     float acc[SL][V];
 #pragma unroll
     for (int k = 0; k < SL; ++k)
@@ -247,7 +258,7 @@ __global__ __launch_bounds__(kThreads) void k_gather_rows(GatherArgs a, const T*
 #pragma unroll
     for (int k = 0; k < SL; ++k) {
         if (!at.stores(a, k)) break;
-        O* to = out + at.item * a.out_ld + at.col[k];
+        O* to = out + row * a.out_ld + at.col[k];
         if (at.col[k] == at.own[k]) {
             if (a.accumulate) {
                 float old[V];
@@ -294,12 +305,13 @@ __global__ __launch_bounds__(kThreads) void k_gather_chunks(GatherArgs a, const 
     const uint64_t c_lo = c * a.chunk, c_hi = c_lo + a.chunk < a.n_elems ? c_lo + a.chunk : a.n_elems;
 #pragma unroll 1
     for (int end = 0; end < 2; ++end) {
-        uint64_t lo, hi;
-        if (a.start) {
-            segment_of(a, segment_at(a.start, a.n_segments, end ? c_hi - 1 : c_lo), lo, hi);
+        const uint64_t p = end ? c_hi - 1 : c_lo;
+        uint64_t lo, hi, row;
+        if (a.keys) {
+            lo = a.begin[p];
+            hi = a.keys[p] < a.out_rows ? a.end[p] : lo;
         } else {
-            lo = (end ? c_hi - 1 : c_lo) / a.row_len * a.row_len;
-            hi = lo + a.row_len;
+            segment_of(a, a.start ? segment_at(a.start, a.n_segments, p) : p / a.row_len, lo, hi, row);
         }
         if (hi - lo <= a.chunk || (end && lo <= c_lo)) continue;   // short, or the first element's segment once more
         float acc[1][V];
@@ -320,15 +332,6 @@ __global__ __launch_bounds__(kThreads) void k_gather_chunks(GatherArgs a, const 
         }
         __syncthreads();
     }
-}
-
-// The longest run of elements that one group of lanes sums by itself: long enough that few segments need a second step, short
-// enough that the longest does not outlast the rest.
-uint32_t chunk_of(uint64_t n_segments, uint64_t n_elems) {
-    const uint64_t mean = n_elems / (n_segments ? n_segments : 1);
-    uint32_t chunk = 64;
-    while (chunk < 4 * mean && chunk < 1024) chunk *= 2;
-    return chunk;
 }
 
 uint32_t log2_of(uint64_t v) {
@@ -376,7 +379,7 @@ int launch_rows(const GatherSum& g, GatherArgs a, uint64_t mean, hipStream_t str
     uint64_t grid = blocks * a.slices;
     a.xcd_slices = 0;
     a.blocks = (uint32_t)blocks;
-    if (U > 1 && blocks >= 8) {
+    if (U > 1 && LANES != 64 && blocks >= 8) {
         if (a.slices >= 8) {
             a.xcd_slices = 1;
             grid = blocks * ((a.slices + 7) / 8 * 8);
@@ -409,18 +412,29 @@ int launch_typed(const GatherSum& g, GatherArgs a, hipStream_t stream) {
         if (a.dim >= 16u * kWide) return launch_rows<kWide, 1, 16, 8, BUFFER, T, O>(g, a, mean, stream);
         return launch_rows<kWide, 1, 0, 4, BUFFER, T, O>(g, a, mean, stream);
     }
-    if (a.dim >= 64u * kEven) return launch_rows<kEven, 4, 64, 1, BUFFER, T, O>(g, a, mean, stream);
+    if (a.dim >= 64u * kEven) {
+        if (g.keys) return launch_rows<kEven, 4, 64, 2, BUFFER, T, O>(g, a, mean, stream);   // (runs have an element at least)
+        return launch_rows<kEven, 4, 64, 1, BUFFER, T, O>(g, a, mean, stream);
+    }
     return launch_rows<kEven, 1, 0, 1, BUFFER, T, O>(g, a, mean, stream);
 }
 
 }  // namespace
 
-size_t gather_partial_bytes(uint64_t n_segments, uint64_t n_elems, bool ragged, uint32_t dim) {
+// The longest run of elements that one group of lanes sums by itself: long enough that few segments need a second step, short
+// enough that the longest does not outlast the rest.
+uint32_t segment_chunk(uint64_t n_segments, uint64_t n_elems, bool ragged) {
     if (n_segments == 0 || n_elems == 0) return 0;
-    const uint32_t chunk = chunk_of(n_segments, n_elems);
-    if (!ragged && n_elems / n_segments <= chunk) return 0;
-    if (n_elems <= chunk) return 0;
-    return (size_t)((n_elems + chunk - 1) / chunk) * 2 * dim * sizeof(float);
+    const uint64_t mean = n_elems / n_segments;
+    uint32_t chunk = 64;
+    while (chunk < 4 * mean && chunk < 1024) chunk *= 2;
+    return n_elems <= chunk || (!ragged && mean <= chunk) ? 0 : chunk;
+}
+// the same for runs of a sorted list, most of them of an element or two; some 4096 chunks at most
+uint32_t run_chunk(uint64_t n_elems) {
+    uint32_t chunk = 32;
+    while (n_elems > 4096ull * chunk) chunk *= 2;
+    return n_elems <= chunk ? 0 : chunk;
 }
 
 int launch_gather_sum(const GatherSum& g, hipStream_t stream) {
@@ -439,7 +453,11 @@ int launch_gather_sum(const GatherSum& g, hipStream_t stream) {
     a.scale = g.scale;
     a.row_len = g.start ? 0u : (uint32_t)(g.n_elems / g.n_segments);
     a.dim = g.dim;
-    a.chunk = g.partials ? chunk_of(g.n_segments, g.n_elems) : 0u;
+    a.keys = g.keys;
+    a.begin = g.begin;
+    a.end = g.end;
+    a.out_rows = g.out_rows;
+    a.chunk = g.chunk;
     a.accumulate = g.accumulate ? 1u : 0u;
     return with_type(g.src_type, [&](auto t) {
         return with_type(g.out_type, [&](auto o) {

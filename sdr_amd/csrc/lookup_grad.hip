@@ -18,7 +18,7 @@ namespace {
 // holds), so they take bits(n_table_rows).  A pass sorts by a digit of them, stably: the 64 elements of a wave's turn find
 // the others of their digit by a ballot a digit bit, and a wave counts in LDS what its earlier turns have seen of each digit.
 //
-// Up to 16384 elements one block does it all in LDS (k_sort_small), 8 bits a pass, the elements in registers between passes:
+// Up to 16384 elements one block does it all in LDS (k_sort_small), 9 bits a pass, the elements in registers between passes:
 // every further launch costs more than a pass.  More elements take three launches a pass: digits counted by tile, the
 // counts summed over tiles, and the elements sent to their places.  Digits have up to 12 bits there, so that ids below
 // 4096 -- the widths of sparse codes -- need one pass, and then the counts are the segments' starts too.
@@ -80,14 +80,48 @@ __device__ __forceinline__ uint32_t rank_in_wave(uint32_t* counter, uint32_t dig
     return before + below;
 }
 constexpr uint32_t kSmall = 16384, kSmallThreads = 1024, kSmallWaves = kSmallThreads / 64, kSmallTurns = kSmall / kSmallThreads;
-constexpr uint64_t kStartsInSort = 4096;   // up to so many keys the one block finds their starts as well, four a thread
+constexpr uint32_t kSmallBits = 9, kSmallDigits = 1u << kSmallBits;
 
-__global__ __launch_bounds__(kSmallThreads) void k_sort_small(SortArgs a, uint32_t* __restrict__ keys_out, int32_t* __restrict__ row_out,
-                                                              float* __restrict__ weight_out, uint32_t* __restrict__ start) {
+// what a sort leaves behind
+struct Sorted {
+    int32_t* row;
+    float* weight;                    // or null
+    uint32_t *keys, *begin, *end;     // of the runs of equal keys, or null:
+    uint32_t* start;                  // where every key's elements start, [n_keys + 1]
+};
+// a matrix to be cleared
+struct Fill {
+    char* data;
+    uint64_t n_rows, row_bytes, ld_bytes;
+};
+__device__ __forceinline__ void fill_rows(const Fill& f, uint64_t block, uint64_t blocks, uint32_t threads) {
+    const auto clear = [](char* to, uint64_t bytes) {   // 16 of them, or what is left
+        if (bytes >= 16) {
+            *reinterpret_cast<Bytes16*>(to) = Bytes16{0, 0, 0, 0};
+        } else {
+            for (uint64_t k = 0; k < bytes; k += 2) *reinterpret_cast<uint16_t*>(to + k) = 0;
+        }
+    };
+    if (f.row_bytes == f.ld_bytes) {   // one run of bytes
+        const uint64_t n = f.n_rows * f.row_bytes, step = blocks * threads * 16;
+        for (uint64_t at = (block * threads + threadIdx.x) * 16; at < n; at += step) clear(f.data + at, n - at);
+        return;
+    }
+    for (uint64_t r = block; r < f.n_rows; r += blocks)
+        for (uint64_t at = threadIdx.x * 16; at < f.row_bytes; at += threads * 16) clear(f.data + r * f.ld_bytes + at, f.row_bytes - at);
+}
+__global__ __launch_bounds__(256) void k_fill(Fill f) { fill_rows(f, blockIdx.x, gridDim.x, 256); }
+
+// Block 0 sorts; the others clear the result meanwhile, where rows that no id names have to become zero.
+__global__ __launch_bounds__(kSmallThreads) void k_sort_small(SortArgs a, Sorted out, Fill fill) {
+    if (blockIdx.x > 0) {
+        fill_rows(fill, blockIdx.x - 1, gridDim.x - 1, kSmallThreads);
+        return;
+    }
     __shared__ uint32_t key_at[kSmall];
     __shared__ uint16_t elem_at[kSmall];
-    __shared__ uint32_t counter[kSmallWaves][256];
-    __shared__ uint32_t digit_waves[4];
+    __shared__ uint32_t counter[kSmallWaves][kSmallDigits];
+    __shared__ uint32_t digit_waves[kSmallDigits / 64], first_head[kSmallWaves], last_head[kSmallWaves];
     const uint32_t n = (uint32_t)a.n, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const uint32_t turns = (n + kSmallThreads - 1) / kSmallThreads;   // a wave owns turns * 64 neighbouring elements
     uint32_t key[kSmallTurns], elem[kSmallTurns], place[kSmallTurns];
@@ -96,18 +130,18 @@ __global__ __launch_bounds__(kSmallThreads) void k_sort_small(SortArgs a, uint32
         elem[t] = (wave * turns + t) * 64 + lane;
         key[t] = t < turns && elem[t] < n ? key_of(a, elem[t]) : 0u;
     }
-    for (uint32_t shift = 0; shift < a.key_bits; shift += 8) {
-        for (uint32_t k = threadIdx.x; k < kSmallWaves * 256; k += kSmallThreads) counter[k >> 8][k & 255] = 0;
+    for (uint32_t shift = 0; shift < a.key_bits; shift += kSmallBits) {
+        for (uint32_t k = threadIdx.x; k < kSmallWaves * kSmallDigits; k += kSmallThreads) counter[k >> kSmallBits][k & (kSmallDigits - 1)] = 0;
         __syncthreads();
 #pragma unroll
         for (uint32_t t = 0; t < kSmallTurns; ++t) {
             if (t >= turns) continue;
             // (positions, not elements, say which lanes are live: after the first pass the last ones are the largest keys)
             const bool live = (wave * turns + t) * 64 + lane < n;
-            place[t] = rank_in_wave<8>(counter[wave], (key[t] >> shift) & 255u, live);
+            place[t] = rank_in_wave<kSmallBits>(counter[wave], (key[t] >> shift) & (kSmallDigits - 1), live);
         }
         __syncthreads();
-        if (threadIdx.x < 256) {   // a digit a thread: sums over the waves, then over the digits
+        if (threadIdx.x < kSmallDigits) {   // a digit a thread: sums over the waves, then over the digits
             uint32_t total = 0;
             for (uint32_t w = 0; w < kSmallWaves; ++w) {
                 const uint32_t here = counter[w][threadIdx.x];
@@ -119,7 +153,7 @@ __global__ __launch_bounds__(kSmallThreads) void k_sort_small(SortArgs a, uint32
             key_at[threadIdx.x] = sum - total;   // (its contents have been read)
         }
         __syncthreads();
-        if (threadIdx.x < 256) {
+        if (threadIdx.x < kSmallDigits) {
             uint32_t before = key_at[threadIdx.x];
             for (uint32_t w = 0; w < wave; ++w) before += digit_waves[w];
             for (uint32_t w = 0; w < kSmallWaves; ++w) counter[w][threadIdx.x] += before;
@@ -129,7 +163,7 @@ __global__ __launch_bounds__(kSmallThreads) void k_sort_small(SortArgs a, uint32
         for (uint32_t t = 0; t < kSmallTurns; ++t) {
             if (t >= turns) continue;
             if ((wave * turns + t) * 64 + lane < n) {
-                const uint32_t to = counter[wave][(key[t] >> shift) & 255u] + place[t];
+                const uint32_t to = counter[wave][(key[t] >> shift) & (kSmallDigits - 1)] + place[t];
                 key_at[to] = key[t];
                 elem_at[to] = (uint16_t)elem[t];
             }
@@ -151,22 +185,66 @@ __global__ __launch_bounds__(kSmallThreads) void k_sort_small(SortArgs a, uint32
         if (t >= turns) continue;
         const uint32_t p = (wave * turns + t) * 64 + lane;
         if (p < n) {
-            keys_out[p] = key[t];
-            row_out[p] = (int32_t)row_of(a.off, a.n_rows, a.row_len, elem[t]);
-            if (a.weight) weight_out[p] = a.weight[elem[t]];
+            out.row[p] = (int32_t)row_of(a.off, a.n_rows, a.row_len, elem[t]);
+            if (out.weight) out.weight[p] = a.weight[elem[t]];
+            if (out.keys) out.keys[p] = key[t];
             key_at[p] = key[t];
         }
     }
-    if (a.n_keys > kStartsInSort) return;
     __syncthreads();
-    for (uint32_t v = threadIdx.x; v <= a.n_keys; v += kSmallThreads) {
-        uint32_t lo = 0, hi = n;
-        while (lo < hi) {
-            const uint32_t mid = (lo + hi) >> 1;
-            if (key_at[mid] < v) lo = mid + 1;
-            else hi = mid;
+    if (out.start) {
+        for (uint32_t v = threadIdx.x; v <= a.n_keys; v += kSmallThreads) {
+            uint32_t lo = 0, hi = n;
+            while (lo < hi) {
+                const uint32_t mid = (lo + hi) >> 1;
+                if (key_at[mid] < v) lo = mid + 1;
+                else hi = mid;
+            }
+            out.start[v] = lo;
         }
-        start[v] = lo;
+        return;
+    }
+    // A run begins at the nearest head -- an element whose key differs from the one before -- at or before, and ends at the next
+    // head after: found in the wave's ballots, and in the waves' first and last heads.
+    unsigned long long heads[kSmallTurns];
+    uint32_t first = n, last = 0;
+#pragma unroll
+    for (uint32_t t = 0; t < kSmallTurns; ++t) {
+        heads[t] = 0;
+        if (t >= turns) continue;
+        const uint32_t p0 = (wave * turns + t) * 64, p = p0 + lane;
+        heads[t] = __builtin_amdgcn_ballot_w64(p < n && (p == 0 || key_at[p - 1] != key[t]));
+        if (heads[t]) {
+            if (first == n) first = p0 + (uint32_t)__builtin_ctzll(heads[t]);
+            last = p0 + 63 - (uint32_t)__builtin_clzll(heads[t]);
+        }
+    }
+    if (lane == 0) {
+        first_head[wave] = first;
+        last_head[wave] = last;   // (0 is a head)
+    }
+    __syncthreads();
+    uint32_t before = 0, after = n;
+    for (uint32_t w = 0; w < kSmallWaves; ++w) {
+        if (w < wave) before = last_head[w] > before ? last_head[w] : before;
+        if (w > wave) after = first_head[w] < after ? first_head[w] : after;
+    }
+#pragma unroll
+    for (uint32_t t = 0; t < kSmallTurns; ++t) {
+        if (t >= turns) continue;
+        const uint32_t p0 = (wave * turns + t) * 64, p = p0 + lane;
+        const unsigned long long upto = heads[t] & (~0ull >> (63 - lane));
+        if (p < n) out.begin[p] = upto ? p0 + 63 - (uint32_t)__builtin_clzll(upto) : before;
+        if (heads[t]) before = p0 + 63 - (uint32_t)__builtin_clzll(heads[t]);
+    }
+#pragma unroll
+    for (uint32_t i = 0; i < kSmallTurns; ++i) {
+        const uint32_t t = kSmallTurns - 1 - i;
+        if (t >= turns) continue;
+        const uint32_t p0 = (wave * turns + t) * 64, p = p0 + lane;
+        const unsigned long long later = lane == 63 ? 0ull : heads[t] & (~0ull << (lane + 1));
+        if (p < n) out.end[p] = later ? p0 + (uint32_t)__builtin_ctzll(later) : after;
+        if (heads[t]) after = p0 + (uint32_t)__builtin_ctzll(heads[t]);
     }
 }
 
@@ -199,24 +277,35 @@ __global__ __launch_bounds__(256) void k_count(SortArgs a, PassArgs s) {
     for (uint32_t d = threadIdx.x; d < digits; d += 256) s.counts[(uint64_t)blockIdx.x * digits + d] = h[d];
 }
 
-// counts[tile][digit] become what the tiles before hold of the digit; totals[digit] what all do
-__global__ __launch_bounds__(64) void k_sum_tiles(PassArgs s) {
-    const uint32_t digits = 1u << s.bits, d = blockIdx.x * 64 + threadIdx.x;
-    if (d >= digits) return;
-    uint32_t total = 0;
-    uint32_t* at = s.counts + d;
-    constexpr uint32_t kAhead = 32;   // reads in flight
-    for (uint32_t t = 0; t < s.n_tiles; t += kAhead) {
-        uint32_t c[kAhead];
+// counts[tile][digit] become what the tiles before hold of the digit; totals[digit] what all do.  A block takes 64 digits, its
+// eight waves sixteen tiles each at a time, all read at once.
+constexpr uint32_t kSumWaves = 8, kSumTiles = 16;
+__global__ __launch_bounds__(64 * kSumWaves) void k_sum_tiles(PassArgs s) {
+    __shared__ uint32_t sums[kSumWaves][64];
+    const uint32_t digits = 1u << s.bits, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, d = blockIdx.x * 64 + lane;   // (digits: a multiple of 64)
+    uint32_t carry = 0;
+    for (uint32_t t0 = 0; t0 < s.n_tiles; t0 += kSumWaves * kSumTiles) {
+        const uint32_t first = t0 + wave * kSumTiles;
+        uint32_t c[kSumTiles], sum = 0;
 #pragma unroll
-        for (uint32_t k = 0; k < kAhead; ++k) c[k] = t + k < s.n_tiles ? at[(uint64_t)(t + k) * digits] : 0u;
+        for (uint32_t k = 0; k < kSumTiles; ++k) c[k] = first + k < s.n_tiles ? s.counts[(uint64_t)(first + k) * digits + d] : 0u;
 #pragma unroll
-        for (uint32_t k = 0; k < kAhead; ++k) {
-            if (t + k < s.n_tiles) at[(uint64_t)(t + k) * digits] = total;
-            total += c[k];
+        for (uint32_t k = 0; k < kSumTiles; ++k) sum += c[k];
+        sums[wave][lane] = sum;
+        __syncthreads();
+        uint32_t before = carry;
+        for (uint32_t w = 0; w < kSumWaves; ++w) {
+            before += w < wave ? sums[w][lane] : 0u;
+            carry += sums[w][lane];
+        }
+        __syncthreads();
+#pragma unroll
+        for (uint32_t k = 0; k < kSumTiles; ++k) {
+            if (first + k < s.n_tiles) s.counts[(uint64_t)(first + k) * digits + d] = before;
+            before += c[k];
         }
     }
-    s.totals[d] = total;
+    if (wave == 0) s.totals[d] = carry;
 }
 
 template <int BITS>
@@ -297,6 +386,29 @@ __global__ __launch_bounds__(256) void k_starts(const uint32_t* __restrict__ key
         else hi = mid;
     }
     start[v] = (uint32_t)lo;
+}
+
+// where the run of equal keys around every sorted position begins and ends
+__global__ __launch_bounds__(256) void k_runs(const uint32_t* __restrict__ keys, uint64_t n, uint32_t* __restrict__ begin,
+                                              uint32_t* __restrict__ end) {
+    const uint64_t p = (uint64_t)blockIdx.x * 256 + threadIdx.x;
+    if (p >= n) return;
+    const uint32_t key = keys[p];
+    uint64_t lo = 0, hi = p;   // first position whose key is `key`
+    while (lo < hi) {
+        const uint64_t mid = (lo + hi) >> 1;
+        if (keys[mid] < key) lo = mid + 1;
+        else hi = mid;
+    }
+    begin[p] = (uint32_t)lo;
+    lo = p + 1;
+    hi = n;
+    while (lo < hi) {
+        const uint64_t mid = (lo + hi) >> 1;
+        if (keys[mid] <= key) lo = mid + 1;
+        else hi = mid;
+    }
+    end[p] = (uint32_t)lo;
 }
 
 // ---- the gradient to the weights ------------------------------------------------------------------------------------------
@@ -411,14 +523,17 @@ SortArgs sort_args(const sdrb_rows& rows, uint64_t n_table_rows) {
     return a;
 }
 
-// what a sort and the sums after it keep in the caller's scratch
-struct Scratch {
-    uint32_t *keys[2], *elems[2], *counts, *totals, *start;
-    int32_t* row;
-    float* weight;
+// How the table's gradient is put together, and what it keeps in the caller's scratch.  Fewer than three elements an id on average
+// (tokens): the runs of the sorted list are summed, and the result is cleared first -- by the blocks that the sort does not
+// need, where one block sorts.  More (codes): the ids are the segments, and those without elements write their zeros.
+struct Plan {
+    bool runs, small;
+    uint32_t chunk;
+    Sorted sorted;
+    uint32_t *keys[2], *elems[2], *counts, *totals;
     float* partials;
     size_t bytes;
-    Scratch(void* base, uint64_t n, uint64_t n_keys, bool weighted, uint32_t dim) {
+    Plan(void* base, uint64_t n, uint64_t n_keys, bool weighted, uint32_t dim) {
         size_t at = 0;
         const auto take = [&](size_t count) {
             char* p = static_cast<char*>(base) + (base ? at : 0);
@@ -426,57 +541,76 @@ struct Scratch {
             return reinterpret_cast<uint32_t*>(p);
         };
         const Passes p(n, bits_of(n_keys));
-        const bool small = n <= kSmall;
-        row = reinterpret_cast<int32_t*>(take(n));
-        weight = reinterpret_cast<float*>(take(weighted ? n : 0));
-        for (int k = 0; k < 2; ++k) {   // as many as the passes write: k_starts reads the keys of more than one
-            keys[k] = take(small ? (k ? 0 : n) : p.count > 1 ? n : 0);
-            elems[k] = take(!small && p.count > 1u + k ? n : 0);
+        runs = n < 3 * n_keys;
+        small = n <= kSmall;
+        chunk = runs ? run_chunk(n) : segment_chunk(n_keys, n, true);
+        sorted.row = reinterpret_cast<int32_t*>(take(n));
+        sorted.weight = weighted ? reinterpret_cast<float*>(take(n)) : nullptr;
+        // what the passes hand on; the last one's keys where runs or starts are looked for in them
+        const bool keep = runs || (!small && p.count > 1);
+        for (uint32_t k = 0; k < 2; ++k) {
+            const bool last = (p.count - 1) % 2 == k;
+            keys[k] = take(small ? (k == 0 && keep ? n : 0) : p.count > 1 + k || (last && keep) ? n : 0);
+            elems[k] = take(!small && p.count > 1 + k ? n : 0);
         }
+        sorted.keys = keep ? keys[small ? 0 : (p.count - 1) % 2] : nullptr;
+        sorted.begin = runs ? take(n) : nullptr;
+        sorted.end = runs ? take(n) : nullptr;
+        sorted.start = runs ? nullptr : take(n_keys + 1);
         counts = take(small ? 0 : (size_t)p.n_tiles << p.bits);
         totals = take(small ? 0 : (size_t)1 << p.bits);
-        start = take(n_keys + 1);
-        partials = gather_partial_bytes(n_keys, n, true, dim) ? reinterpret_cast<float*>(take(0)) : nullptr;
-        bytes = at + gather_partial_bytes(n_keys, n, true, dim);
+        partials = reinterpret_cast<float*>(take(0));
+        bytes = at + partial_bytes(chunk, n, dim);
     }
 };
 
-int sort_by_id(const SortArgs& a, const Scratch& s, hipStream_t stream) {
-    const uint32_t* sorted = nullptr;   // keys whose starts are still to be found
-    if (a.n <= kSmall) {
-        hipLaunchKernelGGL(k_sort_small, dim3(1), dim3(kSmallThreads), 0, stream, a, s.keys[0], s.row, s.weight, s.start);
+int sort_by_id(const SortArgs& a, const Plan& s, const Fill& fill, hipStream_t stream) {
+    const uint64_t to_fill = s.runs ? fill.n_rows * fill.row_bytes : 0;
+    if (s.small) {
+        // 64 KiB or more a clearing block, and a CU each
+        const uint32_t blocks = (uint32_t)std::min<uint64_t>((to_fill + 65535) / 65536, 255);
+        hipLaunchKernelGGL(k_sort_small, dim3(1 + blocks), dim3(kSmallThreads), 0, stream, a, s.sorted, fill);
         SDRB_HIP(hipGetLastError());
-        if (a.n_keys > kStartsInSort) sorted = s.keys[0];
-    } else {
-        const Passes passes(a.n, a.key_bits);
-        for (uint32_t k = 0; k < passes.count; ++k) {
-            PassArgs p{};
-            p.keys = k ? s.keys[(k - 1) & 1] : nullptr;
-            p.elems = k ? s.elems[(k - 1) & 1] : nullptr;
-            p.counts = s.counts;
-            p.totals = s.totals;
-            p.shift = k * passes.bits;
-            p.bits = passes.bits;
-            p.turns = passes.turns;
-            p.n_tiles = passes.n_tiles;
-            p.last = k + 1 == passes.count;
-            p.keys_out = passes.count > 1 ? s.keys[k & 1] : nullptr;
-            p.elems_out = p.last ? nullptr : s.elems[k & 1];
-            p.row_out = s.row;
-            p.weight_out = s.weight;
-            p.start = passes.count == 1 ? s.start : nullptr;
-            hipLaunchKernelGGL(k_count, dim3(passes.n_tiles), dim3(256), 0, stream, a, p);
-            SDRB_HIP(hipGetLastError());
-            hipLaunchKernelGGL(k_sum_tiles, dim3(((1u << passes.bits) + 63) / 64), dim3(64), 0, stream, p);
-            SDRB_HIP(hipGetLastError());
-            const auto scatter = passes.bits == 12 ? &k_scatter<12> : passes.bits == 11 ? &k_scatter<11> : passes.bits == 10 ? &k_scatter<10> : passes.bits == 9 ? &k_scatter<9> : &k_scatter<8>;
-            hipLaunchKernelGGL(scatter, dim3(passes.n_tiles), dim3(256), 0, stream, a, p);
-            SDRB_HIP(hipGetLastError());
-        }
-        if (passes.count > 1) sorted = s.keys[(passes.count - 1) & 1];
+        return SDRB_OK;
     }
-    if (sorted) {
-        hipLaunchKernelGGL(k_starts, dim3((uint32_t)(a.n_keys / 256 + 1)), dim3(256), 0, stream, sorted, a.n, a.n_keys, s.start);
+    if (to_fill) {
+        hipLaunchKernelGGL(k_fill, dim3((uint32_t)std::min<uint64_t>((to_fill + 16383) / 16384, 2048)), dim3(256), 0, stream, fill);
+        SDRB_HIP(hipGetLastError());
+    }
+    const Passes passes(a.n, a.key_bits);
+    for (uint32_t k = 0; k < passes.count; ++k) {
+        PassArgs p{};
+        p.keys = k ? s.keys[(k - 1) & 1] : nullptr;
+        p.elems = k ? s.elems[(k - 1) & 1] : nullptr;
+        p.counts = s.counts;
+        p.totals = s.totals;
+        p.shift = k * passes.bits;
+        p.bits = passes.bits;
+        p.turns = passes.turns;
+        p.n_tiles = passes.n_tiles;
+        p.last = k + 1 == passes.count;
+        p.keys_out = p.last ? s.sorted.keys : s.keys[k & 1];
+        p.elems_out = s.elems[k & 1];
+        p.row_out = s.sorted.row;
+        p.weight_out = s.sorted.weight;
+        p.start = passes.count == 1 ? s.sorted.start : nullptr;
+        hipLaunchKernelGGL(k_count, dim3(passes.n_tiles), dim3(256), 0, stream, a, p);
+        SDRB_HIP(hipGetLastError());
+        hipLaunchKernelGGL(k_sum_tiles, dim3((1u << passes.bits) / 64), dim3(64 * kSumWaves), 0, stream, p);
+        SDRB_HIP(hipGetLastError());
+        const auto scatter = passes.bits == 12   ? &k_scatter<12>
+                             : passes.bits == 11 ? &k_scatter<11>
+                             : passes.bits == 10 ? &k_scatter<10>
+                             : passes.bits == 9  ? &k_scatter<9>
+                                                 : &k_scatter<8>;
+        hipLaunchKernelGGL(scatter, dim3(passes.n_tiles), dim3(256), 0, stream, a, p);
+        SDRB_HIP(hipGetLastError());
+    }
+    if (s.runs) {
+        hipLaunchKernelGGL(k_runs, dim3((uint32_t)((a.n + 255) / 256)), dim3(256), 0, stream, s.sorted.keys, a.n, s.sorted.begin, s.sorted.end);
+        SDRB_HIP(hipGetLastError());
+    } else if (passes.count > 1) {
+        hipLaunchKernelGGL(k_starts, dim3((uint32_t)(a.n_keys / 256 + 1)), dim3(256), 0, stream, s.sorted.keys, a.n, a.n_keys, s.sorted.start);
         SDRB_HIP(hipGetLastError());
     }
     return SDRB_OK;
@@ -485,23 +619,31 @@ int sort_by_id(const SortArgs& a, const Scratch& s, hipStream_t stream) {
 }  // namespace
 
 size_t table_grad_scratch_bytes(uint64_t n_elems, uint64_t n_table_rows, bool weighted, uint32_t dim) {
-    return Scratch(nullptr, n_elems, n_table_rows, weighted, dim).bytes;
+    return Plan(nullptr, n_elems, n_table_rows, weighted, dim).bytes;
 }
 
-int launch_table_grad(int device, const sdrb_rows& rows, const sdrb_dense& grad, float scale, bool accumulate, const sdrb_dense& out,
-                      void* scratch, hipStream_t stream) {
+int launch_table_grad(const sdrb_rows& rows, const sdrb_dense& grad, float scale, bool accumulate, const sdrb_dense& out, void* scratch,
+                      hipStream_t stream) {
     const uint32_t dim = (uint32_t)out.n_cols;
-    const Scratch s(scratch, rows.n_elems, out.n_rows, rows.weights != nullptr, dim);
+    const Plan plan(scratch, rows.n_elems, out.n_rows, rows.weights != nullptr, dim);
     const SortArgs a = sort_args(rows, out.n_rows);
-    if (const int rc = sort_by_id(a, s, stream)) return rc;
+    const size_t size = type_size(out.type);
+    const Fill fill{static_cast<char*>(out.data), accumulate ? 0 : out.n_rows, dim * size, out.ld * size};
+    if (const int rc = sort_by_id(a, plan, fill, stream)) return rc;
+    if (plan.runs && rows.n_elems == 0) return SDRB_OK;
     GatherSum g{};
-    g.device = device;
-    g.n_segments = out.n_rows;
+    g.n_segments = plan.runs ? rows.n_elems : out.n_rows;
     g.n_elems = rows.n_elems;
-    g.start = s.start;
-    g.index = s.row;
+    g.start = plan.sorted.start;
+    if (plan.runs) {
+        g.keys = plan.sorted.keys;
+        g.begin = plan.sorted.begin;
+        g.end = plan.sorted.end;
+    }
+    g.out_rows = out.n_rows;
+    g.index = plan.sorted.row;
     g.index_bits = 32;
-    g.weight = rows.weights ? s.weight : nullptr;
+    g.weight = plan.sorted.weight;
     g.src = grad.data;
     g.src_type = grad.type;
     g.src_rows = grad.n_rows;
@@ -512,7 +654,8 @@ int launch_table_grad(int device, const sdrb_rows& rows, const sdrb_dense& grad,
     g.out_ld = out.ld;
     g.scale = scale;
     g.accumulate = accumulate;
-    g.partials = s.partials;
+    g.chunk = plan.chunk;
+    g.partials = plan.partials;
     return launch_gather_sum(g, stream);
 }
 
