@@ -434,7 +434,7 @@ uint32_t segment_chunk(uint64_t n_segments, uint64_t n_elems, bool ragged) {
 uint32_t run_chunk(uint64_t n_elems) {
     uint32_t chunk = 32;
     while (n_elems > 4096ull * chunk) chunk *= 2;
-    return n_elems <= chunk ? 0 : chunk;
+    return n_elems <= 2 * chunk ? 0 : chunk;
 }
 
 int launch_gather_sum(const GatherSum& g, hipStream_t stream) {

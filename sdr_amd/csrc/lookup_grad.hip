@@ -79,7 +79,7 @@ __device__ __forceinline__ uint32_t rank_in_wave(uint32_t* counter, uint32_t dig
     __builtin_amdgcn_wave_barrier();
     return before + below;
 }
-constexpr uint32_t kSmall = 16384, kSmallThreads = 1024, kSmallWaves = kSmallThreads / 64, kSmallTurns = kSmall / kSmallThreads;
+constexpr uint32_t kSmall = 16384, kSmallThreads = 1024, kSmallWaves = kSmallThreads / 64;
 constexpr uint32_t kSmallBits = 9, kSmallDigits = 1u << kSmallBits;
 
 // what a sort leaves behind
@@ -104,7 +104,11 @@ __device__ __forceinline__ void fill_rows(const Fill& f, uint64_t block, uint64_
     };
     if (f.row_bytes == f.ld_bytes) {   // one run of bytes
         const uint64_t n = f.n_rows * f.row_bytes, step = blocks * threads * 16;
-        for (uint64_t at = (block * threads + threadIdx.x) * 16; at < n; at += step) clear(f.data + at, n - at);
+        uint64_t at = (block * threads + threadIdx.x) * 16;
+        for (; at + 3 * step + 16 <= n; at += 4 * step)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) *reinterpret_cast<Bytes16*>(f.data + at + k * step) = Bytes16{0, 0, 0, 0};
+        for (; at < n; at += step) clear(f.data + at, n - at);
         return;
     }
     for (uint64_t r = block; r < f.n_rows; r += blocks)
@@ -112,21 +116,24 @@ __device__ __forceinline__ void fill_rows(const Fill& f, uint64_t block, uint64_
 }
 __global__ __launch_bounds__(256) void k_fill(Fill f) { fill_rows(f, blockIdx.x, gridDim.x, 256); }
 
-// Block 0 sorts; the others clear the result meanwhile, where rows that no id names have to become zero.
+// Block 0 sorts up to TURNS * 1024 elements; the others clear the result meanwhile, where rows that no id names have to
+// become zero.
+template <uint32_t TURNS>
 __global__ __launch_bounds__(kSmallThreads) void k_sort_small(SortArgs a, Sorted out, Fill fill) {
     if (blockIdx.x > 0) {
         fill_rows(fill, blockIdx.x - 1, gridDim.x - 1, kSmallThreads);
         return;
     }
-    __shared__ uint32_t key_at[kSmall];
-    __shared__ uint16_t elem_at[kSmall];
+    constexpr uint32_t kRoom = TURNS * kSmallThreads > kSmallDigits ? TURNS * kSmallThreads : kSmallDigits;
+    __shared__ uint32_t key_at[kRoom];
+    __shared__ uint16_t elem_at[TURNS * kSmallThreads];
     __shared__ uint32_t counter[kSmallWaves][kSmallDigits];
     __shared__ uint32_t digit_waves[kSmallDigits / 64], first_head[kSmallWaves], last_head[kSmallWaves];
     const uint32_t n = (uint32_t)a.n, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const uint32_t turns = (n + kSmallThreads - 1) / kSmallThreads;   // a wave owns turns * 64 neighbouring elements
-    uint32_t key[kSmallTurns], elem[kSmallTurns], place[kSmallTurns];
+    uint32_t key[TURNS], elem[TURNS], place[TURNS];
 #pragma unroll
-    for (uint32_t t = 0; t < kSmallTurns; ++t) {
+    for (uint32_t t = 0; t < TURNS; ++t) {
         elem[t] = (wave * turns + t) * 64 + lane;
         key[t] = t < turns && elem[t] < n ? key_of(a, elem[t]) : 0u;
     }
@@ -134,7 +141,7 @@ __global__ __launch_bounds__(kSmallThreads) void k_sort_small(SortArgs a, Sorted
         for (uint32_t k = threadIdx.x; k < kSmallWaves * kSmallDigits; k += kSmallThreads) counter[k >> kSmallBits][k & (kSmallDigits - 1)] = 0;
         __syncthreads();
 #pragma unroll
-        for (uint32_t t = 0; t < kSmallTurns; ++t) {
+        for (uint32_t t = 0; t < TURNS; ++t) {
             if (t >= turns) continue;
             // (positions, not elements, say which lanes are live: after the first pass the last ones are the largest keys)
             const bool live = (wave * turns + t) * 64 + lane < n;
@@ -160,7 +167,7 @@ __global__ __launch_bounds__(kSmallThreads) void k_sort_small(SortArgs a, Sorted
         }
         __syncthreads();
 #pragma unroll
-        for (uint32_t t = 0; t < kSmallTurns; ++t) {
+        for (uint32_t t = 0; t < TURNS; ++t) {
             if (t >= turns) continue;
             if ((wave * turns + t) * 64 + lane < n) {
                 const uint32_t to = counter[wave][(key[t] >> shift) & (kSmallDigits - 1)] + place[t];
@@ -170,7 +177,7 @@ __global__ __launch_bounds__(kSmallThreads) void k_sort_small(SortArgs a, Sorted
         }
         __syncthreads();
 #pragma unroll
-        for (uint32_t t = 0; t < kSmallTurns; ++t) {
+        for (uint32_t t = 0; t < TURNS; ++t) {
             if (t >= turns) continue;
             const uint32_t p = (wave * turns + t) * 64 + lane;
             if (p < n) {
@@ -181,7 +188,7 @@ __global__ __launch_bounds__(kSmallThreads) void k_sort_small(SortArgs a, Sorted
         __syncthreads();
     }
 #pragma unroll
-    for (uint32_t t = 0; t < kSmallTurns; ++t) {
+    for (uint32_t t = 0; t < TURNS; ++t) {
         if (t >= turns) continue;
         const uint32_t p = (wave * turns + t) * 64 + lane;
         if (p < n) {
@@ -206,10 +213,10 @@ __global__ __launch_bounds__(kSmallThreads) void k_sort_small(SortArgs a, Sorted
     }
     // A run begins at the nearest head -- an element whose key differs from the one before -- at or before, and ends at the next
     // head after: found in the wave's ballots, and in the waves' first and last heads.
-    unsigned long long heads[kSmallTurns];
+    unsigned long long heads[TURNS];
     uint32_t first = n, last = 0;
 #pragma unroll
-    for (uint32_t t = 0; t < kSmallTurns; ++t) {
+    for (uint32_t t = 0; t < TURNS; ++t) {
         heads[t] = 0;
         if (t >= turns) continue;
         const uint32_t p0 = (wave * turns + t) * 64, p = p0 + lane;
@@ -230,7 +237,7 @@ __global__ __launch_bounds__(kSmallThreads) void k_sort_small(SortArgs a, Sorted
         if (w > wave) after = first_head[w] < after ? first_head[w] : after;
     }
 #pragma unroll
-    for (uint32_t t = 0; t < kSmallTurns; ++t) {
+    for (uint32_t t = 0; t < TURNS; ++t) {
         if (t >= turns) continue;
         const uint32_t p0 = (wave * turns + t) * 64, p = p0 + lane;
         const unsigned long long upto = heads[t] & (~0ull >> (63 - lane));
@@ -238,8 +245,8 @@ __global__ __launch_bounds__(kSmallThreads) void k_sort_small(SortArgs a, Sorted
         if (heads[t]) before = p0 + 63 - (uint32_t)__builtin_clzll(heads[t]);
     }
 #pragma unroll
-    for (uint32_t i = 0; i < kSmallTurns; ++i) {
-        const uint32_t t = kSmallTurns - 1 - i;
+    for (uint32_t i = 0; i < TURNS; ++i) {
+        const uint32_t t = TURNS - 1 - i;
         if (t >= turns) continue;
         const uint32_t p0 = (wave * turns + t) * 64, p = p0 + lane;
         const unsigned long long later = lane == 63 ? 0ull : heads[t] & (~0ull << (lane + 1));
@@ -256,7 +263,7 @@ struct PassArgs {
     uint32_t* counts;        // [tile][digit]
     uint32_t* totals;        // [digit]
     uint32_t shift, bits, turns, n_tiles;   // turns: of 64 elements a wave
-    uint32_t last;
+    uint32_t last, only;     // the only pass leaves out what contributes nothing: a key of n_keys needs no digit
     uint32_t* keys_out;
     uint32_t* elems_out;
     int32_t* row_out;        // in the last pass
@@ -271,8 +278,10 @@ __global__ __launch_bounds__(256) void k_count(SortArgs a, PassArgs s) {
     for (uint32_t d = threadIdx.x; d < digits; d += 256) h[d] = 0;
     __syncthreads();
     const uint64_t tile = (uint64_t)kTileWaves * s.turns * 64, t0 = blockIdx.x * tile;
-    for (uint64_t i = threadIdx.x; i < tile && t0 + i < a.n; i += 256)
-        atomicAdd(&h[(pass_key(a, s, t0 + i) >> s.shift) & (digits - 1)], 1u);   // (a count does not depend on their order)
+    for (uint64_t i = threadIdx.x; i < tile && t0 + i < a.n; i += 256) {
+        const uint32_t key = pass_key(a, s, t0 + i);
+        if (!s.only || key < a.n_keys) atomicAdd(&h[(key >> s.shift) & (digits - 1)], 1u);   // (a count does not depend on their order)
+    }
     __syncthreads();
     for (uint32_t d = threadIdx.x; d < digits; d += 256) s.counts[(uint64_t)blockIdx.x * digits + d] = h[d];
 }
@@ -326,7 +335,10 @@ __global__ __launch_bounds__(256) void k_scatter(SortArgs a, PassArgs s) {
     const uint64_t w0 = ((uint64_t)blockIdx.x * kTileWaves + wave) * s.turns * 64;
     for (uint32_t t = 0; t < s.turns; ++t) {
         const uint64_t p = w0 + t * 64 + lane;
-        if (p < a.n) atomicAdd(&next[wave][(pass_key(a, s, p) >> s.shift) & (kDigits - 1)], 1u);
+        if (p < a.n) {
+            const uint32_t key = pass_key(a, s, p);
+            if (!s.only || key < a.n_keys) atomicAdd(&next[wave][(key >> s.shift) & (kDigits - 1)], 1u);
+        }
     }
     // a digit's first place: the digits before it, the tiles before this one, the waves before
     uint32_t first[kEach];
@@ -347,7 +359,10 @@ __global__ __launch_bounds__(256) void k_scatter(SortArgs a, PassArgs s) {
         const uint32_t d = i * 256 + threadIdx.x;
         if (d >= kDigits) continue;
         first[i] += sums[i * 4 + wave];
-        if (s.start && blockIdx.x == 0 && d <= a.n_keys) s.start[d] = first[i];
+        if (s.start && blockIdx.x == 0) {
+            if (d < a.n_keys) s.start[d] = first[i];
+            if (d + 1 == a.n_keys) s.start[a.n_keys] = first[i] + total[i];
+        }
         uint32_t at = first[i] + tiles_before[i];
 #pragma unroll
         for (uint32_t w = 0; w < kTileWaves; ++w) {
@@ -359,8 +374,8 @@ __global__ __launch_bounds__(256) void k_scatter(SortArgs a, PassArgs s) {
     __syncthreads();
     for (uint32_t t = 0; t < s.turns; ++t) {
         const uint64_t p = w0 + t * 64 + lane;
-        const bool live = p < a.n;
-        const uint32_t key = live ? pass_key(a, s, p) : 0u;
+        const uint32_t key = p < a.n ? pass_key(a, s, p) : 0u;
+        const bool live = p < a.n && (!s.only || key < a.n_keys);
         const uint32_t to = rank_in_wave<BITS>(next[wave], (key >> s.shift) & (kDigits - 1), live);
         if (!live) continue;
         const uint32_t e = s.elems ? s.elems[p] : (uint32_t)p;
@@ -446,22 +461,27 @@ __global__ __launch_bounds__(256) void k_weight_grad(SortArgs a, const G* __rest
         const bool one_row = g[0] == g[1] && g[0] == g[2] && g[0] == g[3] && g[0] == g[4] && g[0] == g[5] && g[0] == g[6] && g[0] == g[7];
         for (uint32_t c = lane * V; c < dim; c += 64 * V) {
             if (c + V <= dim) {
-                float x[B][V], y[B][V];
+                T x[B][V];
 #pragma unroll
                 for (int j = 0; j < B; ++j) load_n<V>(t[j] + c, x[j]);
                 if (one_row) {
-                    load_n<V>(g[0] + c, y[0]);
+                    G y[V];
+                    load_n<V>(g[0] + c, y);
 #pragma unroll
                     for (int j = 0; j < B; ++j)
 #pragma unroll
-                        for (int k = 0; k < V; ++k) sum[j] = fmaf(x[j][k], y[0][k], sum[j]);
+                        for (int k = 0; k < V; ++k) sum[j] = fmaf(to_f32(x[j][k]), to_f32(y[k]), sum[j]);
                 } else {
 #pragma unroll
-                    for (int j = 0; j < B; ++j) load_n<V>(g[j] + c, y[j]);
+                    for (int h = 0; h < B; h += 4) {
+                        G y[4][V];
 #pragma unroll
-                    for (int j = 0; j < B; ++j)
+                        for (int j = 0; j < 4; ++j) load_n<V>(g[h + j] + c, y[j]);
 #pragma unroll
-                        for (int k = 0; k < V; ++k) sum[j] = fmaf(x[j][k], y[j][k], sum[j]);
+                        for (int j = 0; j < 4; ++j)
+#pragma unroll
+                            for (int k = 0; k < V; ++k) sum[h + j] = fmaf(to_f32(x[h + j][k]), to_f32(y[j][k]), sum[h + j]);
+                    }
                 }
             } else {
                 for (uint32_t k = c; k < dim; ++k)
@@ -500,7 +520,8 @@ uint32_t bits_of(uint64_t v) {
 // How many elements are sorted by more than one block: turns of 64 a wave, so that the tiles are some 500 at most, and passes.
 struct Passes {
     uint32_t turns, n_tiles, count, bits;
-    Passes(uint64_t n, uint32_t key_bits) {
+    Passes(uint64_t n, uint64_t n_keys) {
+        const uint32_t key_bits = n_keys && n_keys <= kMostDigits ? bits_of(n_keys - 1) : bits_of(n_keys);   // (one pass needs no key of n_keys)
         turns = 8;
         while (turns < 64 && n > (uint64_t)512 * kTileWaves * turns * 64) turns *= 2;
         n_tiles = (uint32_t)((n + kTileWaves * turns * 64 - 1) / (kTileWaves * turns * 64));
@@ -540,7 +561,7 @@ struct Plan {
             at += up(count * 4);
             return reinterpret_cast<uint32_t*>(p);
         };
-        const Passes p(n, bits_of(n_keys));
+        const Passes p(n, n_keys);
         runs = n < 3 * n_keys;
         small = n <= kSmall;
         chunk = runs ? run_chunk(n) : segment_chunk(n_keys, n, true);
@@ -569,7 +590,8 @@ int sort_by_id(const SortArgs& a, const Plan& s, const Fill& fill, hipStream_t s
     if (s.small) {
         // 64 KiB or more a clearing block, and a CU each
         const uint32_t blocks = (uint32_t)std::min<uint64_t>((to_fill + 65535) / 65536, 255);
-        hipLaunchKernelGGL(k_sort_small, dim3(1 + blocks), dim3(kSmallThreads), 0, stream, a, s.sorted, fill);
+        const auto sort = a.n <= kSmallThreads ? &k_sort_small<1> : a.n <= 4 * kSmallThreads ? &k_sort_small<4> : &k_sort_small<16>;
+        hipLaunchKernelGGL(sort, dim3(1 + blocks), dim3(kSmallThreads), 0, stream, a, s.sorted, fill);
         SDRB_HIP(hipGetLastError());
         return SDRB_OK;
     }
@@ -577,7 +599,7 @@ int sort_by_id(const SortArgs& a, const Plan& s, const Fill& fill, hipStream_t s
         hipLaunchKernelGGL(k_fill, dim3((uint32_t)std::min<uint64_t>((to_fill + 16383) / 16384, 2048)), dim3(256), 0, stream, fill);
         SDRB_HIP(hipGetLastError());
     }
-    const Passes passes(a.n, a.key_bits);
+    const Passes passes(a.n, a.n_keys);
     for (uint32_t k = 0; k < passes.count; ++k) {
         PassArgs p{};
         p.keys = k ? s.keys[(k - 1) & 1] : nullptr;
@@ -589,6 +611,7 @@ int sort_by_id(const SortArgs& a, const Plan& s, const Fill& fill, hipStream_t s
         p.turns = passes.turns;
         p.n_tiles = passes.n_tiles;
         p.last = k + 1 == passes.count;
+        p.only = passes.count == 1;
         p.keys_out = p.last ? s.sorted.keys : s.keys[k & 1];
         p.elems_out = s.elems[k & 1];
         p.row_out = s.sorted.row;
