@@ -89,7 +89,8 @@ struct Sorted {
     uint32_t *keys, *begin, *end;     // of the runs of equal keys, or null:
     uint32_t* start;                  // where every key's elements start, [n_keys + 1]
 };
-// a matrix to be cleared
+// A matrix to be cleared.  Measured over 512 MiB: pieces of 16 KiB a block of 256 threads 89 us, of 256 KiB a block of 1024 threads
+// 88 us, all blocks side by side through the whole matrix 112 us, the runtime's own fill 83 us.
 struct Fill {
     char* data;
     uint64_t n_rows, row_bytes, ld_bytes;
@@ -102,13 +103,10 @@ __device__ __forceinline__ void fill_rows(const Fill& f, uint64_t block, uint64_
             for (uint64_t k = 0; k < bytes; k += 2) *reinterpret_cast<uint16_t*>(to + k) = 0;
         }
     };
-    if (f.row_bytes == f.ld_bytes) {   // one run of bytes
-        const uint64_t n = f.n_rows * f.row_bytes, step = blocks * threads * 16;
-        uint64_t at = (block * threads + threadIdx.x) * 16;
-        for (; at + 3 * step + 16 <= n; at += 4 * step)
-#pragma unroll
-            for (int k = 0; k < 4; ++k) *reinterpret_cast<Bytes16*>(f.data + at + k * step) = Bytes16{0, 0, 0, 0};
-        for (; at < n; at += step) clear(f.data + at, n - at);
+    if (f.row_bytes == f.ld_bytes) {   // one run of bytes, a piece a block
+        const uint64_t n = f.n_rows * f.row_bytes, each = ((n + blocks - 1) / blocks + 15) / 16 * 16, first = block * each;
+        const uint64_t end = first + each < n ? first + each : n;
+        for (uint64_t at = first + threadIdx.x * 16; at < end; at += threads * 16) clear(f.data + at, end - at);
         return;
     }
     for (uint64_t r = block; r < f.n_rows; r += blocks)
@@ -588,15 +586,14 @@ struct Plan {
 int sort_by_id(const SortArgs& a, const Plan& s, const Fill& fill, hipStream_t stream) {
     const uint64_t to_fill = s.runs ? fill.n_rows * fill.row_bytes : 0;
     if (s.small) {
-        // 64 KiB or more a clearing block, and a CU each
-        const uint32_t blocks = (uint32_t)std::min<uint64_t>((to_fill + 65535) / 65536, 255);
+        const uint32_t blocks = (uint32_t)std::min<uint64_t>((to_fill + 262143) / 262144, 1u << 20);
         const auto sort = a.n <= kSmallThreads ? &k_sort_small<1> : a.n <= 4 * kSmallThreads ? &k_sort_small<4> : &k_sort_small<16>;
         hipLaunchKernelGGL(sort, dim3(1 + blocks), dim3(kSmallThreads), 0, stream, a, s.sorted, fill);
         SDRB_HIP(hipGetLastError());
         return SDRB_OK;
     }
     if (to_fill) {
-        hipLaunchKernelGGL(k_fill, dim3((uint32_t)std::min<uint64_t>((to_fill + 16383) / 16384, 2048)), dim3(256), 0, stream, fill);
+        hipLaunchKernelGGL(k_fill, dim3((uint32_t)std::min<uint64_t>((to_fill + 16383) / 16384, 1u << 20)), dim3(256), 0, stream, fill);
         SDRB_HIP(hipGetLastError());
     }
     const Passes passes(a.n, a.n_keys);
