@@ -22,44 +22,55 @@ from .batch import _torch_stream
 
 _SCORES = {"softmax": 0, "sigmoid": 1}
 _types = {}
+_devices = []
+_raw_stream = None
 
 
 def _torch():
     import torch  # plumbing only: device buffers and streams
     if not _types:
+        global _raw_stream
+        # the current stream's handle without making a stream object, where this torch offers it
+        _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", lambda device: torch.cuda.current_stream(device).cuda_stream)
+        _devices.extend(torch.device("cuda", k) for k in range(64))
         _types.update({torch.float32: 0, torch.float16: 1, torch.bfloat16: 2})
     return torch
 
 
 def _device_of(t) -> int:
-    if not t.is_cuda:
+    device = t.get_device()
+    if device < 0:
         raise ValueError("tensors must be on a GPU")
-    return t.device.index
+    return device
 
 
 def _matrix(name, t, device) -> Dense:
-    if t.dim() != 2 or t.dtype not in _types:
+    code = _types.get(t.dtype)
+    if code is None or t.dim() != 2:
         raise ValueError(f"{name} must be a 2-d float32, float16 or bfloat16 tensor")
-    if not t.is_cuda or t.device.index != device:
+    if t.get_device() != device:
         raise ValueError(f"{name} must be on cuda:{device} like the other tensors")
     n, m = t.shape
-    ld = t.stride(0) if n > 1 else m
-    if (m > 1 and t.stride(1) != 1) or ld < m:
+    ld, inner = t.stride()
+    if n <= 1:
+        ld = m
+    if (m > 1 and inner != 1) or ld < m:
         raise ValueError(f"{name} must have adjacent elements in a row and rows that do not overlap (call .contiguous())")
-    return Dense(t.data_ptr(), n, m, ld, _types[t.dtype])
+    return Dense(t.data_ptr(), n, m, ld, code)
 
 
 def _vector(name, t, dtype, device, shape=None):
     if t.dtype != dtype or not t.is_contiguous() or (shape is not None and t.shape != shape):
         raise ValueError(f"{name} must be a contiguous {dtype} tensor" + ("" if shape is None else f" of shape {tuple(shape)}"))
-    if not t.is_cuda or t.device.index != device:
+    if t.get_device() != device:
         raise ValueError(f"{name} must be on cuda:{device} like the other tensors")
     return t.data_ptr()
 
 
 def _rows(torch, ids, weights, offsets) -> Rows:
     device = _device_of(ids)
-    if ids.dtype not in (torch.int32, torch.int64) or not ids.is_contiguous() or ids.dim() not in (1, 2):
+    wide = ids.dtype == torch.int64
+    if not (wide or ids.dtype == torch.int32) or not ids.is_contiguous() or ids.dim() not in (1, 2):
         raise ValueError("ids must be a contiguous 1-d or 2-d int32 or int64 tensor")
     off = None
     if offsets is not None:
@@ -70,41 +81,44 @@ def _rows(torch, ids, weights, offsets) -> Rows:
     else:
         n = ids.shape[0]
     w = None if weights is None else _vector("weights", weights, torch.float32, device, ids.shape)
-    return Rows(n, ids.numel(), off, ids.data_ptr(), w, 64 if ids.dtype == torch.int64 else 32)
+    return Rows(n, ids.numel(), off, ids.data_ptr(), w, 64 if wide else 32)
 
 
 def _empty(torch, shape, dtype, device, stream):
     if stream is None:
-        return torch.empty(shape, dtype=dtype, device=torch.device("cuda", device))
+        return torch.empty(shape, dtype=dtype, device=_devices[device])
     with torch.cuda.stream(_torch_stream(device, stream)):   # memory that this stream may write at once
-        return torch.empty(shape, dtype=dtype, device=torch.device("cuda", device))
+        return torch.empty(shape, dtype=dtype, device=_devices[device])
 
 
-def _output(torch, out, shape, dtype, device, stream):
+def _result(torch, out, n, m, dtype, device, stream):
+    """(tensor, its description) of a result [n, m]: ``out``, or a new tensor"""
     if out is None:
-        return _empty(torch, shape, dtype, device, stream)
-    if tuple(out.shape) != tuple(shape) or (dtype is not None and out.dtype != dtype):
-        raise ValueError(f"out must have shape {tuple(shape)}" + ("" if dtype is None else f" and type {dtype}"))
-    return out
+        out = _empty(torch, (n, m), dtype, device, stream)
+        if dtype not in _types:
+            raise ValueError("results are float32, float16 or bfloat16")
+        return out, Dense(out.data_ptr(), n, m, m, _types[dtype])
+    if tuple(out.shape) != (n, m) or (dtype is not None and out.dtype != dtype):
+        raise ValueError(f"out must have shape {(n, m)}" + ("" if dtype is None else f" and type {dtype}"))
+    return out, _matrix("out", out, device)
 
 
 def _scratch(torch, size, device, stream):
     return (None, 0, None) if size == 0 else (t := _empty(torch, size, torch.uint8, device, stream), size, t.data_ptr())
 
 
-def _handle(torch, device, stream) -> int:
-    return (torch.cuda.current_stream(device) if stream is None else _torch_stream(device, stream)).cuda_stream
+def _handle(device, stream) -> int:
+    return _raw_stream(device) if stream is None else _torch_stream(device, stream).cuda_stream
 
 
 def _lookup(lib, rows, device, table, scale, dtype, out, stream):
     torch = _torch()
     t = _matrix("table", table, device)
-    out = _output(torch, out, (rows.n_rows, t.n_cols), dtype if out is not None else dtype or table.dtype, device, stream)
+    out, o = _result(torch, out, rows.n_rows, t.n_cols, dtype if out is not None else dtype or table.dtype, device, stream)
     need = C.c_size_t()
-    check(lib.sdrb_lookup_scratch(C.byref(rows), t.n_cols, C.byref(need)))
+    check(lib.sdrb_lookup_scratch(rows, t.n_cols, need))
     keep, size, at = _scratch(torch, need.value, device, stream)
-    o = _matrix("out", out, device)
-    check(lib.sdrb_lookup(device, C.byref(rows), C.byref(t), scale, C.byref(o), at, size, _handle(torch, device, stream)))
+    check(lib.sdrb_lookup(device, rows, t, scale, o, at, size, _handle(device, stream)))
     return out
 
 
@@ -117,22 +131,21 @@ def _lookup_grad_table(lib, rows, device, grad, n_table_rows, scale, dtype, out,
         n_table_rows = out.shape[0]
     if n_table_rows < 0:
         raise ValueError("n_table_rows must not be negative")
-    out = _output(torch, out, (n_table_rows, g.n_cols), dtype if out is not None else dtype or torch.float32, device, stream)
-    o = _matrix("out", out, device)
+    out, o = _result(torch, out, n_table_rows, g.n_cols, dtype if out is not None else dtype or torch.float32, device, stream)
     need = C.c_size_t()
-    check(lib.sdrb_lookup_grad_table_scratch(C.byref(rows), n_table_rows, g.n_cols, C.byref(need)))
+    check(lib.sdrb_lookup_grad_table_scratch(rows, n_table_rows, g.n_cols, need))
     keep, size, at = _scratch(torch, need.value, device, stream)
-    check(lib.sdrb_lookup_grad_table(device, C.byref(rows), C.byref(g), scale, int(accumulate), C.byref(o), at, size,
-                                     _handle(torch, device, stream)))
+    check(lib.sdrb_lookup_grad_table(device, rows, g, scale, int(accumulate), o, at, size, _handle(device, stream)))
     return out
 
 
 def _lookup_grad_weights(lib, rows, device, grad, table, scale, shape, out, stream):
     torch = _torch()
     g, t = _matrix("grad", grad, device), _matrix("table", table, device)
-    out = _output(torch, out, shape, torch.float32, device, stream)
-    check(lib.sdrb_lookup_grad_weights(device, C.byref(rows), C.byref(g), C.byref(t), scale,
-                                       _vector("out", out, torch.float32, device), _handle(torch, device, stream)))
+    if out is None:
+        out = _empty(torch, shape, torch.float32, device, stream)
+    check(lib.sdrb_lookup_grad_weights(device, rows, g, t, scale, _vector("out", out, torch.float32, device, torch.Size(shape)),
+                                       _handle(device, stream)))
     return out
 
 
@@ -141,7 +154,7 @@ def lookup(ids, table, weights=None, *, offsets=None, scale: float = 1.0, dtype=
     table's type unless ``dtype`` (or ``out``) says otherwise.  An embedding lookup where rows hold one id; a row without
     ids, or with none inside the table, yields zeros."""
     rows = _rows(_torch(), ids, weights, offsets)
-    return _lookup(_lib.load(), rows, ids.device.index, table, scale, dtype, out, stream)
+    return _lookup(_lib.load(), rows, ids.get_device(), table, scale, dtype, out, stream)
 
 
 def lookup_grad_table(ids, grad, n_table_rows=None, weights=None, *, offsets=None, scale: float = 1.0, dtype=None, out=None,
@@ -153,14 +166,14 @@ def lookup_grad_table(ids, grad, n_table_rows=None, weights=None, *, offsets=Non
     rows = _rows(_torch(), ids, weights, offsets)
     if n_table_rows is None and out is None:
         raise ValueError("give n_table_rows or out")
-    return _lookup_grad_table(_lib.load(), rows, ids.device.index, grad, n_table_rows, scale, dtype, out, accumulate, stream)
+    return _lookup_grad_table(_lib.load(), rows, ids.get_device(), grad, n_table_rows, scale, dtype, out, accumulate, stream)
 
 
 def lookup_grad_weights(ids, grad, table, *, offsets=None, scale: float = 1.0, out=None, stream=None):
     """The gradient of :func:`lookup` to its weights: ``scale * <grad[row], table[id]>`` an id, float32 in the shape of
     ``ids``; 0 for an id outside the table."""
     rows = _rows(_torch(), ids, None, offsets)
-    return _lookup_grad_weights(_lib.load(), rows, ids.device.index, grad, table, scale, ids.shape, out, stream)
+    return _lookup_grad_weights(_lib.load(), rows, ids.get_device(), grad, table, scale, ids.shape, out, stream)
 
 
 def _spec(torch, k, score, renormalise, scale, device, bias=None, groups=1, top_groups=None, group_top=1, n_ids=0) -> WinnersSpec:
@@ -190,7 +203,7 @@ def winners(scores, k: int, *, score: str = "softmax", bias=None, groups: int = 
     spec = _spec(torch, k, score, renormalise, scale, device, bias, groups, top_groups, group_top, s.n_cols)
     ids = _empty(torch, (s.n_rows, k), torch.int32, device, stream)
     weights = _empty(torch, (s.n_rows, k), torch.float32, device, stream)
-    check(_lib.load().sdrb_winners(device, C.byref(s), C.byref(spec), ids.data_ptr(), weights.data_ptr(), _handle(torch, device, stream)))
+    check(_lib.load().sdrb_winners(device, s, spec, ids.data_ptr(), weights.data_ptr(), _handle(device, stream)))
     return ids, weights
 
 
@@ -207,7 +220,6 @@ def winners_grad(scores, ids, grad_weights, *, score: str = "softmax", renormali
     i = _vector("ids", ids, torch.int32, device)
     g = _vector("grad_weights", grad_weights, torch.float32, device, ids.shape)
     spec = _spec(torch, ids.shape[1], score, renormalise, scale, device)
-    out = _output(torch, out, (s.n_rows, s.n_cols), dtype if out is not None else dtype or scores.dtype, device, stream)
-    o = _matrix("out", out, device)
-    check(_lib.load().sdrb_winners_grad(device, C.byref(s), C.byref(spec), i, g, C.byref(o), _handle(torch, device, stream)))
+    out, o = _result(torch, out, s.n_rows, s.n_cols, dtype if out is not None else dtype or scores.dtype, device, stream)
+    check(_lib.load().sdrb_winners_grad(device, s, spec, i, g, o, _handle(device, stream)))
     return out
