@@ -294,14 +294,14 @@ __device__ __forceinline__ uint64_t segment_at(const uint32_t* __restrict__ star
     return lo;
 }
 
-// The sums that chunk c of the element list contributes to segments longer than a chunk.  A block takes a chunk and
-// some of the slices; its groups of 8 lanes are parts of the chunk.  Where no segment is long, it finds that and ends.
+// The sums that chunk c of the element list contributes to segments longer than a chunk.  A block takes a chunk, its groups of 8
+// lanes parts of the chunk and as many slices as that leaves, one step after another.  Where no segment is long, it finds
+// that and ends: few blocks and few steps of search, since rows of unknown lengths pay for them on every call.
 template <int V, int LANES, int U, bool BUFFER, typename T>
 __global__ __launch_bounds__(kThreads) void k_gather_chunks(GatherArgs a, const T* __restrict__ src) {
     __shared__ float shared[V * kThreads];
-    const uint32_t l = lanes_log2<LANES>(a), group = threadIdx.x >> l, per_block = kThreads >> l >> a.split_log2;   // slices
-    const uint64_t c = blockIdx.x / a.blocks;
-    const Place<V, 1, LANES> at(a, (blockIdx.x % a.blocks) * per_block + (group >> a.split_log2), c);
+    const uint32_t l = lanes_log2<LANES>(a), group = threadIdx.x >> l, a_step = kThreads >> l >> a.split_log2;   // slices
+    const uint64_t c = blockIdx.x;
     const uint64_t c_lo = c * a.chunk, c_hi = c_lo + a.chunk < a.n_elems ? c_lo + a.chunk : a.n_elems;
 #pragma unroll 1
     for (int end = 0; end < 2; ++end) {
@@ -314,23 +314,26 @@ __global__ __launch_bounds__(kThreads) void k_gather_chunks(GatherArgs a, const 
             segment_of(a, a.start ? segment_at(a.start, a.n_segments, p) : p / a.row_len, lo, hi, row);
         }
         if (hi - lo <= a.chunk || (end && lo <= c_lo)) continue;   // short, or the first element's segment once more
-        float acc[1][V];
+        for (uint32_t s0 = blockIdx.y * a_step; s0 < a.slices; s0 += gridDim.y * a_step) {
+            const Place<V, 1, LANES> at(a, s0 + (group >> a.split_log2), c);
+            float acc[1][V];
 #pragma unroll
-        for (int k = 0; k < V; ++k) acc[0][k] = 0.0f;
-        if (at.live) add_elements<V, 1, LANES, U, BUFFER>(a, at, src, lo > c_lo ? lo : c_lo, hi < c_hi ? hi : c_hi, acc);
-        join_parts<V, 1, LANES>(a, at.part, acc, shared);
-        if (at.part == 0 && at.stores(a, 0)) {
-            float* to = a.partials + (2 * c + end) * a.dim + at.col[0];
-            if (at.col[0] == at.own[0]) {
-                store_n<V>(to, acc[0]);
-            } else {
-                const uint32_t skip = at.own[0] - at.col[0];
+            for (int k = 0; k < V; ++k) acc[0][k] = 0.0f;
+            if (at.live) add_elements<V, 1, LANES, U, BUFFER>(a, at, src, lo > c_lo ? lo : c_lo, hi < c_hi ? hi : c_hi, acc);
+            join_parts<V, 1, LANES>(a, at.part, acc, shared);
+            if (at.part == 0 && at.stores(a, 0)) {
+                float* to = a.partials + (2 * c + end) * a.dim + at.col[0];
+                if (at.col[0] == at.own[0]) {
+                    store_n<V>(to, acc[0]);
+                } else {
+                    const uint32_t skip = at.own[0] - at.col[0];
 #pragma unroll
-                for (int k = 0; k < V; ++k)
-                    if ((uint32_t)k >= skip) to[k] = acc[0][k];
+                    for (int k = 0; k < V; ++k)
+                        if ((uint32_t)k >= skip) to[k] = acc[0][k];
+                }
             }
+            __syncthreads();
         }
-        __syncthreads();
     }
 }
 
@@ -351,15 +354,14 @@ int launch_chunks(const GatherSum& g, GatherArgs a, hipStream_t stream) {
     a.split_log2 = std::min<uint32_t>(log2_of(groups), log2_of(std::max<uint32_t>(a.chunk >> a.lanes_log2, 1)));
     a.slices = (uint32_t)((vectors + (1u << a.lanes_log2) - 1) >> a.lanes_log2);
     while (a.split_log2 > 2 && (groups >> a.split_log2) < a.slices) --a.split_log2;
-    const uint32_t per_block = groups >> a.split_log2;
-    a.blocks = (a.slices + per_block - 1) / per_block;   // of a chunk
-    a.xcd_slices = 0;
-    if (n_chunks * a.blocks > 0x7FFFFFFFull) {
-        set_error("too many elements and columns for one launch");
+    // runs of a sorted list are known to be long or not by one load, and the long ones wait for the slowest chunk
+    const uint32_t steps = (a.slices + (groups >> a.split_log2) - 1) / (groups >> a.split_log2);
+    if (n_chunks > 0x7FFFFFull) {
+        set_error("too many elements for one launch");
         return SDRB_ERR_OVERFLOW;
     }
-    hipLaunchKernelGGL((k_gather_chunks<V, LANES, 8, BUFFER, T>), dim3((uint32_t)(n_chunks * a.blocks)), dim3(kThreads), 0, stream, a,
-                       static_cast<const T*>(g.src));
+    hipLaunchKernelGGL((k_gather_chunks<V, LANES, 8, BUFFER, T>), dim3((uint32_t)n_chunks, g.keys ? std::min(steps, 4u) : 1), dim3(kThreads), 0,
+                       stream, a, static_cast<const T*>(g.src));
     SDRB_HIP(hipGetLastError());
     return SDRB_OK;
 }

@@ -425,86 +425,95 @@ __global__ __launch_bounds__(256) void k_runs(const uint32_t* __restrict__ keys,
 }
 
 // ---- the gradient to the weights ------------------------------------------------------------------------------------------
-// A wave takes 64 elements, a lane finding the row and the table row of each, and works through them B at a time: every lane
-// loads 16 bytes of the B rows of grad and table, column after column, and the B sums over the lanes are formed together: in
-// three steps eight values a lane become one value an eighth of the lanes, half of the values changing sides each time.
-template <typename T, typename G>
+// A wave takes kDots elements, a lane finding the row and the table row of each, and works through them B at a time: every lane
+// loads 16 bytes of the B table rows and of their gradients' row, column after column, and the B sums over the lanes are
+// formed together: in three steps eight values a lane become one value an eighth of the lanes, half of the values changing
+// sides each time.  Bound: instruction issue (16 of a table row's 16 bytes' conversions and products) and L2.
+// (On the matrix cores, as the diagonal of sixteen rows times sixteen rows, the same takes 48 us where this takes 23 (8192 x 40 dot products of 512 bf16): what a
+// lane has to load there are 16 bytes of a row of its own, and L1 looks up a line for each of them.)
+constexpr uint32_t kDots = 32;
+
+// ALIGNED: rows hold a multiple of B elements each, so that B neighbours always share theirs
+template <bool ALIGNED, typename T, typename G>
 __global__ __launch_bounds__(256) void k_weight_grad(SortArgs a, const G* __restrict__ grad, uint64_t grad_ld, const T* __restrict__ table,
                                                      uint64_t table_ld, uint32_t dim, float scale, float* __restrict__ out) {
     constexpr int V = 16 / (sizeof(T) > sizeof(G) ? sizeof(T) : sizeof(G)), B = 8;
-    const uint64_t e0 = ((uint64_t)blockIdx.x * 4 + (threadIdx.x >> 6)) * 64;
+    const uint64_t e0 = ((uint64_t)blockIdx.x * 4 + (threadIdx.x >> 6)) * kDots;
     const uint32_t lane = threadIdx.x & 63;
     if (e0 >= a.n) return;
     uint32_t id = (uint32_t)a.n_keys, row = 0;
-    if (e0 + lane < a.n) {
+    if (lane < kDots && e0 + lane < a.n) {
         id = key_of(a, e0 + lane);
         row = row_of(a.off, a.n_rows, a.row_len, e0 + lane);
     }
-    float mine = 0.0f;   // of the lane's own element
-    const uint32_t n = a.n - e0 < 64 ? (uint32_t)(a.n - e0) : 64;
-    for (uint32_t u = 0; u < n; u += B) {
-        float sum[B];
+    const unsigned long long live = __builtin_amdgcn_ballot_w64(id < a.n_keys);
+    if (id >= a.n_keys) id = 0;   // (where any element is live, the matrices have rows)
+    float mine = 0.0f;            // of the lane's own element
+    for (uint32_t u = 0; u < kDots; u += B) {
+        if (((live >> u) & 0xFFu) == 0) continue;
         const T* t[B];
-        const G* g[B];
-        uint32_t live = 0;
+        uint32_t r[B];
+        bool one_row = true;
 #pragma unroll
         for (int j = 0; j < B; ++j) {
-            const uint32_t of_id = (uint32_t)__builtin_amdgcn_readlane((int)id, (int)(u + j)), of_row = (uint32_t)__builtin_amdgcn_readlane((int)row, (int)(u + j));
-            if (of_id < a.n_keys) live |= 1u << j;
-            t[j] = table + (uint64_t)(of_id < a.n_keys ? of_id : 0u) * table_ld;
-            g[j] = grad + (uint64_t)of_row * grad_ld;
-            sum[j] = 0.0f;
+            t[j] = table + (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)id, (int)u + j) * table_ld;
+            r[j] = (uint32_t)__builtin_amdgcn_readlane((int)row, (int)u + j);
+            one_row = one_row && (ALIGNED || r[j] == r[0]);
         }
-        if (live == 0) continue;
-        const bool one_row = g[0] == g[1] && g[0] == g[2] && g[0] == g[3] && g[0] == g[4] && g[0] == g[5] && g[0] == g[6] && g[0] == g[7];
+        float sum[B] = {};
+        const G* g = grad + (uint64_t)r[0] * grad_ld;
+#pragma unroll 1
         for (uint32_t c = lane * V; c < dim; c += 64 * V) {
             if (c + V <= dim) {
                 T x[B][V];
 #pragma unroll
                 for (int j = 0; j < B; ++j) load_n<V>(t[j] + c, x[j]);
-                if (one_row) {
+                if (ALIGNED || one_row) {
                     G y[V];
-                    load_n<V>(g[0] + c, y);
+                    load_n<V>(g + c, y);
 #pragma unroll
                     for (int j = 0; j < B; ++j)
 #pragma unroll
                         for (int k = 0; k < V; ++k) sum[j] = fmaf(to_f32(x[j][k]), to_f32(y[k]), sum[j]);
                 } else {
+                    G y[B][V];
 #pragma unroll
-                    for (int h = 0; h < B; h += 4) {
-                        G y[4][V];
+                    for (int j = 0; j < B; ++j) load_n<V>(grad + (uint64_t)r[j] * grad_ld + c, y[j]);
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) load_n<V>(g[h + j] + c, y[j]);
+                    for (int j = 0; j < B; ++j)
 #pragma unroll
-                        for (int j = 0; j < 4; ++j)
-#pragma unroll
-                            for (int k = 0; k < V; ++k) sum[h + j] = fmaf(to_f32(x[h + j][k]), to_f32(y[j][k]), sum[h + j]);
-                    }
+                        for (int k = 0; k < V; ++k) sum[j] = fmaf(to_f32(x[j][k]), to_f32(y[j][k]), sum[j]);
                 }
             } else {
                 for (uint32_t k = c; k < dim; ++k)
 #pragma unroll
-                    for (int j = 0; j < B; ++j) sum[j] = fmaf(to_f32(t[j][k]), to_f32(g[j][k]), sum[j]);
+                    for (int j = 0; j < B; ++j)
+                        sum[j] = fmaf(to_f32(t[j][k]), to_f32(ALIGNED ? g[k] : grad[(uint64_t)r[j] * grad_ld + k]), sum[j]);
             }
         }
-        // lane bits 0, 1, 2 choose which half of the values a lane keeps; what is left is that of element lane & 7
-        const auto halve = [&](auto count, int bit) {
-            constexpr int kHalf = decltype(count)::value / 2;
-            const bool high = (lane >> bit) & 1u;
+        // lane bits 3, 2 and 1 choose which half of the values a lane keeps; the other half comes from the lane across
 #pragma unroll
-            for (int j = 0; j < kHalf; ++j) {
-                const float keep = high ? sum[2 * j + 1] : sum[2 * j], give = high ? sum[2 * j] : sum[2 * j + 1];
-                sum[j] = keep + __shfl_xor(give, 1 << bit, 64);
-            }
-        };
-        halve(std::integral_constant<int, 8>{}, 0);
-        halve(std::integral_constant<int, 4>{}, 1);
-        halve(std::integral_constant<int, 2>{}, 2);
+        for (int j = 0; j < 4; ++j) {
+            const float keep = lane & 8 ? sum[2 * j + 1] : sum[2 * j], give = lane & 8 ? sum[2 * j] : sum[2 * j + 1];
+            sum[j] = keep + dpp<0x140, 0xF>(give, give);   // 15 - lane in a row of 16
+        }
 #pragma unroll
-        for (int s = 8; s < 64; s <<= 1) sum[0] += __shfl_xor(sum[0], s, 64);
-        if (lane >= u && lane < u + B && ((live >> (lane - u)) & 1u)) mine = scale * sum[0];   // (u is a multiple of 8)
+        for (int j = 0; j < 2; ++j) {
+            const float keep = lane & 4 ? sum[2 * j + 1] : sum[2 * j], give = lane & 4 ? sum[2 * j] : sum[2 * j + 1];
+            sum[j] = keep + dpp<0x141, 0xF>(give, give);   // 7 - lane
+        }
+        {
+            const float keep = lane & 2 ? sum[1] : sum[0], give = lane & 2 ? sum[0] : sum[1];
+            sum[0] = keep + dpp<0x1B, 0xF>(give, give);    // 3 - lane
+        }
+        sum[0] += dpp<0xB1, 0xF>(sum[0], sum[0]);          // 1 - lane
+        sum[0] += __shfl_xor(sum[0], 16, 64);
+        sum[0] += __shfl_xor(sum[0], 32, 64);
+        // bit 0 of an element lies in lane bit 3, bit 1 in bit 2, bit 2 in bit 1
+        const float dot = __shfl(sum[0], (int)((lane & 1) * 8 + (lane & 2) * 2 + (lane & 4) / 2), 64);
+        if ((lane & ~7u) == u) mine = scale * dot;
     }
-    if (e0 + lane < a.n) out[e0 + lane] = mine;
+    if (lane < kDots && e0 + lane < a.n) out[e0 + lane] = (live >> lane) & 1 ? mine : 0.0f;
 }
 
 size_t up(size_t bytes) { return (bytes + 255) / 256 * 256; }
@@ -687,7 +696,8 @@ int launch_weight_grad(const sdrb_rows& rows, const sdrb_dense& grad, const sdrb
         return with_type(grad.type, [&](auto g) {
             using T = decltype(t);
             using G = decltype(g);
-            hipLaunchKernelGGL((k_weight_grad<T, G>), dim3((uint32_t)((a.n + 255) / 256)), dim3(256), 0, stream, a,
+            const auto kernel = !a.off && a.row_len % 8 == 0 ? &k_weight_grad<true, T, G> : &k_weight_grad<false, T, G>;
+            hipLaunchKernelGGL(kernel, dim3((uint32_t)((a.n + 4 * kDots - 1) / (4 * kDots))), dim3(256), 0, stream, a,
                                static_cast<const G*>(grad.data), grad.ld, static_cast<const T*>(table.data), table.ld, (uint32_t)table.n_cols,
                                scale, out);
             SDRB_HIP(hipGetLastError());

@@ -32,8 +32,8 @@ def some_rows(g, form, n, n_table, id_type):
         return torch.where(stray > 0.95, torch.tensor(n_table), ids).to(id_type)
     if form == "tokens":
         return draw(n).cuda(), None
-    if form == "fives":
-        return draw(n, 5).cuda(), None
+    if form in ("fives", "sixteens"):
+        return draw(n, 5 if form == "fives" else 16).cuda(), None
     lens = torch.randint(0, 9, (n,), generator=g) * (torch.rand(n, generator=g) < 0.7)
     offsets = torch.zeros(n + 1, dtype=torch.int32)
     offsets[1:] = lens.cumsum(0)
@@ -179,7 +179,7 @@ def test_lookup_grad_table_of_many_ids():
     assert torch.equal(sdr_amd.lookup_grad_table(ids[:9000], go[:9000], n_table), torch.zeros(n_table, 3, device="cuda").index_add_(0, ids[:9000], go[:9000]))
 
 
-@pytest.mark.parametrize("form", ["tokens", "fives", "ragged"])
+@pytest.mark.parametrize("form", ["tokens", "fives", "sixteens", "ragged"])
 @pytest.mark.parametrize("grad,table,dim", [(F32, F32, 1), (F16, F32, 7), (BF16, BF16, 64), (F32, BF16, 100), (F16, F16, 1001), (BF16, F16, 2048)])
 def test_lookup_grad_weights(form, grad, table, dim):
     import sdr_amd
