@@ -529,7 +529,7 @@ struct Passes {
     uint32_t turns, n_tiles, count, bits;
     Passes(uint64_t n, uint64_t n_keys) {
         const uint32_t key_bits = n_keys && n_keys <= kMostDigits ? bits_of(n_keys - 1) : bits_of(n_keys);   // (one pass needs no key of n_keys)
-        turns = 8;
+        turns = 2;
         while (turns < 64 && n > (uint64_t)512 * kTileWaves * turns * 64) turns *= 2;
         n_tiles = (uint32_t)((n + kTileWaves * turns * 64 - 1) / (kTileWaves * turns * 64));
         count = (key_bits + 11) / 12;
