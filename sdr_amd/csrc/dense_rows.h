@@ -113,6 +113,16 @@ int allow_lds(F* kernel, size_t dynamic_bytes) {
         SDRB_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)dynamic_bytes));
     return SDRB_OK;
 }
+// A launch takes fewer than 2^32 threads: more blocks become several launches.  go(first block, blocks)
+template <typename F>
+int in_launches(uint64_t blocks, uint32_t threads, F&& go) {
+    const uint64_t most = 0xFFFFFFFFu / threads / 64 * 64;
+    for (uint64_t first = 0; first < blocks; first += most) {
+        const int rc = go(first, (uint32_t)(blocks - first < most ? blocks - first : most));
+        if (rc != SDRB_OK) return rc;
+    }
+    return SDRB_OK;
+}
 inline size_t type_size(int type) { return type == SDRB_F32 ? 4 : 2; }
 
 // A ragged sum: out[s, :] (+)= scale * sum over the elements p of segment s of weight[p] * src[index[p], :].

@@ -45,6 +45,7 @@ struct GatherArgs {
     uint32_t slices;         // of the columns
     uint32_t xcd_slices;     // 1: a block's slice follows from its XCD
     uint32_t blocks;         // of a slice
+    uint32_t first_block;    // of the launch
     uint32_t wide_index;     // 64-bit indexes
     uint32_t accumulate;
 };
@@ -105,12 +106,13 @@ struct Place {
     // of the segments' groups: blocks of one slice each
     __device__ __forceinline__ static Place of_segments(const GatherArgs& a) {
         const uint32_t l = lanes_log2<LANES>(a), items = kThreads >> l >> a.split_log2;   // of a block
+        const uint32_t number = a.first_block + blockIdx.x;
         uint32_t slice;
         uint64_t block;
         if (a.xcd_slices) {
             // XCD x takes the slices x, x + 8, ..., one after another over all segments (slices: 8 or more), or its share of
             // one slice's segments (slices: 1, 2 or 4)
-            const uint32_t xcd = blockIdx.x & 7, turn = blockIdx.x >> 3;
+            const uint32_t xcd = number & 7, turn = number >> 3;
             if (a.slices >= 8) {
                 slice = xcd + 8 * (turn / a.blocks);
                 block = turn % a.blocks;
@@ -119,8 +121,8 @@ struct Place {
                 block = (uint64_t)turn * (8 / a.slices) + xcd / a.slices;
             }
         } else {
-            slice = blockIdx.x % a.slices;
-            block = blockIdx.x / a.slices;
+            slice = number % a.slices;
+            block = number / a.slices;
         }
         Place p(a, slice, block * items + (threadIdx.x >> l >> a.split_log2));
         p.live = p.live && p.item < a.n_segments;
@@ -356,10 +358,6 @@ int launch_chunks(const GatherSum& g, GatherArgs a, hipStream_t stream) {
     while (a.split_log2 > 2 && (groups >> a.split_log2) < a.slices) --a.split_log2;
     // runs of a sorted list are known to be long or not by one load, and the long ones wait for the slowest chunk
     const uint32_t steps = (a.slices + (groups >> a.split_log2) - 1) / (groups >> a.split_log2);
-    if (n_chunks > 0x7FFFFFull) {
-        set_error("too many elements for one launch");
-        return SDRB_ERR_OVERFLOW;
-    }
     hipLaunchKernelGGL((k_gather_chunks<V, LANES, 8, BUFFER, T>), dim3((uint32_t)n_chunks, g.keys ? std::min(steps, 4u) : 1), dim3(kThreads), 0,
                        stream, a, static_cast<const T*>(g.src));
     SDRB_HIP(hipGetLastError());
@@ -394,10 +392,13 @@ int launch_rows(const GatherSum& g, GatherArgs a, uint64_t mean, hipStream_t str
         set_error("too many rows and columns for one launch");
         return SDRB_ERR_OVERFLOW;
     }
-    hipLaunchKernelGGL((k_gather_rows<V, SL, LANES, U, BUFFER, T, O>), dim3((uint32_t)grid), dim3(kThreads), 0, stream, a,
-                       static_cast<const T*>(g.src), static_cast<O*>(g.out));
-    SDRB_HIP(hipGetLastError());
-    return SDRB_OK;
+    return in_launches(grid, kThreads, [&](uint64_t first, uint32_t n_blocks) {
+        a.first_block = (uint32_t)first;
+        hipLaunchKernelGGL((k_gather_rows<V, SL, LANES, U, BUFFER, T, O>), dim3(n_blocks), dim3(kThreads), 0, stream, a,
+                           static_cast<const T*>(g.src), static_cast<O*>(g.out));
+        SDRB_HIP(hipGetLastError());
+        return SDRB_OK;
+    });
 }
 
 template <bool BUFFER, typename T, typename O>
@@ -429,7 +430,7 @@ uint32_t segment_chunk(uint64_t n_segments, uint64_t n_elems, bool ragged) {
     if (n_segments == 0 || n_elems == 0) return 0;
     const uint64_t mean = n_elems / n_segments;
     uint32_t chunk = 64;
-    while (chunk < 4 * mean && chunk < 1024) chunk *= 2;
+    while ((chunk < 4 * mean && chunk < 1024) || n_elems > ((uint64_t)chunk << 22)) chunk *= 2;   // (one launch: 4 million at most)
     return n_elems <= chunk || (!ragged && mean <= chunk) ? 0 : chunk;
 }
 // the same for runs of a sorted list, most of them of an element or two; some 4096 chunks at most

@@ -402,9 +402,9 @@ __global__ __launch_bounds__(256) void k_starts(const uint32_t* __restrict__ key
 }
 
 // where the run of equal keys around every sorted position begins and ends
-__global__ __launch_bounds__(256) void k_runs(const uint32_t* __restrict__ keys, uint64_t n, uint32_t* __restrict__ begin,
+__global__ __launch_bounds__(256) void k_runs(const uint32_t* __restrict__ keys, uint64_t first, uint64_t n, uint32_t* __restrict__ begin,
                                               uint32_t* __restrict__ end) {
-    const uint64_t p = (uint64_t)blockIdx.x * 256 + threadIdx.x;
+    const uint64_t p = first + (uint64_t)blockIdx.x * 256 + threadIdx.x;
     if (p >= n) return;
     const uint32_t key = keys[p];
     uint64_t lo = 0, hi = p;   // first position whose key is `key`
@@ -435,10 +435,10 @@ constexpr uint32_t kDots = 32;
 
 // ALIGNED: rows hold a multiple of B elements each, so that B neighbours always share theirs
 template <bool ALIGNED, typename T, typename G>
-__global__ __launch_bounds__(256) void k_weight_grad(SortArgs a, const G* __restrict__ grad, uint64_t grad_ld, const T* __restrict__ table,
+__global__ __launch_bounds__(256) void k_weight_grad(SortArgs a, uint64_t first, const G* __restrict__ grad, uint64_t grad_ld, const T* __restrict__ table,
                                                      uint64_t table_ld, uint32_t dim, float scale, float* __restrict__ out) {
     constexpr int V = 16 / (sizeof(T) > sizeof(G) ? sizeof(T) : sizeof(G)), B = 8;
-    const uint64_t e0 = ((uint64_t)blockIdx.x * 4 + (threadIdx.x >> 6)) * kDots;
+    const uint64_t e0 = first + ((uint64_t)blockIdx.x * 4 + (threadIdx.x >> 6)) * kDots;
     const uint32_t lane = threadIdx.x & 63;
     if (e0 >= a.n) return;
     uint32_t id = (uint32_t)a.n_keys, row = 0;
@@ -636,9 +636,13 @@ int sort_by_id(const SortArgs& a, const Plan& s, const Fill& fill, hipStream_t s
         SDRB_HIP(hipGetLastError());
     }
     if (s.runs) {
-        hipLaunchKernelGGL(k_runs, dim3((uint32_t)((a.n + 255) / 256)), dim3(256), 0, stream, s.sorted.keys, a.n, s.sorted.begin, s.sorted.end);
-        SDRB_HIP(hipGetLastError());
-    } else if (passes.count > 1) {
+        return in_launches((a.n + 255) / 256, 256, [&](uint64_t first, uint32_t blocks) {
+            hipLaunchKernelGGL(k_runs, dim3(blocks), dim3(256), 0, stream, s.sorted.keys, first * 256, a.n, s.sorted.begin, s.sorted.end);
+            SDRB_HIP(hipGetLastError());
+            return SDRB_OK;
+        });
+    }
+    if (passes.count > 1) {
         hipLaunchKernelGGL(k_starts, dim3((uint32_t)(a.n_keys / 256 + 1)), dim3(256), 0, stream, s.sorted.keys, a.n, a.n_keys, s.sorted.start);
         SDRB_HIP(hipGetLastError());
     }
@@ -697,11 +701,12 @@ int launch_weight_grad(const sdrb_rows& rows, const sdrb_dense& grad, const sdrb
             using T = decltype(t);
             using G = decltype(g);
             const auto kernel = !a.off && a.row_len % 8 == 0 ? &k_weight_grad<true, T, G> : &k_weight_grad<false, T, G>;
-            hipLaunchKernelGGL(kernel, dim3((uint32_t)((a.n + 4 * kDots - 1) / (4 * kDots))), dim3(256), 0, stream, a,
-                               static_cast<const G*>(grad.data), grad.ld, static_cast<const T*>(table.data), table.ld, (uint32_t)table.n_cols,
-                               scale, out);
-            SDRB_HIP(hipGetLastError());
-            return SDRB_OK;
+            return in_launches((a.n + 4 * kDots - 1) / (4 * kDots), 256, [&](uint64_t first, uint32_t blocks) {
+                hipLaunchKernelGGL(kernel, dim3(blocks), dim3(256), 0, stream, a, first * 4 * kDots, static_cast<const G*>(grad.data), grad.ld,
+                                   static_cast<const T*>(table.data), table.ld, (uint32_t)table.n_cols, scale, out);
+                SDRB_HIP(hipGetLastError());
+                return SDRB_OK;
+            });
         });
     });
 }

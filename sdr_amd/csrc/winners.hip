@@ -950,10 +950,14 @@ int launch_winners(const sdrb_dense& scores, const sdrb_winners_spec& spec, int3
                 a.lds_row = a.lds_groups + (spec.groups > 1 ? up(kWinnersMaxGroups + (spec.groups + 3) * (SHARES ? sizeof(double) : sizeof(float))) : 0);
                 const size_t lds = (size_t)a.lds_row * kPerBlock;
                 if (const int rc = allow_lds(&k_winners<R, THREADS, SHARES, T>, lds)) return rc;
-                hipLaunchKernelGGL((k_winners<R, THREADS, SHARES, T>), dim3((uint32_t)((a.n_rows + kPerBlock - 1) / kPerBlock)),
-                                   dim3(block_of(THREADS)), lds, stream, a, static_cast<const T*>(scores.data), ids, weights);
-                SDRB_HIP(hipGetLastError());
-                return SDRB_OK;
+                return in_launches((scores.n_rows + kPerBlock - 1) / kPerBlock, block_of(THREADS), [&](uint64_t first, uint32_t blocks) {
+                    const uint64_t row = first * kPerBlock;
+                    a.n_rows = scores.n_rows - row;
+                    hipLaunchKernelGGL((k_winners<R, THREADS, SHARES, T>), dim3(blocks), dim3(block_of(THREADS)), lds, stream, a,
+                                       static_cast<const T*>(scores.data) + row * a.ld, ids + row * spec.k, weights + row * spec.k);
+                    SDRB_HIP(hipGetLastError());
+                    return SDRB_OK;
+                });
             };
             return shares ? go(std::true_type{}) : go(std::false_type{});
         });
@@ -978,11 +982,15 @@ int launch_winners_grad(const sdrb_dense& scores, const sdrb_winners_spec& spec,
                 using O = decltype(o);
                 const auto go = [&](auto all) {
                     constexpr bool WHOLE = decltype(all)::value;
-                    hipLaunchKernelGGL((k_winners_grad<R, THREADS, WHOLE, T, O>), dim3((uint32_t)((a.n_rows + kPerBlock - 1) / kPerBlock)),
-                                       dim3(block_of(THREADS)), 0, stream, a, static_cast<const T*>(scores.data), ids, grad_weights,
-                                       static_cast<O*>(out.data));
-                    SDRB_HIP(hipGetLastError());
-                    return SDRB_OK;
+                    return in_launches((scores.n_rows + kPerBlock - 1) / kPerBlock, block_of(THREADS), [&](uint64_t first, uint32_t blocks) {
+                        const uint64_t row = first * kPerBlock;
+                        a.n_rows = scores.n_rows - row;
+                        hipLaunchKernelGGL((k_winners_grad<R, THREADS, WHOLE, T, O>), dim3(blocks), dim3(block_of(THREADS)), 0, stream, a,
+                                           static_cast<const T*>(scores.data) + row * a.ld, ids + row * spec.k, grad_weights + row * spec.k,
+                                           static_cast<O*>(out.data) + row * a.out_ld);
+                        SDRB_HIP(hipGetLastError());
+                        return SDRB_OK;
+                    });
                 };
                 return whole ? go(std::true_type{}) : go(std::false_type{});
             });

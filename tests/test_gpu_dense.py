@@ -109,6 +109,38 @@ def test_lookup_beyond_32_bit_offsets():
     assert torch.equal(sdr_amd.lookup(ids.view(2, 3), t, dtype=F32), t[ids].float().view(2, 3, dim).sum(1))
 
 
+def test_more_threads_than_one_launch_takes():
+    """a launch has fewer than 2^32 threads: rows on both sides of where the next one begins, and the last ones"""
+    import sdr_amd
+    blocks = (2 ** 32 - 1) // 256 // 64 * 64
+    g = rng(3)
+    ends = torch.arange(-70, 70, device="cuda")
+    t = matrix(g, 53, 7, BF16)
+    n = 32 * blocks + 1000   # eight lanes a row of seven columns
+    ids = torch.arange(n, dtype=torch.int32, device="cuda").remainder_(53)
+    out = torch.full((n, 7), float("nan"), dtype=BF16, device="cuda")
+    sdr_amd.lookup(ids, t, out=out)
+    for r in (32 * blocks + ends, n - 1 - ends.abs()):
+        assert torch.equal(out[r], t[ids[r].long()])
+    del out, ids
+    n = 16 * blocks + 100    # sixteen lanes a row
+    even = torch.arange(n, dtype=torch.int32, device="cuda").remainder_(2)
+    s = torch.stack([1 - even, even], 1).to(BF16)
+    won, w = sdr_amd.winners(s, 1, score="sigmoid")
+    gone = sdr_amd.winners_grad(s, won, w, score="sigmoid")
+    for r in (16 * blocks + ends, n - 1 - ends.abs()):
+        assert torch.equal(won[r, 0], even[r])
+        assert (w[r] - 0.7310586).abs().max() < 1e-6
+        assert torch.equal(gone[r] != 0, s[r] == 1)
+    del won, w, gone, s, even
+    n = 128 * blocks + 4096
+    ids = torch.arange(n, dtype=torch.int32, device="cuda").remainder_(3).view(1, n)
+    t, go = matrix(g, 3, 8, F32), matrix(g, 1, 8, F32)
+    got = sdr_amd.lookup_grad_weights(ids, go, t)
+    for r in (128 * blocks + ends, n - 1 - ends.abs()):
+        plain.assert_sum(got[0, r].view(1, -1), *(x.view(1, -1) for x in plain.lookup_grad_weights(ids[:, r], go, t)), 8)
+
+
 def test_lookup_of_non_finite_values():
     import sdr_amd
     t = torch.tensor([[1.0, float("inf"), float("nan"), 65504.0], [1.0, float("-inf"), 1.0, 65504.0], [0.0, 1.0, 1.0, 1.0]], device="cuda")
