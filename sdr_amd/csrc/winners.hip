@@ -18,8 +18,9 @@
 //     at or above the middle.
 // Shares that enter keys are computed in binary64 in the second step: whether an id wins hangs on the difference of two keys,
 // which binary32 exponentials would decide by their own error.  Groups that binary32 does not tell apart are scored again
-// exactly; rows whose candidates are too many (many equal scores, or a k above the number of threads) bisect over all their
-// keys.  Both are rolled loops that read the row anew: what runs rarely has to be short, since fetching instructions that no
+// exactly.  Rows whose candidates are too many -- large keys that few threads hold -- look for the threshold among all keys, and of
+// equal keys take the lowest ids; where more keys than the list holds lie within an error of the threshold, the row is bisected by
+// exact keys.  These are rolled loops that read the row anew: what runs rarely has to be short, since fetching instructions that no
 // other wave has run costs more than running them (straight-line code of 900 instructions: 15 us).
 // Bound: instruction issue, not memory.
 #include <type_traits>
@@ -544,10 +545,27 @@ struct Row {
         return found;
     }
 
+    // whether the ids of these registers have the same score and bias, in all threads
+    __device__ __forceinline__ bool alike(uint32_t bits) {
+        uint32_t least[2] = {0xFFFFFFFFu, 0xFFFFFFFFu}, most[2] = {0u, 0u};
+#pragma unroll 1
+        while (bits) {
+            const uint32_t id = L::id(__builtin_ctz(bits));
+            const uint32_t of[2] = {order_of(score_of(id)), a.w.bias ? order_of(a.w.bias[id] + 0.0f) : 0u};
+            bits &= bits - 1;
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                least[i] = of[i] < least[i] ? of[i] : least[i];
+                most[i] = max_u32(most[i], of[i]);
+            }
+        }
+        const bool scores = team.min(least[0]) == team.max(most[0]);
+        const bool biases = !a.w.bias || team.min(least[1]) == team.max(most[1]);
+        return scores && biases;
+    }
     // the candidates that a threshold leaves, and the winners among them; false where the row needs choose_among_all
     __device__ __forceinline__ bool choose_among_candidates(float (&key)[R], uint32_t& found) {
         const sdrb_winners_spec& w = a.w;
-        if (w.k > kMostByThreshold<THREADS> && a.n_ids > (uint32_t)THREADS * kHeld) return false;
         float slack = 0.0f;
         if constexpr (SHARES) {
             // Off by less than 3.1 * 2^-24 for the sigmoid -- 1.5 |x| + 2 steps in its exponential t, which enter the result
@@ -580,34 +598,70 @@ struct Row {
             tops[h] = order_of(most) >> kDrop;
         }
         constexpr uint32_t none = kOrderOfNone >> kDrop;
-        float t = -INFINITY;
-        if (w.k <= kMostByThreshold<THREADS> && team.template count_all<kTops>([&](int h) { return tops[h] > none; }) >= w.k) {
-            uint32_t least = 0xFFFFFFFFu, most = 0;
-#pragma unroll
-            for (int h = 0; h < kTops; ++h) {
-                least = tops[h] > none && tops[h] < least ? tops[h] : least;
-                most = max_u32(most, tops[h]);
-            }
-            uint32_t lo = team.min(least), hi = team.max(most) + 1;
+        // the key from which on `count` finds k keys, or close to it: at least k are >= lo
+        const auto find = [&](uint32_t& lo, uint32_t hi, auto count) {
             uint32_t c = 0;
+#pragma unroll 1
             while (hi - lo > 1 && c != w.k) {
                 const uint32_t mid = lo + (hi - lo) / 2;
-                c = team.template count_all<kTops>([&](int h) { return tops[h] >= mid; });
+                c = count(mid);
                 if (c >= w.k) lo = mid;
                 else hi = mid;
             }
-            t = key_at(lo << kDrop);
-            // k keys are no smaller than t less what a key can be off; a key as large may seem smaller by as much again
-            if (SHARES) t -= 2.0f * slack + fabsf(t) * 0x1p-21f;
+        };
+        uint32_t bits = 0, here[Q], place[Q], n, lo = none, most = 0;
+        const auto collect = [&](float t) {
+            bits = 0;
+#pragma unroll
+            for (int r = 0; r < R; ++r) bits |= key[r] >= t ? 1u << r : 0u;
+#pragma unroll
+            for (int q = 0; q < Q; ++q) here[q] = __popc((bits >> (q * C)) & ((1u << C) - 1u));
+            return team.places(here, place);
+        };
+        // Where k approximate keys are no smaller than t, and fewer are larger, the winners are no smaller than t - off: the k-th
+        // may seem larger than it is, and another one smaller.  (Every key > -inf; an infinite t has become a NaN, and all are
+        // candidates.)
+        const auto off = [&](float t) { return SHARES ? 2.0f * slack + fabsf(t) * 0x1p-21f : 0.0f; };
+        const auto lowered = [&](float t) { return fmaxf(SHARES ? t - off(t) : t, -3.402823466e38f); };
+        if (w.k <= kMostByThreshold<THREADS> && team.template count_all<kTops>([&](int h) { return tops[h] > none; }) >= w.k) {
+            uint32_t least = 0xFFFFFFFFu;
+#pragma unroll
+            for (int h = 0; h < kTops; ++h) least = tops[h] > none && tops[h] < least ? tops[h] : least;
+            lo = team.min(least);
         }
-        t = fmaxf(t, -3.402823466e38f);   // (every key > -inf; an infinite t has become a NaN, and all are candidates)
-        uint32_t bits = 0, here[Q], place[Q];
 #pragma unroll
-        for (int r = 0; r < R; ++r) bits |= key[r] >= t ? 1u << r : 0u;
+        for (int h = 0; h < kTops; ++h) most = max_u32(most, tops[h]);
+        most = team.max(most) + 1;
+        if (lo > none) find(lo, most, [&](uint32_t mid) { return team.template count_all<kTops>([&](int h) { return tops[h] >= mid; }); });
+        n = collect(lowered(key_at(lo << kDrop)));
+        if (n > (uint32_t)THREADS * kHeld) {
+            // too many: k of all keys instead of k of the largest
+            if (lo == none) lo = none + 1;
+            find(lo, most, [&](uint32_t mid) {
+                const float t = key_at(mid << kDrop);
+                return team.template count_all<R>([&](int r) { return key[r] >= t; });
+            });
+            const float t = key_at(lo << kDrop);
+            // keys that are larger for sure, and those that may be the k-th
+            const uint32_t more = w.k - collect(SHARES ? t + off(t) : key_at((lo + 1) << kDrop)), sure = bits;
+            n = collect(lowered(t));
+            if (n > (uint32_t)THREADS * kHeld) {
+                // too many may be the k-th: where they are equal, the lowest ids fill the places
+                bits &= ~sure;
+                if (SHARES && more && !alike(bits)) return false;
 #pragma unroll
-        for (int q = 0; q < Q; ++q) here[q] = __popc((bits >> (q * C)) & ((1u << C) - 1u));
-        const uint32_t n = team.places(here, place);
-        if (n > (uint32_t)THREADS * kHeld) return false;
+                for (int q = 0; q < Q; ++q) here[q] = __popc((bits >> (q * C)) & ((1u << C) - 1u));
+                team.places(here, place);
+                uint32_t taken = sure;
+#pragma unroll
+                for (int r = 0; r < R; ++r)
+                    if ((bits >> r) & 1u) taken |= place[r / C]++ < more ? 1u << r : 0u;
+                bits = taken;
+#pragma unroll
+                for (int q = 0; q < Q; ++q) here[q] = __popc((bits >> (q * C)) & ((1u << C) - 1u));
+                n = team.places(here, place);
+            }
+        }
         int32_t* list = reinterpret_cast<int32_t*>(mine);
 #pragma unroll
         for (int q = 0; q < Q; ++q) {
@@ -648,10 +702,10 @@ struct Row {
         const sdrb_winners_spec& w = a.w;
         bool sure;
         if (w.groups > 1) find_best_groups<K>([&](uint32_t id) { return exact_key_of(id); }, (K)0, sure);
-        const U none = order_of((K)-INFINITY) >> kDrop;
+        const U none = order_of((K)-INFINITY);
         const auto order_at = [&](uint32_t id) {
             if (w.groups > 1 && !best_ones()[__umulhi(2 * id, a.group_magic)]) return (U)0;
-            return (U)(order_of(exact_key_of(id)) >> kDrop);
+            return order_of(exact_key_of(id));
         };
         const auto count = [&](U least) {
             uint32_t c = 0;
@@ -717,7 +771,7 @@ __global__ __launch_bounds__(block_of(THREADS)) void k_winners(WinnersArgs a, co
     Row<R, THREADS, SHARES, T> x{a, scores + row * a.ld, lds + in_block * a.lds_row, {slots, starts, 0}, 0.0f, 0.0f, 0.0};
     const bool sig = x.sig();
     uint32_t found = 0;
-    bool chosen;
+    [[maybe_unused]] bool chosen;
     {
         float s[R];
         read_scores<R, THREADS>(x.s_row, a.n_ids, s);
@@ -743,9 +797,11 @@ __global__ __launch_bounds__(block_of(THREADS)) void k_winners(WinnersArgs a, co
         }
         chosen = x.choose_among_candidates(s, found);
     }
-    if (!chosen) {
-        x.team.sync();
-        found = x.choose_among_all();
+    if constexpr (SHARES) {
+        if (!chosen) {
+            x.team.sync();
+            found = x.choose_among_all();
+        }
     }
 
     // the weights, a winner a thread

@@ -326,6 +326,37 @@ def test_winners_ties_go_to_the_lowest_id(n_ids, k):
             assert_winners(sdr_amd.winners(few, k2, **more), plain.winners(few, k2, **more), weight_bound(few, n_ids, k))
 
 
+@pytest.mark.parametrize("n,n_ids,k,groups,top", [(4100, 152, 11, 4, 2), (4100, 250, 16, 10, 1), (4100, 60, 16, 1, 1), (30, 2000, 60, 8, 1), (9, 16000, 300, 1, 1),
+                                                  (5, 9000, 900, 3, 2), (5, 1500, 1024, 1, 1)])
+@pytest.mark.parametrize("dtype", [F32, F16])
+def test_winners_that_few_threads_hold(n, n_ids, k, groups, top, dtype):
+    """the largest scores side by side, in few groups, or more of them than a threshold over the threads' largest finds"""
+    import sdr_amd
+    g = rng(n_ids + k)
+    s = score_matrix(g, n, n_ids, dtype)
+    s[: n // 2, n_ids // 3: n_ids // 3 + 2 * k] += 9
+    for bias in (None, torch.randn(n_ids, generator=g).cuda() * 0.1, torch.zeros(n_ids, device="cuda")):
+        for spec in (dict(score="softmax"), dict(score="sigmoid", renormalise=True)):
+            more = dict(spec, bias=bias, groups=groups, top_groups=top, group_top=2)
+            assert_winners(sdr_amd.winners(s, k, **more), plain.winners(s, k, **more), weight_bound(s, n_ids, k))
+
+
+@pytest.mark.parametrize("n,n_ids,k", [(4100, 40, 5), (4100, 256, 16), (5, 250, 20), (5, 2048, 64), (5, 5000, 7), (5, 16384, 1024)])
+def test_winners_of_many_equal_keys(n, n_ids, k):
+    import sdr_amd
+    g = rng(n_ids * k)
+    s = torch.randint(0, 2, (n, n_ids), generator=g).float().cuda()
+    s[0], s[1], s[2, 3:] = 0.0, -7.5, float("-inf")
+    s[3] = torch.linspace(-1e-6, 1e-6, n_ids)           # not one of them equal, all within an error of binary32
+    s[4, ::2], s[4, 1::2] = 0.5, 0.5 + 2.0 ** -23       # two values within one
+    two = torch.where(torch.arange(n_ids) % 3 == 0, 0.25, -0.25).cuda()
+    for bias in (None, torch.zeros(n_ids, device="cuda"), two):
+        for score in ("softmax", "sigmoid"):
+            for more in (dict(), dict(groups=n_ids // 5, top_groups=n_ids // 10, group_top=2)) if n_ids == 250 else (dict(),):
+                got = sdr_amd.winners(s, k, score=score, bias=bias, **more)
+                assert_winners(got, plain.winners(s, k, score=score, bias=bias, **more), weight_bound(s, n_ids, k))
+
+
 def test_winners_of_close_keys():
     """sigmoids that differ by less than a step of binary32, and shares that a bias brings within one of each other"""
     import sdr_amd
