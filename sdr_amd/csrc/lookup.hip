@@ -43,8 +43,8 @@ struct GatherArgs {
     uint32_t lanes_log2;     // L
     uint32_t split_log2;     // S
     uint32_t slices;         // of the columns
-    uint32_t xcd_slices;     // 1: a block's slice follows from its XCD
-    uint32_t blocks;         // of a slice
+    uint32_t xcd_slices;     // 1: XCDs take slices one after another
+    uint32_t blocks;         // an eighth of a slice's
     uint32_t first_block;    // of the launch
     uint32_t wide_index;     // 64-bit indexes
     uint32_t accumulate;
@@ -110,16 +110,10 @@ struct Place {
         uint32_t slice;
         uint64_t block;
         if (a.xcd_slices) {
-            // XCD x takes the slices x, x + 8, ..., one after another over all segments (slices: 8 or more), or its share of
-            // one slice's segments (slices: 1, 2 or 4)
-            const uint32_t xcd = number & 7, turn = number >> 3;
-            if (a.slices >= 8) {
-                slice = xcd + 8 * (turn / a.blocks);
-                block = turn % a.blocks;
-            } else {
-                slice = xcd & (a.slices - 1);
-                block = (uint64_t)turn * (8 / a.slices) + xcd / a.slices;
-            }
+            // XCD x takes an eighth of all slices' blocks, slice by slice; of a slice that several share it takes blocks from all over
+            const uint32_t unit = (number & 7) * a.slices * a.blocks + (number >> 3), place = unit % (8 * a.blocks);
+            slice = unit / (8 * a.blocks);
+            block = (uint64_t)(place % a.blocks) * 8 + place / a.blocks;
         } else {
             slice = number % a.slices;
             block = number / a.slices;
@@ -241,17 +235,26 @@ __global__ __launch_bounds__(kThreads) void k_gather_rows(GatherArgs a, const T*
         for (int c = 0; c < V; ++c) acc[k][c] = 0.0f;
     if (a.chunk && hi - lo > a.chunk) {
         // chunk c of the element list keeps two sums: of the segment its first element lies in, and of the one its last
-        if (at.part == 0)
-            for (uint64_t c = lo / a.chunk; c * a.chunk < hi; ++c) {
-                const float* part = a.partials + (2 * c + (c * a.chunk < lo ? 1 : 0)) * a.dim;
+        // (some of them on their way at a time: an id of many elements, as words have, would keep its group waiting)
+        if (at.part == 0) {
+            constexpr int P = V > 4 ? 2 : 4;
+            const uint64_t first = lo / a.chunk, last = (hi - 1) / a.chunk;
 #pragma unroll
-                for (int k = 0; k < SL; ++k) {
-                    float v[V];
-                    load_n<V>(part + at.col[k], v);
+            for (int k = 0; k < SL; ++k)
+#pragma unroll 1
+                for (uint64_t c0 = first; c0 <= last; c0 += P) {
+                    float v[P][V];
 #pragma unroll
-                    for (int j = 0; j < V; ++j) acc[k][j] += v[j];
+                    for (int i = 0; i < P; ++i) {
+                        const uint64_t c = c0 + i < last ? c0 + i : last;
+                        load_n<V>(a.partials + (2 * c + (c * a.chunk < lo ? 1 : 0)) * a.dim + at.col[k], v[i]);
+                    }
+#pragma unroll
+                    for (int i = 0; i < P; ++i)
+#pragma unroll
+                        for (int j = 0; j < V; ++j) acc[k][j] = c0 + i <= last ? acc[k][j] + v[i][j] : acc[k][j];
                 }
-            }
+        }
     } else {
         add_elements<V, SL, LANES, U, BUFFER>(a, at, src, lo, hi, acc);
     }
@@ -376,18 +379,9 @@ int launch_rows(const GatherSum& g, GatherArgs a, uint64_t mean, hipStream_t str
     while ((kThreads >> a.lanes_log2 >> a.split_log2) > 1 && (groups << a.split_log2) < enough && (1ull << a.split_log2) << a.lanes_log2 < mean)
         ++a.split_log2;
     const uint64_t per_block = kThreads >> a.lanes_log2 >> a.split_log2, blocks = (g.n_segments + per_block - 1) / per_block;
-    uint64_t grid = blocks * a.slices;
-    a.xcd_slices = 0;
-    a.blocks = (uint32_t)blocks;
-    if (U > 1 && LANES != 64 && blocks >= 8) {
-        if (a.slices >= 8) {
-            a.xcd_slices = 1;
-            grid = blocks * ((a.slices + 7) / 8 * 8);
-        } else if ((a.slices & (a.slices - 1)) == 0) {
-            a.xcd_slices = 1;
-            grid = (blocks + 8 / a.slices - 1) / (8 / a.slices) * 8;
-        }
-    }
+    a.xcd_slices = U > 1 && LANES != 64 && blocks >= 8;
+    a.blocks = (uint32_t)((blocks + 7) / 8);
+    const uint64_t grid = (a.xcd_slices ? 8ull * a.blocks : blocks) * a.slices;
     if (grid > 0x7FFFFFFFull) {
         set_error("too many rows and columns for one launch");
         return SDRB_ERR_OVERFLOW;
@@ -411,7 +405,9 @@ int launch_typed(const GatherSum& g, GatherArgs a, hipStream_t stream) {
         if (rc != SDRB_OK) return rc;
     }
     if (mean >= 3) {
-        if (a.dim >= 32u * kWide) return launch_rows<kWide, 2, 16, 4, BUFFER, T, O>(g, a, mean, stream);
+        // two of 256 bytes a lane's turn, unless they leave a tenth more lanes without columns than slices of 256 bytes do
+        const uint32_t vectors = (a.dim + kWide - 1) / kWide, twos = (vectors + 31) / 32 * 32, ones = (vectors + 15) / 16 * 16;
+        if (vectors >= 32 && 10 * twos <= 11 * ones) return launch_rows<kWide, 2, 16, 4, BUFFER, T, O>(g, a, mean, stream);
         if (a.dim >= 16u * kWide) return launch_rows<kWide, 1, 16, 8, BUFFER, T, O>(g, a, mean, stream);
         return launch_rows<kWide, 1, 0, 4, BUFFER, T, O>(g, a, mean, stream);
     }
@@ -433,11 +429,14 @@ uint32_t segment_chunk(uint64_t n_segments, uint64_t n_elems, bool ragged) {
     while ((chunk < 4 * mean && chunk < 1024) || n_elems > ((uint64_t)chunk << 22)) chunk *= 2;   // (one launch: 4 million at most)
     return n_elems <= chunk || (!ragged && mean <= chunk) ? 0 : chunk;
 }
-// the same for runs of a sorted list, most of them of an element or two; some 4096 chunks at most
+// The same for runs of a sorted list, most of them of an element or two.  Words' frequencies make the longest run a sixteenth of
+// the list: short chunks leave its group many sums to add up, long ones many elements.  Measured with chunks of 16, 32, 64, 128 and
+// 256: 4000 elements of 512 columns 27.4, 25.9, 32, 39 and 52 us; 60000 of 1024 187, 152, 137, 154 and 201; 262144 of 512 260,
+// 260, 260, 247 and 258.
 uint32_t run_chunk(uint64_t n_elems) {
-    uint32_t chunk = 32;
-    while (n_elems > 4096ull * chunk) chunk *= 2;
-    return n_elems <= 2 * chunk ? 0 : chunk;
+    uint32_t chunk = n_elems <= 1024 ? 16 : 32;
+    while (n_elems > (chunk < 128 ? 1024ull : 4096ull) * chunk) chunk *= 2;
+    return n_elems <= 64 ? 0 : chunk;
 }
 
 int launch_gather_sum(const GatherSum& g, hipStream_t stream) {
