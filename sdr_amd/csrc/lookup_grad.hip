@@ -18,8 +18,8 @@ namespace {
 // holds), so they take bits(n_table_rows).  A pass sorts by a digit of them, stably: the 64 elements of a wave's turn find
 // the others of their digit by a ballot a digit bit, and a wave counts in LDS what its earlier turns have seen of each digit.
 //
-// Up to 16384 elements one block does it all in LDS (k_sort_small), 9 bits a pass, the elements in registers between passes:
-// every further launch costs more than a pass.  More elements take three launches a pass: digits counted by tile, the
+// Few elements one block sorts all by itself in LDS (k_sort_small), 9 bits a pass, in registers between passes: one launch, and
+// its time grows with them, since a block has one CU's issue.  More elements take three launches a pass: digits counted by tile, the
 // counts summed over tiles, and the elements sent to their places.  Digits have up to 12 bits there, so that ids below
 // 4096 -- the widths of sparse codes -- need one pass, and then the counts are the segments' starts too.
 
@@ -425,31 +425,30 @@ __global__ __launch_bounds__(256) void k_runs(const uint32_t* __restrict__ keys,
 }
 
 // ---- the gradient to the weights ------------------------------------------------------------------------------------------
-// A wave takes kDots elements, a lane finding the row and the table row of each, and works through them B at a time: every lane
+// A wave takes 8 or 16 elements, a lane finding the row and the table row of each, and works through them B at a time: every lane
 // loads 16 bytes of the B table rows and of their gradients' row, column after column, and the B sums over the lanes are
 // formed together: in three steps eight values a lane become one value an eighth of the lanes, half of the values changing
 // sides each time.  Bound: instruction issue (16 of a table row's 16 bytes' conversions and products) and L2.
-// (On the matrix cores, as the diagonal of sixteen rows times sixteen rows, the same takes 48 us where this takes 23 (8192 x 40 dot products of 512 bf16): what a
-// lane has to load there are 16 bytes of a row of its own, and L1 looks up a line for each of them.)
-constexpr uint32_t kDots = 32;
+// (On the matrix cores, as the diagonal of sixteen rows times sixteen rows, the same takes 48 us where this takes 23 (8192 x 40
+// dot products of 512 bf16): what a lane has to load there are 16 bytes of a row of its own, and L1 looks up a line for each.)
 
 // ALIGNED: rows hold a multiple of B elements each, so that B neighbours always share theirs
 template <bool ALIGNED, typename T, typename G>
-__global__ __launch_bounds__(256) void k_weight_grad(SortArgs a, uint64_t first, const G* __restrict__ grad, uint64_t grad_ld, const T* __restrict__ table,
+__global__ __launch_bounds__(256) void k_weight_grad(SortArgs a, uint64_t first, uint32_t dots, const G* __restrict__ grad, uint64_t grad_ld, const T* __restrict__ table,
                                                      uint64_t table_ld, uint32_t dim, float scale, float* __restrict__ out) {
     constexpr int V = 16 / (sizeof(T) > sizeof(G) ? sizeof(T) : sizeof(G)), B = 8;
-    const uint64_t e0 = first + ((uint64_t)blockIdx.x * 4 + (threadIdx.x >> 6)) * kDots;
+    const uint64_t e0 = first + ((uint64_t)blockIdx.x * 4 + (threadIdx.x >> 6)) * dots;
     const uint32_t lane = threadIdx.x & 63;
     if (e0 >= a.n) return;
     uint32_t id = (uint32_t)a.n_keys, row = 0;
-    if (lane < kDots && e0 + lane < a.n) {
+    if (lane < dots && e0 + lane < a.n) {
         id = key_of(a, e0 + lane);
         row = row_of(a.off, a.n_rows, a.row_len, e0 + lane);
     }
     const unsigned long long live = __builtin_amdgcn_ballot_w64(id < a.n_keys);
     if (id >= a.n_keys) id = 0;   // (where any element is live, the matrices have rows)
     float mine = 0.0f;            // of the lane's own element
-    for (uint32_t u = 0; u < kDots; u += B) {
+    for (uint32_t u = 0; u < dots; u += B) {
         if (((live >> u) & 0xFFu) == 0) continue;
         const T* t[B];
         uint32_t r[B];
@@ -513,7 +512,7 @@ __global__ __launch_bounds__(256) void k_weight_grad(SortArgs a, uint64_t first,
         const float dot = __shfl(sum[0], (int)((lane & 1) * 8 + (lane & 2) * 2 + (lane & 4) / 2), 64);
         if ((lane & ~7u) == u) mine = scale * dot;
     }
-    if (lane < kDots && e0 + lane < a.n) out[e0 + lane] = (live >> lane) & 1 ? mine : 0.0f;
+    if (lane < dots && e0 + lane < a.n) out[e0 + lane] = (live >> lane) & 1 ? mine : 0.0f;
 }
 
 size_t up(size_t bytes) { return (bytes + 255) / 256 * 256; }
@@ -570,7 +569,10 @@ struct Plan {
         };
         const Passes p(n, n_keys);
         runs = n < 3 * n_keys;
-        small = n <= kSmall;
+        // One block, or three launches a pass: 4096 elements of 2048 ids 19 us against 24, 8192 29 against 18; 8192 of 5000
+        // ids (two passes) 31 either way, 16384 44 against 31.  While a large result is cleared one block's time is hidden:
+        // 16384 with 537 MB to clear 135 us against 160, with 134 MB 77 against 75.
+        small = n <= 4096ull * p.count || (runs && n <= kSmall && n_keys * dim >= 1ull << 25);
         chunk = runs ? run_chunk(n) : segment_chunk(n_keys, n, true);
         sorted.row = reinterpret_cast<int32_t*>(take(n));
         sorted.weight = weighted ? reinterpret_cast<float*>(take(n)) : nullptr;
@@ -701,8 +703,11 @@ int launch_weight_grad(const sdrb_rows& rows, const sdrb_dense& grad, const sdrb
             using T = decltype(t);
             using G = decltype(g);
             const auto kernel = !a.off && a.row_len % 8 == 0 ? &k_weight_grad<true, T, G> : &k_weight_grad<false, T, G>;
-            return in_launches((a.n + 4 * kDots - 1) / (4 * kDots), 256, [&](uint64_t first, uint32_t blocks) {
-                hipLaunchKernelGGL(kernel, dim3(blocks), dim3(256), 0, stream, a, first * 4 * kDots, static_cast<const G*>(grad.data), grad.ld,
+            // of a wave: more of them wait less for the rows and ids of the first, fewer make more waves.  8 against 16 and 32: 1408 of
+            // 1728 columns 6.3, 10.1 and 17.8 us, 65536 of 512 7.1, 6.8 and 8.1, 262144 20.3, 18.3 and 19.3
+            const uint32_t dots = a.n < 65536 ? 8 : 16;
+            return in_launches((a.n + 4 * dots - 1) / (4 * dots), 256, [&](uint64_t first, uint32_t blocks) {
+                hipLaunchKernelGGL(kernel, dim3(blocks), dim3(256), 0, stream, a, first * 4 * dots, dots, static_cast<const G*>(grad.data), grad.ld,
                                    static_cast<const T*>(table.data), table.ld, (uint32_t)table.n_cols, scale, out);
                 SDRB_HIP(hipGetLastError());
                 return SDRB_OK;
