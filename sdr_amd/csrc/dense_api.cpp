@@ -134,7 +134,7 @@ int sdrb_lookup_grad_table_scratch(const sdrb_rows* rows, uint64_t n_table_rows,
     if (const int rc = check_rows(what, rows)) return rc;
     if (!bytes || n_cols > kMaxCols || n_table_rows > kMaxRows)
         return refuse(SDRB_ERR_INVALID_ARG, what, "bytes is null, n_cols above 2^24 or n_table_rows above 2^31-2");
-    *bytes = table_grad_scratch_bytes(rows->n_elems, n_table_rows, rows->weights != nullptr, (uint32_t)n_cols);
+    *bytes = table_grad_scratch_bytes(*rows, n_table_rows, (uint32_t)n_cols);
     return SDRB_OK;
 }
 
@@ -148,7 +148,7 @@ int sdrb_lookup_grad_table(int device, const sdrb_rows* rows, const sdrb_dense* 
     if (grad->n_rows != rows->n_rows || grad->n_cols != out->n_cols)
         return refuse(SDRB_ERR_INVALID_ARG, what, "grad must have a row for every row and the columns of out");
     if (out->n_rows == 0 || out->n_cols == 0) return SDRB_OK;
-    const size_t need = table_grad_scratch_bytes(rows->n_elems, out->n_rows, rows->weights != nullptr, (uint32_t)out->n_cols);
+    const size_t need = table_grad_scratch_bytes(*rows, out->n_rows, (uint32_t)out->n_cols);
     if (const int rc = check_scratch(what, need, scratch, scratch_bytes)) return rc;
     DeviceGuard guard(device);
     if (!guard.ok) return no_device(device);

@@ -97,6 +97,21 @@ __device__ __forceinline__ uint32_t scan_lanes(uint32_t v) {
     return v;
 }
 
+// The segment that holds element p is the last one whose first element is at or before p.  A wave looks at 64
+// segments a step.
+__device__ __forceinline__ uint64_t segment_at(const uint32_t* __restrict__ start, uint64_t n_segments, uint64_t p) {
+    uint64_t lo = 0, n = n_segments;   // it is one of [lo, lo + n)
+    while (n > 1) {
+        const uint64_t stride = (n + 63) / 64, at = lo + (threadIdx.x & 63) * stride;
+        const bool reached = at < lo + n && start[at] <= p;
+        const uint64_t last = (uint64_t)__builtin_popcountll(__builtin_amdgcn_ballot_w64(reached));   // lane 0 always, unless p is before all
+        const uint64_t step = last ? (last - 1) * stride : 0;
+        n = n - step < stride ? n - step : stride;
+        lo += step;
+    }
+    return lo;
+}
+
 // Calls f(T{}) with the element type named by `type` (checked by the caller).
 template <typename F>
 int with_type(int type, F&& f) {
@@ -159,7 +174,7 @@ inline size_t partial_bytes(uint32_t chunk, uint64_t n_elems, uint32_t dim) {
 int launch_gather_sum(const GatherSum& g, hipStream_t stream);
 
 // lookup_grad.hip
-size_t table_grad_scratch_bytes(uint64_t n_elems, uint64_t n_table_rows, bool weighted, uint32_t dim);
+size_t table_grad_scratch_bytes(const sdrb_rows& rows, uint64_t n_table_rows, uint32_t dim);
 int launch_table_grad(const sdrb_rows& rows, const sdrb_dense& grad, float scale, bool accumulate,
                       const sdrb_dense& out, void* scratch, hipStream_t stream);
 int launch_weight_grad(const sdrb_rows& rows, const sdrb_dense& grad, const sdrb_dense& table, float scale, float* out,

@@ -284,21 +284,6 @@ __global__ __launch_bounds__(kThreads) void k_gather_rows(GatherArgs a, const T*
     }
 }
 
-// The segment that holds element p (p < n_elems) is the last one whose first element is at or before p.  A wave looks at 64
-// segments a step.
-__device__ __forceinline__ uint64_t segment_at(const uint32_t* __restrict__ start, uint64_t n_segments, uint64_t p) {
-    uint64_t lo = 0, n = n_segments;   // it is one of [lo, lo + n)
-    while (n > 1) {
-        const uint64_t stride = (n + 63) / 64, at = lo + (threadIdx.x & 63) * stride;
-        const bool reached = at < lo + n && start[at] <= p;
-        const uint64_t last = (uint64_t)__builtin_popcountll(__builtin_amdgcn_ballot_w64(reached));   // lane 0 always, unless p is before all
-        const uint64_t step = last ? (last - 1) * stride : 0;
-        n = n - step < stride ? n - step : stride;
-        lo += step;
-    }
-    return lo;
-}
-
 // The sums that chunk c of the element list contributes to segments longer than a chunk.  A block takes a chunk, its groups of 8
 // lanes parts of the chunk and as many slices as that leaves, one step after another.  Where no segment is long, it finds
 // that and ends: few blocks and few steps of search, since rows of unknown lengths pay for them on every call.

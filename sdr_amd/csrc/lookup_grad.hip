@@ -86,6 +86,7 @@ constexpr uint32_t kSmallBits = 9, kSmallDigits = 1u << kSmallBits;
 struct Sorted {
     int32_t* row;
     float* weight;                    // or null
+    uint32_t* row_at;                 // of elements in their own order: one block's, where rows are ragged
     uint32_t *keys, *begin, *end;     // of the runs of equal keys, or null:
     uint32_t* start;                  // where every key's elements start, [n_keys + 1]
 };
@@ -134,6 +135,21 @@ __global__ __launch_bounds__(kSmallThreads) void k_sort_small(SortArgs a, Sorted
     for (uint32_t t = 0; t < TURNS; ++t) {
         elem[t] = (wave * turns + t) * 64 + lane;
         key[t] = t < turns && elem[t] < n ? key_of(a, elem[t]) : 0u;
+    }
+    if (a.off) {
+        // The rows, while neighbouring lanes still search for neighbouring elements, and in all turns at once (3450 elements of 1381
+        // rows: 23.5 us, and 26.4 where sorted elements look for theirs)
+        uint32_t row[TURNS] = {};
+        for (uint64_t left = a.n_rows; left > 1;) {   // row[t]: the last of so many that starts at or before the element
+            const uint32_t half = (uint32_t)(left >> 1);
+#pragma unroll
+            for (uint32_t t = 0; t < TURNS; ++t)
+                if (t < turns) row[t] = a.off[row[t] + half] <= elem[t] ? row[t] + half : row[t];
+            left -= half;
+        }
+#pragma unroll
+        for (uint32_t t = 0; t < TURNS; ++t)
+            if (t < turns && elem[t] < n) out.row_at[elem[t]] = row[t];
     }
     for (uint32_t shift = 0; shift < a.key_bits; shift += kSmallBits) {
         for (uint32_t k = threadIdx.x; k < kSmallWaves * kSmallDigits; k += kSmallThreads) counter[k >> kSmallBits][k & (kSmallDigits - 1)] = 0;
@@ -190,7 +206,7 @@ __global__ __launch_bounds__(kSmallThreads) void k_sort_small(SortArgs a, Sorted
         if (t >= turns) continue;
         const uint32_t p = (wave * turns + t) * 64 + lane;
         if (p < n) {
-            out.row[p] = (int32_t)row_of(a.off, a.n_rows, a.row_len, elem[t]);
+            out.row[p] = (int32_t)(a.off ? out.row_at[elem[t]] : elem[t] / a.row_len);
             if (out.weight) out.weight[p] = a.weight[elem[t]];
             if (out.keys) out.keys[p] = key[t];
             key_at[p] = key[t];
@@ -441,9 +457,22 @@ __global__ __launch_bounds__(256) void k_weight_grad(SortArgs a, uint64_t first,
     const uint32_t lane = threadIdx.x & 63;
     if (e0 >= a.n) return;
     uint32_t id = (uint32_t)a.n_keys, row = 0;
-    if (lane < dots && e0 + lane < a.n) {
-        id = key_of(a, e0 + lane);
-        row = row_of(a.off, a.n_rows, a.row_len, e0 + lane);
+    if (lane < dots && e0 + lane < a.n) id = key_of(a, e0 + lane);
+    if (a.off) {
+        // the row of the first one, and how many of the next 64 rows start at or before the others
+        const uint64_t row0 = segment_at(a.off, a.n_rows, e0), next = row0 + 1 + lane;
+        const uint64_t begins = next <= a.n_rows ? a.off[next] : ~0ull;
+        uint32_t passed = 0;
+        for (uint32_t u = 0; u < dots; ++u) {
+            const uint32_t k = (uint32_t)__builtin_popcountll(__builtin_amdgcn_ballot_w64(begins <= e0 + u));
+            if (lane == u) passed = k;
+        }
+        row = (uint32_t)row0 + passed;
+        if (passed == 64) row = row_of(a.off, a.n_rows, a.row_len, e0 + lane);   // (many empty rows)
+        row = row < a.n_rows ? row : 0;   // (behind the last row: an element that contributes nothing)
+    } else {
+        row = (uint32_t)(e0 + lane) / a.row_len;
+        row = row < a.n_rows ? row : 0;
     }
     const unsigned long long live = __builtin_amdgcn_ballot_w64(id < a.n_keys);
     if (id >= a.n_keys) id = 0;   // (where any element is live, the matrices have rows)
@@ -560,7 +589,7 @@ struct Plan {
     uint32_t *keys[2], *elems[2], *counts, *totals;
     float* partials;
     size_t bytes;
-    Plan(void* base, uint64_t n, uint64_t n_keys, bool weighted, uint32_t dim) {
+    Plan(void* base, uint64_t n, uint64_t n_keys, bool weighted, bool ragged, uint32_t dim) {
         size_t at = 0;
         const auto take = [&](size_t count) {
             char* p = static_cast<char*>(base) + (base ? at : 0);
@@ -576,6 +605,7 @@ struct Plan {
         chunk = runs ? run_chunk(n) : segment_chunk(n_keys, n, true);
         sorted.row = reinterpret_cast<int32_t*>(take(n));
         sorted.weight = weighted ? reinterpret_cast<float*>(take(n)) : nullptr;
+        sorted.row_at = take(small && ragged ? n : 0);
         // what the passes hand on; the last one's keys where runs or starts are looked for in them
         const bool keep = runs || (!small && p.count > 1);
         for (uint32_t k = 0; k < 2; ++k) {
@@ -653,14 +683,14 @@ int sort_by_id(const SortArgs& a, const Plan& s, const Fill& fill, hipStream_t s
 
 }  // namespace
 
-size_t table_grad_scratch_bytes(uint64_t n_elems, uint64_t n_table_rows, bool weighted, uint32_t dim) {
-    return Plan(nullptr, n_elems, n_table_rows, weighted, dim).bytes;
+size_t table_grad_scratch_bytes(const sdrb_rows& rows, uint64_t n_table_rows, uint32_t dim) {
+    return Plan(nullptr, rows.n_elems, n_table_rows, rows.weights != nullptr, rows.row_offsets != nullptr, dim).bytes;
 }
 
 int launch_table_grad(const sdrb_rows& rows, const sdrb_dense& grad, float scale, bool accumulate, const sdrb_dense& out, void* scratch,
                       hipStream_t stream) {
     const uint32_t dim = (uint32_t)out.n_cols;
-    const Plan plan(scratch, rows.n_elems, out.n_rows, rows.weights != nullptr, dim);
+    const Plan plan(scratch, rows.n_elems, out.n_rows, rows.weights != nullptr, rows.row_offsets != nullptr, dim);
     const SortArgs a = sort_args(rows, out.n_rows);
     const size_t size = type_size(out.type);
     const Fill fill{static_cast<char*>(out.data), accumulate ? 0 : out.n_rows, dim * size, out.ld * size};

@@ -227,6 +227,27 @@ def test_lookup_grad_weights(form, grad, table, dim):
     assert not got[stray].any()
 
 
+@pytest.mark.parametrize("scale", [1, 40, 1500])
+def test_lookup_gradients_of_ragged_rows_with_gaps(scale):
+    """runs of empty rows, elements before the first row and behind the last one; short lists and long ones"""
+    import sdr_amd
+    g = rng(scale)
+    lens = [0] * 70 + [3] + [0] * 63 + [1] + [0] * 64 + [2] + [0] * 200 + [17, 0, 1, 1, 1, 9, 0, 0] + [0] * 65
+    lens = [m * scale for m in lens]
+    before, behind, dim, n_table = 5, 11, 72, 90
+    offsets = torch.tensor([before] + [before + int(m) for m in np.cumsum(lens)], dtype=torch.int32).cuda()
+    total = int(offsets[-1]) + behind
+    ids = torch.randint(-1, n_table + 1, (total,), generator=g, dtype=torch.int32).cuda()
+    t, go = matrix(g, n_table, dim, BF16), matrix(g, len(lens), dim, F32)
+    w = torch.rand(total, generator=g).cuda()
+    inside = slice(before, total - behind)
+    own, at = ids[inside], (offsets - before).contiguous()
+    plain.assert_sum(sdr_amd.lookup_grad_table(ids, go, n_table, w, offsets=offsets), *plain.lookup_grad_table(own, go, n_table, w[inside], at))
+    got = sdr_amd.lookup_grad_weights(ids, go, t, offsets=offsets)
+    plain.assert_sum(got[inside], *plain.lookup_grad_weights(own, go, t, at), dim)
+    assert not got[:before].any() and not got[total - behind:].any()
+
+
 def test_lookup_gradients_against_differences():
     """the sum of result * r changes by its gradients; it is linear in table and weights, so a step of 1 has no curvature"""
     import sdr_amd
