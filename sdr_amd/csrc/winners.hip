@@ -6,9 +6,9 @@
 // Weights: scale * u, or, renormalised, scale * p with p = u / sum of the winners' u -- a softmax over the winners of
 // l = s (softmax) or l = log sigmoid(s), which holds where every u underflows.
 //
-// A team of threads owns a row and holds its scores in registers, read once: 64 threads, 512 for more than 2048 ids, or 16
-// where there are many short rows (four rows a wave: what a team does once, it does for four rows at a time).  Two steps
-// choose the winners:
+// A team of threads owns a row and holds its scores in registers, read once: 64 threads, two, four or eight times as many for
+// more than 2048, 4096 and 8192 ids, or 16 where there are many short rows (four rows a wave: what a team does once, it does
+// for four rows at a time).  Two steps choose the winners:
 //  1. Candidates.  Of the threads' largest keys -- two a thread, each of half its registers -- a threshold is found that k of
 //     them reach (a compare and a count a step), so at least k keys reach it, and few more: about 47 of 2048 for k = 40.  Keys
 //     are binary32 here; where shares enter them the threshold is lowered by what their arithmetic can be off, so that no
@@ -76,7 +76,7 @@ constexpr uint32_t kOrderOfNone = 0x007FFFFFu;   // of -inf
 template <typename T>
 constexpr int kAlike = std::is_same_v<T, bf16> ? 16 : std::is_same_v<T, f16> ? 13 : 0;
 
-// ---- the threads of a row: 16 lanes, a wave, or eight waves that meet in LDS ----
+// ---- the threads of a row: 16 lanes, a wave, or up to eight waves that meet in LDS ----
 template <int THREADS>
 struct Team {
     static constexpr int kWaves = THREADS / 64;   // 0: a row of 16 lanes
@@ -334,8 +334,7 @@ struct WinnersArgs {
 };
 
 constexpr int kHeld = 2;   // candidates a thread takes at most
-// The k for which a threshold leaves few enough candidates: with 2 * THREADS largest keys, half of them at most.  Rows of no more
-// ids than the threads hold need none.
+// The k for which the threads' largest keys, two a thread, give a threshold that leaves few enough candidates: half of them at most.
 template <int THREADS>
 constexpr uint32_t kMostByThreshold = THREADS;
 
@@ -569,9 +568,10 @@ struct Row {
         float slack = 0.0f;
         if constexpr (SHARES) {
             // Off by less than 3.1 * 2^-24 for the sigmoid -- 1.5 |x| + 2 steps in its exponential t, which enter the result
-            // with t / (1 + t)^2, and two roundings -- and than 2^-17 of the largest share for the softmax, 67 * 2^-24 by its
-            // own exponential and a sum of at most 32 + 6 + 8 additions.
-            slack = sig() ? 0x1p-22f : inv_sum * 0x1p-17f;
+            // with t / (1 + t)^2, and two roundings.  A softmax's share e^-d / sum is off by 3 d + 4 times 2^-24 of itself -- d, its
+            // product with log2 e and that constant, a step of the exponential, and two roundings -- and so by less than
+            // 4.1 * 2^-24 of the largest share there can be, 1 / sum: (3 d + 4) e^-d falls from 4 on.
+            slack = sig() ? 0x1p-22f : inv_sum * 0x1p-21f;
             float b[R];
             if (w.bias) read_row<R, THREADS>(w.bias, a.n_ids, 0.0f, b);
 #pragma unroll
@@ -609,14 +609,18 @@ struct Row {
                 else hi = mid;
             }
         };
-        uint32_t bits = 0, here[Q], place[Q], n, lo = none, most = 0;
+        uint32_t bits = 0;
+        uint32_t here[Q], place[Q], n, lo = none, most = 0;
+        const auto placed = [&]() {
+#pragma unroll
+            for (int q = 0; q < Q; ++q) here[q] = __popc((bits >> (q * C)) & ((1u << C) - 1u));
+            return team.places(here, place);
+        };
         const auto collect = [&](float t) {
             bits = 0;
 #pragma unroll
             for (int r = 0; r < R; ++r) bits |= key[r] >= t ? 1u << r : 0u;
-#pragma unroll
-            for (int q = 0; q < Q; ++q) here[q] = __popc((bits >> (q * C)) & ((1u << C) - 1u));
-            return team.places(here, place);
+            return placed();
         };
         // Where k approximate keys are no smaller than t, and fewer are larger, the winners are no smaller than t - off: the k-th
         // may seem larger than it is, and another one smaller.  (Every key > -inf; an infinite t has become a NaN, and all are
@@ -643,23 +647,20 @@ struct Row {
             });
             const float t = key_at(lo << kDrop);
             // keys that are larger for sure, and those that may be the k-th
-            const uint32_t more = w.k - collect(SHARES ? t + off(t) : key_at((lo + 1) << kDrop)), sure = bits;
+            const uint32_t more = w.k - collect(SHARES ? t + off(t) : key_at((lo + 1) << kDrop));
+            const uint32_t sure = bits;
             n = collect(lowered(t));
             if (n > (uint32_t)THREADS * kHeld) {
                 // too many may be the k-th: where they are equal, the lowest ids fill the places
                 bits &= ~sure;
                 if (SHARES && more && !alike(bits)) return false;
-#pragma unroll
-                for (int q = 0; q < Q; ++q) here[q] = __popc((bits >> (q * C)) & ((1u << C) - 1u));
-                team.places(here, place);
+                placed();
                 uint32_t taken = sure;
 #pragma unroll
                 for (int r = 0; r < R; ++r)
                     if ((bits >> r) & 1u) taken |= place[r / C]++ < more ? 1u << r : 0u;
                 bits = taken;
-#pragma unroll
-                for (int q = 0; q < Q; ++q) here[q] = __popc((bits >> (q * C)) & ((1u << C) - 1u));
-                n = team.places(here, place);
+                n = placed();
             }
         }
         int32_t* list = reinterpret_cast<int32_t*>(mine);
@@ -754,8 +755,7 @@ struct Row {
     }
 };
 
-// (k is at most 16, 128 and 1024 for 16, 64 and 512 threads)
-constexpr uint32_t block_of(int threads) { return threads < 256 ? 256 : threads; }
+constexpr uint32_t block_of(int threads) { return threads <= 64 ? 256 : threads; }
 
 template <int R, int THREADS, bool SHARES, typename T>
 __global__ __launch_bounds__(block_of(THREADS)) void k_winners(WinnersArgs a, const T* __restrict__ scores, int32_t* __restrict__ out_ids,
@@ -951,15 +951,20 @@ __global__ __launch_bounds__(block_of(THREADS)) void k_winners_grad(WinnersGradA
         }
 }
 
-// Calls f(R, THREADS) with the smallest layout that holds n ids and chooses k of them by a threshold.  Four rows share a wave
-// where rows are short and enough of them to fill the chip that way (1024 SIMDs, a wave each); with fewer the row's latency
-// counts, and 64 lanes have less to do each.
+// Calls f(R, THREADS) for rows of n ids, k of which win: as few waves as hold the ids in 32 registers and choose k of them by a
+// threshold.  Waves that meet in LDS at every step of a bisection cost more than registers do: 4096 rows of 4096 ids, k = 40,
+// take 22.6 us with two waves a row and 72.7 with eight, 64 such rows 8.9 and 13.5, a single one 8.5 and 13.0.  (Beyond 32 the
+// registers cost more: 4096 rows of 16384 ids, k = 328, 122 us with eight waves and 191 with four.)
+// Four rows share a wave where rows are short and enough of them to fill the chip that way (1024 SIMDs, a wave each); with fewer
+// the row's latency counts, and 64 lanes have less to do each.
 template <typename F>
 int with_layout(uint32_t n, uint64_t n_rows, uint32_t k, F&& f) {
     using std::integral_constant;
     const auto lanes = integral_constant<int, 16>{};
     const auto wave = integral_constant<int, 64>{};
-    const auto waves = integral_constant<int, 512>{};
+    const auto two = integral_constant<int, 128>{};
+    const auto four = integral_constant<int, 256>{};
+    const auto eight = integral_constant<int, 512>{};
     if (n <= 256 && n_rows >= 4096 && k <= kMostByThreshold<16>) {
         if (n <= 64) return f(integral_constant<int, 4>{}, lanes);
         if (n <= 128) return f(integral_constant<int, 8>{}, lanes);
@@ -973,10 +978,44 @@ int with_layout(uint32_t n, uint64_t n_rows, uint32_t k, F&& f) {
         if (n <= 1024) return f(integral_constant<int, 16>{}, wave);
         return f(integral_constant<int, 32>{}, wave);
     }
-    if (n <= 1024) return f(integral_constant<int, 2>{}, waves);
-    if (n <= 4096) return f(integral_constant<int, 8>{}, waves);
-    if (n <= 8192) return f(integral_constant<int, 16>{}, waves);
-    return f(integral_constant<int, 32>{}, waves);
+    if (n <= 4096 && k <= kMostByThreshold<128>) {
+        if (n <= 1024) return f(integral_constant<int, 8>{}, two);
+        if (n <= 2048) return f(integral_constant<int, 16>{}, two);
+        return f(integral_constant<int, 32>{}, two);
+    }
+    if (n <= 8192 && k <= kMostByThreshold<256>) {
+        if (n <= 2048) return f(integral_constant<int, 8>{}, four);
+        if (n <= 4096) return f(integral_constant<int, 16>{}, four);
+        return f(integral_constant<int, 32>{}, four);
+    }
+    if (n <= 1024) return f(integral_constant<int, 2>{}, eight);
+    if (n <= 4096) return f(integral_constant<int, 8>{}, eight);
+    if (n <= 8192) return f(integral_constant<int, 16>{}, eight);
+    return f(integral_constant<int, 32>{}, eight);
+}
+// The same for the gradient, where k counts only because a thread takes two winners at most.  (Without a softmax over the whole row
+// nothing is held in registers.)
+template <typename F>
+int with_grad_layout(bool whole, uint32_t n, uint64_t n_rows, uint32_t k, F&& f) {
+    using std::integral_constant;
+    const auto go = [&](auto r, auto threads) { return whole ? f(r, threads, std::true_type{}) : f(integral_constant<int, 1>{}, threads, std::false_type{}); };
+    const auto lanes = integral_constant<int, 16>{};
+    const auto wave = integral_constant<int, 64>{};
+    if (n <= 256 && n_rows >= 4096 && k <= 32) {
+        if (n <= 64) return go(integral_constant<int, 4>{}, lanes);
+        if (n <= 128) return go(integral_constant<int, 8>{}, lanes);
+        return go(integral_constant<int, 16>{}, lanes);
+    }
+    if (n <= 2048 && k <= 128) {
+        if (n <= 64) return go(integral_constant<int, 1>{}, wave);
+        if (n <= 256) return go(integral_constant<int, 4>{}, wave);
+        if (n <= 512) return go(integral_constant<int, 8>{}, wave);
+        if (n <= 1024) return go(integral_constant<int, 16>{}, wave);
+        return go(integral_constant<int, 32>{}, wave);
+    }
+    if (n <= 4096 && k <= 256) return go(integral_constant<int, 32>{}, integral_constant<int, 128>{});
+    if (n <= 8192 && k <= 512) return go(integral_constant<int, 32>{}, integral_constant<int, 256>{});
+    return go(integral_constant<int, 32>{}, integral_constant<int, 512>{});
 }
 
 }  // namespace
@@ -1028,27 +1067,23 @@ int launch_winners_grad(const sdrb_dense& scores, const sdrb_winners_spec& spec,
     a.ld = scores.ld;
     a.out_ld = out.ld;
     a.n_ids = (uint32_t)scores.n_cols;
-    const bool whole = spec.score == SDRB_SCORE_SOFTMAX && !spec.renormalise;
-    return with_layout(a.n_ids, a.n_rows, spec.k, [&](auto r, auto n_threads) {
+    return with_grad_layout(spec.score == SDRB_SCORE_SOFTMAX && !spec.renormalise, a.n_ids, a.n_rows, spec.k, [&](auto r, auto n_threads, auto all) {
         constexpr int R = decltype(r)::value, THREADS = decltype(n_threads)::value;
+        constexpr bool WHOLE = decltype(all)::value;
         constexpr uint32_t kPerBlock = block_of(THREADS) / THREADS;
         return with_type(scores.type, [&](auto t) {
             return with_type(out.type, [&](auto o) {
                 using T = decltype(t);
                 using O = decltype(o);
-                const auto go = [&](auto all) {
-                    constexpr bool WHOLE = decltype(all)::value;
-                    return in_launches((scores.n_rows + kPerBlock - 1) / kPerBlock, block_of(THREADS), [&](uint64_t first, uint32_t blocks) {
-                        const uint64_t row = first * kPerBlock;
-                        a.n_rows = scores.n_rows - row;
-                        hipLaunchKernelGGL((k_winners_grad<R, THREADS, WHOLE, T, O>), dim3(blocks), dim3(block_of(THREADS)), 0, stream, a,
-                                           static_cast<const T*>(scores.data) + row * a.ld, ids + row * spec.k, grad_weights + row * spec.k,
-                                           static_cast<O*>(out.data) + row * a.out_ld);
-                        SDRB_HIP(hipGetLastError());
-                        return SDRB_OK;
-                    });
-                };
-                return whole ? go(std::true_type{}) : go(std::false_type{});
+                return in_launches((scores.n_rows + kPerBlock - 1) / kPerBlock, block_of(THREADS), [&](uint64_t first, uint32_t blocks) {
+                    const uint64_t row = first * kPerBlock;
+                    a.n_rows = scores.n_rows - row;
+                    hipLaunchKernelGGL((k_winners_grad<R, THREADS, WHOLE, T, O>), dim3(blocks), dim3(block_of(THREADS)), 0, stream, a,
+                                       static_cast<const T*>(scores.data) + row * a.ld, ids + row * spec.k, grad_weights + row * spec.k,
+                                       static_cast<O*>(out.data) + row * a.out_ld);
+                    SDRB_HIP(hipGetLastError());
+                    return SDRB_OK;
+                });
             });
         });
     });
