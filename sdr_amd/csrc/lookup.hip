@@ -7,11 +7,12 @@
 // addition, the load, and an fma a column.  Rows of src are read by buffer loads, which yield 0 beyond the matrix: an element
 // that contributes nothing has an offset there and a weight of 0, and needs no branch.  (Matrices beyond 2 GiB, or not aligned
 // to 4 bytes, are read by address.)
-// Short segments (tokens): whole waves, four slices at once, one element a turn: a copy, bound by HBM.
+// Short segments (tokens): whole waves, four slices at once, one element a turn: a copy, bound by HBM (16384 tokens of 4096 bf16
+// columns in 33-39 us: 245 MB read and written at 6.3 to 7.4 TB/s, some of it from the memory-side cache).
 // Long segments (codes): L = 16, two slices of 256 bytes a lane's turn, four elements in flight: bound by L2.  Each XCD (block
 // number modulo 8) works through slices of its own, one after another: 512 bytes of every row of a table are what its L2 has
 // to hold at a time, not the whole table.  Measured on 4096 rows of 328 of 16384 ids, 1024 bf16 columns (2.75 GB read):
-// 126 us = 22 TB/s; slices of 128 bytes 175 us, 256 bytes 138 us, one slice of 1 KiB for all XCDs 226 us.
+// 114 us = 24 TB/s; slices of 128 bytes 175 us, 256 bytes 128 us, one slice of 1 KiB for all XCDs 226 us.
 // S groups share a segment where there are too few of them to fill the chip, and join their sums in LDS.
 // A segment of more than `chunk` elements would keep its group busy long after the others: its elements are summed by groups
 // that own a chunk of the element list each (k_gather_chunks), and the segment's own group adds those sums up in order.
@@ -407,12 +408,13 @@ int launch_typed(const GatherSum& g, GatherArgs a, hipStream_t stream) {
 }  // namespace
 
 // The longest run of elements that one group of lanes sums by itself: long enough that few segments need a second step, short
-// enough that the longest does not outlast the rest.
+// enough that the longest does not outlast the rest; 4096 of them if that leaves 1024 elements or fewer, since all have to be looked
+// at (a million elements of 65536 ids, none of whose segments is long: 13 us, and 45 with chunks of 64).
 uint32_t segment_chunk(uint64_t n_segments, uint64_t n_elems, bool ragged) {
     if (n_segments == 0 || n_elems == 0) return 0;
     const uint64_t mean = n_elems / n_segments;
     uint32_t chunk = 64;
-    while ((chunk < 4 * mean && chunk < 1024) || n_elems > ((uint64_t)chunk << 22)) chunk *= 2;   // (one launch: 4 million at most)
+    while (((chunk < 4 * mean || n_elems > 4096ull * chunk) && chunk < 1024) || n_elems > ((uint64_t)chunk << 22)) chunk *= 2;   // (one launch: 4 million at most)
     return n_elems <= chunk || (!ragged && mean <= chunk) ? 0 : chunk;
 }
 // The same for runs of a sorted list, most of them of an element or two.  Words' frequencies make the longest run a sixteenth of
