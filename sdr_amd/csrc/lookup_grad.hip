@@ -22,6 +22,9 @@ namespace {
 // its time grows with them, since a block has one CU's issue.  More elements take three launches a pass: digits counted by tile, the
 // counts summed over tiles, and the elements sent to their places.  Digits have up to 12 bits there, so that ids below
 // 4096 -- the widths of sparse codes -- need one pass, and then the counts are the segments' starts too.
+// Measured: up to 1024 elements 6 us, 4096 14, 16384 42, in one block (bound by its issue: some 150 instructions a turn of 64);
+// 327680 elements of 2048 ids 4 us to count, 7 to sum and 14 to send; 1.3 million of 16384 ids, two passes, 7, 6 and 27, then 7, 6
+// and 54 (bound by stores of 4 bytes to lines of their own; loading further ahead changes nothing).
 
 struct SortArgs {
     const void* ids;
@@ -444,7 +447,8 @@ __global__ __launch_bounds__(256) void k_runs(const uint32_t* __restrict__ keys,
 // A wave takes 8 or 16 elements, a lane finding the row and the table row of each, and works through them B at a time: every lane
 // loads 16 bytes of the B table rows and of their gradients' row, column after column, and the B sums over the lanes are
 // formed together: in three steps eight values a lane become one value an eighth of the lanes, half of the values changing
-// sides each time.  Bound: instruction issue (16 of a table row's 16 bytes' conversions and products) and L2.
+// sides each time.  Bound: instruction issue (16 of a table row's 16 bytes' conversions and products) and L2.  Measured: 8192 rows of
+// 40 elements of 512 bf16 columns (336 MB of table rows read) in 22.5 us = 15 TB/s.
 // (On the matrix cores, as the diagonal of sixteen rows times sixteen rows, the same takes 48 us where this takes 23 (8192 x 40
 // dot products of 512 bf16): what a lane has to load there are 16 bytes of a row of its own, and L1 looks up a line for each.)
 
