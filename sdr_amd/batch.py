@@ -45,6 +45,16 @@ def _torch_stream(device: int, stream):
     return torch.cuda.ExternalStream(int(stream), device=device)
 
 
+def _empty(shape, dtype, device: int, stream):
+    """Device memory for a call on ``stream``: the allocator hands it on only to what follows on that stream, so a result that
+    is dropped while its call still runs is not another stream's yet."""
+    torch = _torch()
+    if stream is None:
+        return torch.empty(shape, dtype=dtype, device=f"cuda:{device}")
+    with torch.cuda.stream(_torch_stream(device, stream)):
+        return torch.empty(shape, dtype=dtype, device=f"cuda:{device}")
+
+
 def rows_to_csr(rows: Iterable, with_data: bool):
     """``rows``: iterable of id sequences, or of ``(ids, data)`` pairs when ``with_data``."""
     offsets = [0]
@@ -346,7 +356,7 @@ class SDRBatch:
         torch = _torch()
         unit = self.data_kind != DATA_EMPTY
         words = self.n_rows + 1 + self.nnz * (2 if unit else 1)
-        wire = torch.empty(words, dtype=torch.int32, device=f"cuda:{self.device}")
+        wire = _empty(words, torch.int32, self.device, stream)
         ids_t = wire[self.n_rows + 1: self.n_rows + 1 + self.nnz]
         data_t = wire[self.n_rows + 1 + self.nnz:]
         check(self._lib.sdrb_batch_export_device_csr(
@@ -422,7 +432,7 @@ class SDRBatch:
             raise ValueError("dtype must be torch.int32 (default), torch.uint8 or torch.int16 (uint16 values)")
         ld = (other.n_rows + 3) // 4 * 4
         if out is None:
-            out = torch.empty((max(self.n_rows, 1), max(ld, 4)), dtype=dtype, device=f"cuda:{other.device}")
+            out = _empty((max(self.n_rows, 1), max(ld, 4)), dtype, other.device, stream)
         if out.dtype != dtype or out.dim() != 2 or out.shape[0] < self.n_rows or out.stride(1) != 1 or out.stride(0) < other.n_rows:
             raise ValueError("out must be a [>=na, >=nb] tensor of the requested dtype with unit inner stride")
         check(self._lib.sdrb_size_op_narrow(self._h, other._h, op, FLAG_SWAP if swap else 0, out.data_ptr(), out.stride(0),
@@ -436,8 +446,7 @@ class SDRBatch:
                 raise ValueError("narrow counts come from the bit-sliced kernel only")
             return self._size_op_narrow(op, other, swap, out, stream, dtype)
         if out is None:
-            out = torch.empty((self.n_rows, other.n_rows), dtype=torch.int32,
-                              device=f"cuda:{other.device}")
+            out = _empty((self.n_rows, other.n_rows), torch.int32, other.device, stream)
         if out.dtype != torch.int32 or out.dim() != 2 or out.shape[0] < self.n_rows \
                 or out.shape[1] < other.n_rows or out.stride(1) != 1:
             raise ValueError("out must be an int32 [>=na, >=nb] tensor with unit inner stride")
@@ -462,7 +471,7 @@ class SDRBatch:
         torch = _torch()
         lo = np.ascontiguousarray(lo, dtype=np.int32)
         hi = np.ascontiguousarray(hi, dtype=np.int32)
-        out = torch.empty((max(lo.size, 1), max(self.n_rows, 1)), dtype=torch.int32, device=f"cuda:{self.device}")
+        out = _empty((max(lo.size, 1), max(self.n_rows, 1)), torch.int32, self.device, stream)
         check(self._lib.sdrb_range_size(self._h, lo.size, lo.ctypes.data, hi.ctypes.data, out.data_ptr(),
                                         out.stride(0), _stream_handle(self.device, stream)))
         return out[: lo.size, : self.n_rows]
@@ -470,18 +479,17 @@ class SDRBatch:
     def range_elems(self, lo, hi, *, stream=None) -> ElemResult:
         """CSR of ``self[j].ande(lo[r], hi[r])`` over the pairs (r, j) (SDR.hpp:881-929)."""
         torch = _torch()
-        dev = f"cuda:{self.device}"
         lo = np.ascontiguousarray(lo, dtype=np.int32)
         hi = np.ascontiguousarray(hi, dtype=np.int32)
         s = _stream_handle(self.device, stream)
         pairs = lo.size * self.n_rows
-        offsets = torch.empty(pairs + 1, dtype=torch.int32, device=dev)
+        offsets = _empty(pairs + 1, torch.int32, self.device, stream)
         total = C.c_uint64()
         check(self._lib.sdrb_range_elems_count(self._h, lo.size, lo.ctypes.data, hi.ctypes.data, offsets.data_ptr(),
                                                C.byref(total), s))
         n = int(total.value)
-        ids_buf = torch.empty(max(n, 1), dtype=torch.int32, device=dev)
-        data_buf = torch.empty(max(n, 1), dtype=torch.float32, device=dev) if self.data_kind != DATA_EMPTY else None
+        ids_buf = _empty(max(n, 1), torch.int32, self.device, stream)
+        data_buf = _empty(max(n, 1), torch.float32, self.device, stream) if self.data_kind != DATA_EMPTY else None
         check(self._lib.sdrb_range_elems_fill(self._h, lo.size, lo.ctypes.data, hi.ctypes.data, offsets.data_ptr(),
                                               ids_buf.data_ptr(),
                                               data_buf.data_ptr() if data_buf is not None else None, s))
@@ -492,7 +500,7 @@ class SDRBatch:
         (SDR.hpp:860-879); the payload of a hit is ``data[row_offsets[j] + position]``."""
         torch = _torch()
         ids = np.ascontiguousarray(ids, dtype=np.int32)
-        out = torch.empty((max(ids.size, 1), max(self.n_rows, 1)), dtype=torch.int32, device=f"cuda:{self.device}")
+        out = _empty((max(ids.size, 1), max(self.n_rows, 1)), torch.int32, self.device, stream)
         check(self._lib.sdrb_point_query(self._h, ids.size, ids.ctypes.data, out.data_ptr(), out.stride(0),
                                          _stream_handle(self.device, stream)))
         return out[: ids.size, : self.n_rows]
@@ -506,7 +514,7 @@ class SDRBatch:
         rows, ``row_major_mul_vec``."""
         torch = _torch()
         if out is None:
-            out = torch.empty((self.n_rows, other.n_rows), dtype=torch.float32, device=f"cuda:{other.device}")
+            out = _empty((self.n_rows, other.n_rows), torch.float32, other.device, stream)
         if out.dtype != torch.float32 or out.dim() != 2 or out.shape[0] < self.n_rows \
                 or out.shape[1] < other.n_rows or out.stride(1) != 1:
             raise ValueError("out must be a float32 [>=na, >=nb] tensor with unit inner stride")
@@ -569,9 +577,8 @@ class SDRBatch:
         when it applies, else matrix cores), ``"bitslice"`` or ``"mfma"``."""
         flags = {None: 0, "bitslice": FLAG_FORCE_BITSLICE, "mfma": FLAG_FORCE_MFMA}[algo]
         torch = _torch()
-        dev = f"cuda:{other.device}"
-        counts = torch.empty((max(self.n_rows, 1), k), dtype=torch.int32, device=dev)[: self.n_rows]
-        rows = torch.empty((max(self.n_rows, 1), k), dtype=torch.int32, device=dev)[: self.n_rows]
+        counts = _empty((max(self.n_rows, 1), k), torch.int32, other.device, stream)[: self.n_rows]
+        rows = _empty((max(self.n_rows, 1), k), torch.int32, other.device, stream)[: self.n_rows]
         check(self._lib.sdrb_allpairs_topk(self._h, other._h, k, exclude_offset, flags, counts.data_ptr(),
                                            rows.data_ptr(), _stream_handle(other.device, stream)))
         return counts, rows
@@ -596,12 +603,11 @@ class SDRBatch:
 
     def _elem_op(self, op: int, other: "SDRBatch", swap: bool, stream, algo, rowwise: bool = False) -> ElemResult:
         torch = _torch()
-        dev = f"cuda:{other.device}"
         if rowwise and self.n_rows != other.n_rows:
             raise ValueError("row-wise evaluation needs batches of equal length")
         pairs = other.n_rows if rowwise else self.n_rows * other.n_rows
         s = _stream_handle(other.device, stream)
-        offsets = torch.empty(pairs + 1, dtype=torch.int32, device=dev)
+        offsets = _empty(pairs + 1, torch.int32, other.device, stream)
         total = C.c_uint64()
         flags = self._flags(swap, algo, rowwise)
         this_kind = other.data_kind if swap else self.data_kind
@@ -622,10 +628,10 @@ class SDRBatch:
             has_data = this_kind != DATA_EMPTY
 
             def run(capacity):
-                off_t = torch.empty(pairs + 1, dtype=torch.int32, device=dev)
-                ids_t = torch.empty(max(capacity, 1), dtype=torch.int32, device=dev)
-                data_t = torch.empty(max(capacity, 1), dtype=torch.float32, device=dev) if has_data else None
-                tot_t = torch.empty(1, dtype=torch.int64, device=dev)
+                off_t = _empty(pairs + 1, torch.int32, other.device, stream)
+                ids_t = _empty(max(capacity, 1), torch.int32, other.device, stream)
+                data_t = _empty(max(capacity, 1), torch.float32, other.device, stream) if has_data else None
+                tot_t = _empty(1, torch.int64, other.device, stream)
                 check(self._lib.sdrb_ande_few(self._h, other._h, flags & FLAG_SWAP, off_t.data_ptr(), ids_t.data_ptr(),
                                               data_t.data_ptr() if data_t is not None else None, capacity,
                                               tot_t.data_ptr(), s))
@@ -653,9 +659,9 @@ class SDRBatch:
             check(self._lib.sdrb_elem_op_bound(self._h, other._h, op, flags, C.byref(bound)))
             cap = int(bound.value)
             if 0 < cap <= 0xFFFFFFFF and cap * (8 if this_kind != DATA_EMPTY else 4) <= self.SINGLE_CALL_BYTES:
-                ids_buf = torch.empty(cap, dtype=torch.int32, device=dev)
-                data_buf = torch.empty(cap, dtype=torch.float32, device=dev) if this_kind != DATA_EMPTY else None
-                total_dev = torch.empty(1, dtype=torch.int64, device=dev)
+                ids_buf = _empty(cap, torch.int32, other.device, stream)
+                data_buf = _empty(cap, torch.float32, other.device, stream) if this_kind != DATA_EMPTY else None
+                total_dev = _empty(1, torch.int64, other.device, stream)
                 check(self._lib.sdrb_elem_op(self._h, other._h, op, flags, offsets.data_ptr(), ids_buf.data_ptr(),
                                              data_buf.data_ptr() if data_buf is not None else None, cap,
                                              total_dev.data_ptr(), s))
@@ -666,8 +672,8 @@ class SDRBatch:
         n = int(total.value)
         # buffers keep at least one element so an empty result still has a valid pointer
         this_bits = other.id_bits if swap else self.id_bits      # a result holds ids of `this`'s width
-        ids_buf = torch.empty(max(n, 1), dtype=torch.int64 if this_bits == 64 else torch.int32, device=dev)
-        data_buf = torch.empty(max(n, 1), dtype=torch.float32, device=dev) if this_kind != DATA_EMPTY else None
+        ids_buf = _empty(max(n, 1), torch.int64 if this_bits == 64 else torch.int32, other.device, stream)
+        data_buf = _empty(max(n, 1), torch.float32, other.device, stream) if this_kind != DATA_EMPTY else None
         fill = self._lib.sdrb_elem_op_fill64 if this_bits == 64 else self._lib.sdrb_elem_op_fill
         check(fill(self._h, other._h, op, flags, offsets.data_ptr(),
                                           ids_buf.data_ptr(),
@@ -730,7 +736,7 @@ class SDRBatch:
         of equal length (int32 tensor [n])."""
         torch = _torch()
         op = {"ands": OP_AND, "ors": OP_OR, "xors": OP_XOR, "rms": OP_RM}[name]
-        out = torch.empty(max(other.n_rows, 1), dtype=torch.int32, device=f"cuda:{other.device}")
+        out = _empty(max(other.n_rows, 1), torch.int32, other.device, stream)
         check(self._lib.sdrb_size_op(self._h, other._h, op, self._flags(swap, None, True), out.data_ptr(),
                                      other.n_rows, _stream_handle(other.device, stream)))
         return out[: other.n_rows]
@@ -840,13 +846,12 @@ class SDRBatch:
         same ids in the same positions and, where both batches carry payloads, equal payloads.  ``rowwise``:
         ``out[j] = (self[j] == other[j])``."""
         torch = _torch()
-        dev = f"cuda:{other.device}"
         if rowwise:
             if self.n_rows != other.n_rows:
                 raise ValueError("row-wise evaluation needs batches of equal length")
-            out = torch.empty(max(other.n_rows, 1), dtype=torch.int32, device=dev)
+            out = _empty(max(other.n_rows, 1), torch.int32, other.device, stream)
         else:
-            out = torch.empty((max(self.n_rows, 1), max(other.n_rows, 1)), dtype=torch.int32, device=dev)
+            out = _empty((max(self.n_rows, 1), max(other.n_rows, 1)), torch.int32, other.device, stream)
         check(self._lib.sdrb_equal(self._h, other._h, FLAG_ROWWISE if rowwise else 0, out.data_ptr(),
                                    other.n_rows, _stream_handle(other.device, stream)))
         return out[: other.n_rows] if rowwise else out[: self.n_rows, : other.n_rows]
@@ -854,18 +859,17 @@ class SDRBatch:
     # -- batched visitors ------------------------------------------------------------------------
     def _visit(self, which: int, other: "SDRBatch", swap, stream, algo, rowwise) -> VisitResult:
         torch = _torch()
-        dev = f"cuda:{other.device}"
         if rowwise and self.n_rows != other.n_rows:
             raise ValueError("row-wise evaluation needs batches of equal length")
         pairs = other.n_rows if rowwise else self.n_rows * other.n_rows
         s = _stream_handle(other.device, stream)
         flags = self._flags(swap, algo, rowwise)
-        offsets = torch.empty(pairs + 1, dtype=torch.int32, device=dev)
+        offsets = _empty(pairs + 1, torch.int32, other.device, stream)
         total = C.c_uint64()
         check(self._lib.sdrb_visit_count(self._h, other._h, which, flags, offsets.data_ptr(), C.byref(total), s))
         n = int(total.value)
-        tp = torch.empty(max(n, 1), dtype=torch.int32, device=dev)
-        ap = torch.empty(max(n, 1), dtype=torch.int32, device=dev)
+        tp = _empty(max(n, 1), torch.int32, other.device, stream)
+        ap = _empty(max(n, 1), torch.int32, other.device, stream)
         check(self._lib.sdrb_visit_fill(self._h, other._h, which, flags, offsets.data_ptr(), tp.data_ptr(),
                                         ap.data_ptr(), s))
         return VisitResult(1 if rowwise else self.n_rows, other.n_rows, offsets, tp[:n], ap[:n], n)

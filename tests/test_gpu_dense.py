@@ -139,6 +139,8 @@ def test_more_threads_than_one_launch_takes():
     got = sdr_amd.lookup_grad_weights(ids, go, t)
     for r in (128 * blocks + ends, n - 1 - ends.abs()):
         plain.assert_sum(got[0, r].view(1, -1), *(x.view(1, -1) for x in plain.lookup_grad_weights(ids[:, r], go, t)), 8)
+    del got, ids
+    torch.cuda.empty_cache()   # (some 30 GB)
 
 
 def test_lookup_of_non_finite_values():
