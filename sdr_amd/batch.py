@@ -538,13 +538,15 @@ class SDRBatch:
 
     def lookup_grad_table(self, grad, n_table_rows=None, *, scale: float = 1.0, dtype=None, out=None, accumulate: bool = False,
                           stream=None):
-        """The gradient of :meth:`lookup` to its table (``n_table_rows``: by default the batch's declared width).  See
+        """The gradient of :meth:`lookup` to its table (``n_table_rows``: by default the rows of ``out``, or the batch's declared
+        width).  See
         :func:`sdr_amd.lookup_grad_table`."""
         from . import dense
         if n_table_rows is None and out is None and not self.width:
             raise ValueError("a batch without a declared width needs n_table_rows")
-        return dense._lookup_grad_table(self._lib, self._rows(), self.device, grad, self.width if n_table_rows is None else n_table_rows,
-                                        scale, dtype, out, accumulate, stream)
+        if n_table_rows is None and out is None:
+            n_table_rows = self.width
+        return dense._lookup_grad_table(self._lib, self._rows(), self.device, grad, n_table_rows, scale, dtype, out, accumulate, stream)
 
     def lookup_grad_data(self, grad, table, *, scale: float = 1.0, out=None, stream=None):
         """The gradient of :meth:`lookup` to the payloads: float32 ``[nnz]``, in element order.  See

@@ -559,6 +559,19 @@ def test_batches_take_the_same_operators():
         SDRBatch(0, 10).lookup(t)
 
 
+def test_a_batch_without_a_width_adds_to_the_rows_it_is_given():
+    from sdr_amd import SDRBatch
+    g = rng(9)
+    b = SDRBatch.from_rows([[1, 4], [], [0, 4, 6]])
+    go = matrix(g, 3, 24, F32)
+    want = b.lookup_grad_table(go, 9)
+    into = torch.ones(9, 24, device="cuda")
+    assert b.lookup_grad_table(go, out=into, accumulate=True) is into
+    plain.assert_sum(into, want.cpu().double() + 1, want.cpu().double().abs() + 1, torch.tensor(3.0))
+    with pytest.raises(ValueError):
+        b.lookup_grad_table(go)
+
+
 def test_winners_become_a_batch():
     import sdr_amd
     from sdr_amd import SDRBatch
