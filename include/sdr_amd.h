@@ -451,6 +451,7 @@ int sdrb_batch_rows(const sdrb_batch* batch, sdrb_rows* rows);
 /*
  * out[r, :] = scale * sum over the ids of row r, in their order, of weight * table[id, :]  (out: n_rows x table columns).
  * An embedding lookup where rows hold one id; a row without ids, or with none inside the table, yields zeros.
+ * Without row_offsets rows of up to 64 ids need no scratch.
  */
 int sdrb_lookup_scratch(const sdrb_rows* rows, uint64_t n_cols, size_t* bytes);
 int sdrb_lookup(int device, const sdrb_rows* rows, const sdrb_dense* table, float scale, const sdrb_dense* out, void* scratch,

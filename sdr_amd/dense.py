@@ -22,7 +22,6 @@ from .batch import _torch_stream
 
 _SCORES = {"softmax": 0, "sigmoid": 1}
 _types = {}
-_devices = []
 _raw_stream = None
 
 
@@ -32,7 +31,6 @@ def _torch():
         global _raw_stream
         # the current stream's handle without making a stream object, where this torch offers it
         _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", lambda device: torch.cuda.current_stream(device).cuda_stream)
-        _devices.extend(torch.device("cuda", k) for k in range(64))
         _types.update({torch.float32: 0, torch.float16: 1, torch.bfloat16: 2})
     return torch
 
@@ -84,27 +82,28 @@ def _rows(torch, ids, weights, offsets) -> Rows:
     return Rows(n, ids.numel(), off, ids.data_ptr(), w, 64 if wide else 32)
 
 
-def _empty(torch, shape, dtype, device, stream):
+def _empty(torch, shape, dtype, like, stream):
     if stream is None:
-        return torch.empty(shape, dtype=dtype, device=_devices[device])
-    with torch.cuda.stream(_torch_stream(device, stream)):   # memory that this stream may write at once
-        return torch.empty(shape, dtype=dtype, device=_devices[device])
+        return like.new_empty(shape, dtype=dtype)
+    with torch.cuda.stream(_torch_stream(like.get_device(), stream)):   # memory that this stream may write at once
+        return like.new_empty(shape, dtype=dtype)
 
 
-def _result(torch, out, n, m, dtype, device, stream):
+def _result(torch, out, n, m, dtype, like, stream):
     """(tensor, its description) of a result [n, m]: ``out``, or a new tensor"""
     if out is None:
-        out = _empty(torch, (n, m), dtype, device, stream)
-        if dtype not in _types:
+        code = _types.get(dtype)
+        if code is None:
             raise ValueError("results are float32, float16 or bfloat16")
-        return out, Dense(out.data_ptr(), n, m, m, _types[dtype])
+        out = _empty(torch, (n, m), dtype, like, stream)
+        return out, Dense(out.data_ptr(), n, m, m, code)
     if tuple(out.shape) != (n, m) or (dtype is not None and out.dtype != dtype):
         raise ValueError(f"out must have shape {(n, m)}" + ("" if dtype is None else f" and type {dtype}"))
-    return out, _matrix("out", out, device)
+    return out, _matrix("out", out, like.get_device())
 
 
-def _scratch(torch, size, device, stream):
-    return (None, 0, None) if size == 0 else (t := _empty(torch, size, torch.uint8, device, stream), size, t.data_ptr())
+def _scratch(torch, size, like, stream):
+    return (None, 0, None) if size == 0 else (t := _empty(torch, size, torch.uint8, like, stream), size, t.data_ptr())
 
 
 def _handle(device, stream) -> int:
@@ -114,10 +113,12 @@ def _handle(device, stream) -> int:
 def _lookup(lib, rows, device, table, scale, dtype, out, stream):
     torch = _torch()
     t = _matrix("table", table, device)
-    out, o = _result(torch, out, rows.n_rows, t.n_cols, dtype if out is not None else dtype or table.dtype, device, stream)
-    need = C.c_size_t()
-    check(lib.sdrb_lookup_scratch(rows, t.n_cols, need))
-    keep, size, at = _scratch(torch, need.value, device, stream)
+    out, o = _result(torch, out, rows.n_rows, t.n_cols, dtype if out is not None else dtype or table.dtype, table, stream)
+    keep, size, at = None, 0, None
+    if rows.row_offsets or rows.n_elems > 64 * rows.n_rows:   # (rows of equal length need none up to 64 ids)
+        need = C.c_size_t()
+        check(lib.sdrb_lookup_scratch(rows, t.n_cols, need))
+        keep, size, at = _scratch(torch, need.value, table, stream)
     check(lib.sdrb_lookup(device, rows, t, scale, o, at, size, _handle(device, stream)))
     return out
 
@@ -131,10 +132,10 @@ def _lookup_grad_table(lib, rows, device, grad, n_table_rows, scale, dtype, out,
         n_table_rows = out.shape[0]
     if n_table_rows < 0:
         raise ValueError("n_table_rows must not be negative")
-    out, o = _result(torch, out, n_table_rows, g.n_cols, dtype if out is not None else dtype or torch.float32, device, stream)
+    out, o = _result(torch, out, n_table_rows, g.n_cols, dtype if out is not None else dtype or torch.float32, grad, stream)
     need = C.c_size_t()
     check(lib.sdrb_lookup_grad_table_scratch(rows, n_table_rows, g.n_cols, need))
-    keep, size, at = _scratch(torch, need.value, device, stream)
+    keep, size, at = _scratch(torch, need.value, grad, stream)
     check(lib.sdrb_lookup_grad_table(device, rows, g, scale, int(accumulate), o, at, size, _handle(device, stream)))
     return out
 
@@ -143,7 +144,7 @@ def _lookup_grad_weights(lib, rows, device, grad, table, scale, shape, out, stre
     torch = _torch()
     g, t = _matrix("grad", grad, device), _matrix("table", table, device)
     if out is None:
-        out = _empty(torch, shape, torch.float32, device, stream)
+        out = _empty(torch, shape, torch.float32, grad, stream)
     check(lib.sdrb_lookup_grad_weights(device, rows, g, t, scale, _vector("out", out, torch.float32, device, torch.Size(shape)),
                                        _handle(device, stream)))
     return out
@@ -201,8 +202,8 @@ def winners(scores, k: int, *, score: str = "softmax", bias=None, groups: int = 
     if not 1 <= k <= s.n_cols:
         raise ValueError("k must be 1 .. ids")
     spec = _spec(torch, k, score, renormalise, scale, device, bias, groups, top_groups, group_top, s.n_cols)
-    ids = _empty(torch, (s.n_rows, k), torch.int32, device, stream)
-    weights = _empty(torch, (s.n_rows, k), torch.float32, device, stream)
+    ids = _empty(torch, (s.n_rows, k), torch.int32, scores, stream)
+    weights = _empty(torch, (s.n_rows, k), torch.float32, scores, stream)
     check(_lib.load().sdrb_winners(device, s, spec, ids.data_ptr(), weights.data_ptr(), _handle(device, stream)))
     return ids, weights
 
@@ -220,6 +221,6 @@ def winners_grad(scores, ids, grad_weights, *, score: str = "softmax", renormali
     i = _vector("ids", ids, torch.int32, device)
     g = _vector("grad_weights", grad_weights, torch.float32, device, ids.shape)
     spec = _spec(torch, ids.shape[1], score, renormalise, scale, device)
-    out, o = _result(torch, out, s.n_rows, s.n_cols, dtype if out is not None else dtype or scores.dtype, device, stream)
+    out, o = _result(torch, out, s.n_rows, s.n_cols, dtype if out is not None else dtype or scores.dtype, scores, stream)
     check(_lib.load().sdrb_winners_grad(device, s, spec, i, g, o, _handle(device, stream)))
     return out

@@ -122,3 +122,12 @@ def test_python_refuses_tensors_that_are_not_on_a_gpu():
                  lambda: sdr_amd.winners_grad(t, ids.view(1, 3), torch.zeros(1, 3))):
         with pytest.raises(ValueError):
             call()
+
+
+@pytest.mark.parametrize("k", [1, 2, 63, 64])
+def test_rows_of_up_to_64_ids_need_no_scratch(k):
+    """where they have equal lengths: calls with the ids of winners, or of tokens, rely on it"""
+    lib, n = _lib.load(), C.c_size_t(1)
+    for n_rows in (1, 3, 64, 65, 4096, 100_000, 60_000_000):
+        if n_rows * k < 2 ** 32:
+            assert lib.sdrb_lookup_scratch(rows(n_rows=n_rows, n_elems=n_rows * k), 2048, n) == 0 and n.value == 0
