@@ -89,7 +89,7 @@ int sdrb_lookup_scratch(const sdrb_rows* rows, uint64_t n_cols, size_t* bytes) {
     const char* what = "sdrb_lookup_scratch";
     if (const int rc = check_rows(what, rows)) return rc;
     if (!bytes || n_cols > kMaxCols) return refuse(SDRB_ERR_INVALID_ARG, what, "bytes is null or n_cols above 2^24");
-    *bytes = partial_bytes(segment_chunk(rows->n_rows, rows->n_elems, rows->row_offsets != nullptr), rows->n_elems, (uint32_t)n_cols);
+    *bytes = partial_bytes(segment_chunk(rows->n_rows, rows->n_elems, (uint32_t)n_cols, rows->row_offsets != nullptr), rows->n_elems, (uint32_t)n_cols);
     return SDRB_OK;
 }
 
@@ -103,7 +103,7 @@ int sdrb_lookup(int device, const sdrb_rows* rows, const sdrb_dense* table, floa
     if (out->n_rows != rows->n_rows || out->n_cols != table->n_cols)
         return refuse(SDRB_ERR_INVALID_ARG, what, "out must have a row for every row and the table's columns");
     if (out->n_rows == 0 || out->n_cols == 0) return SDRB_OK;
-    const uint32_t chunk = segment_chunk(rows->n_rows, rows->n_elems, rows->row_offsets != nullptr);
+    const uint32_t chunk = segment_chunk(rows->n_rows, rows->n_elems, (uint32_t)out->n_cols, rows->row_offsets != nullptr);
     const size_t need = partial_bytes(chunk, rows->n_elems, (uint32_t)out->n_cols);
     if (const int rc = check_scratch(what, need, scratch, scratch_bytes)) return rc;
     DeviceGuard guard(device);

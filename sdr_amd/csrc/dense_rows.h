@@ -166,7 +166,7 @@ struct GatherSum {
     float* partials;           // ... the first of which leaves its sums here: partial_bytes(...)
 };
 // A chunk for segments of any length, 0 where none can be longer.
-uint32_t segment_chunk(uint64_t n_segments, uint64_t n_elems, bool ragged);
+uint32_t segment_chunk(uint64_t n_segments, uint64_t n_elems, uint32_t dim, bool ragged);
 uint32_t run_chunk(uint64_t n_elems);
 inline size_t partial_bytes(uint32_t chunk, uint64_t n_elems, uint32_t dim) {
     return chunk ? (size_t)((n_elems + chunk - 1) / chunk) * 2 * dim * sizeof(float) : 0;

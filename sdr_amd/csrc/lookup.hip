@@ -381,11 +381,14 @@ int launch_rows(const GatherSum& g, GatherArgs a, uint64_t mean, hipStream_t str
     });
 }
 
+// elements to reckon with in a segment: without chunks one of ragged segments may hold them all
+uint64_t mean_of(const GatherSum& g) { return g.start && !g.chunk ? g.n_elems : g.n_elems / g.n_segments; }
+
 template <bool BUFFER, typename T, typename O>
 int launch_typed(const GatherSum& g, GatherArgs a, hipStream_t stream) {
     // long segments read more than they write: 16 bytes a load; short ones: 16 bytes at most a load or store
     constexpr int kWide = 16 / sizeof(T), kEven = 16 / (sizeof(T) > sizeof(O) ? sizeof(T) : sizeof(O));
-    const uint64_t mean = g.n_elems / g.n_segments;
+    const uint64_t mean = mean_of(g);
     if (a.chunk) {
         const int rc = a.dim >= 8u * kWide ? launch_chunks<kWide, 8, BUFFER, T>(g, a, stream) : launch_chunks<kWide, 0, BUFFER, T>(g, a, stream);
         if (rc != SDRB_OK) return rc;
@@ -410,9 +413,13 @@ int launch_typed(const GatherSum& g, GatherArgs a, hipStream_t stream) {
 // The longest run of elements that one group of lanes sums by itself: long enough that few segments need a second step, short
 // enough that the longest does not outlast the rest; 4096 of them if that leaves 1024 elements or fewer, since all have to be looked
 // at (a million elements of 65536 ids, none of whose segments is long: 13 us, and 45 with chunks of 64).
-uint32_t segment_chunk(uint64_t n_segments, uint64_t n_elems, bool ragged) {
+// None for a few thousand elements in few enough segments and columns that a whole block can share each: one launch, and no scratch.
+// (2000 elements in 200 rows of 512 columns 5.0 us against 6.4, 12.6 against 13.6 with all of them in one row; in 200 rows of 2048
+// columns 10.4 against 7.1, so not there.)
+uint32_t segment_chunk(uint64_t n_segments, uint64_t n_elems, uint32_t dim, bool ragged) {
     if (n_segments == 0 || n_elems == 0) return 0;
     const uint64_t mean = n_elems / n_segments;
+    if (mean >= 3 && n_elems <= 4096 && n_segments * dim <= 1u << 18) return 0;
     uint32_t chunk = 64;
     while (((chunk < 4 * mean || n_elems > 4096ull * chunk) && chunk < 1024) || n_elems > ((uint64_t)chunk << 22)) chunk *= 2;   // (one launch: 4 million at most)
     return n_elems <= chunk || (!ragged && mean <= chunk) ? 0 : chunk;
@@ -459,7 +466,7 @@ int launch_gather_sum(const GatherSum& g, hipStream_t stream) {
             if (a.dim < kWide) {   // narrower than a load: a column a lane
                 if (a.chunk)
                     if (const int rc = launch_chunks<1, 0, false, T>(g, a, stream)) return rc;
-                return launch_rows<1, 1, 0, 1, false, T, O>(g, a, g.n_elems / g.n_segments, stream);
+                return launch_rows<1, 1, 0, 1, false, T, O>(g, a, mean_of(g), stream);
             }
             if (bytes >= kNowhere || !by_words) return launch_typed<false, T, O>(g, a, stream);
             a.row_bytes = (uint32_t)(g.src_ld * sizeof(T));

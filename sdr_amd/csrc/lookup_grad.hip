@@ -606,7 +606,7 @@ struct Plan {
         // ids (two passes) 31 either way, 16384 44 against 31.  While a large result is cleared one block's time is hidden:
         // 16384 with 537 MB to clear 135 us against 160, with 134 MB 77 against 75.
         small = n <= 4096ull * p.count || (runs && n <= kSmall && n_keys * dim >= 1ull << 25);
-        chunk = runs ? run_chunk(n) : segment_chunk(n_keys, n, true);
+        chunk = runs ? run_chunk(n) : segment_chunk(n_keys, n, dim, true);
         sorted.row = reinterpret_cast<int32_t*>(take(n));
         sorted.weight = weighted ? reinterpret_cast<float*>(take(n)) : nullptr;
         sorted.row_at = take(small && ragged ? n : 0);
