@@ -162,10 +162,10 @@ struct GatherSum {
     uint64_t out_ld;
     float scale;
     bool accumulate;           // segments without elements are then left as they are
-    uint32_t chunk;            // segments longer than this are summed in two steps (0: there are none) ...
+    uint32_t chunk;            // segments longer than this are summed in two steps (0: all in one) ...
     float* partials;           // ... the first of which leaves its sums here: partial_bytes(...)
 };
-// A chunk for segments of any length, 0 where none can be longer.
+// A chunk for ragged segments or equal ones; 0: none is longer, or each is summed by a whole block.
 uint32_t segment_chunk(uint64_t n_segments, uint64_t n_elems, uint32_t dim, bool ragged);
 uint32_t run_chunk(uint64_t n_elems);
 inline size_t partial_bytes(uint32_t chunk, uint64_t n_elems, uint32_t dim) {

@@ -40,7 +40,7 @@ struct GatherArgs {
     float scale;
     uint32_t row_len;        // where start is null
     uint32_t dim;
-    uint32_t chunk;          // longer segments come from `partials` (0: there are none)
+    uint32_t chunk;          // longer segments come from `partials` (0: none does)
     uint32_t lanes_log2;     // L
     uint32_t split_log2;     // S
     uint32_t slices;         // of the columns
