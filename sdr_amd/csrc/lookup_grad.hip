@@ -280,7 +280,7 @@ struct PassArgs {
     uint32_t* counts;        // [tile][digit]
     uint32_t* totals;        // [digit]
     uint32_t shift, bits, turns, n_tiles;   // turns: of 64 elements a wave
-    uint32_t last, only;     // the only pass leaves out what contributes nothing: a key of n_keys needs no digit
+    uint32_t last, only;     // the only pass sends nothing that does not contribute (a key of n_keys needs no digit), and hands on its keys alone
     uint32_t* keys_out;
     uint32_t* elems_out;
     int32_t* row_out;        // in the last pass
@@ -338,7 +338,7 @@ template <int BITS>
 __global__ __launch_bounds__(256) void k_scatter(SortArgs a, PassArgs s) {
     constexpr uint32_t kDigits = 1u << BITS, kEach = (kDigits + 255) / 256;   // digits of a thread
     __shared__ uint32_t next[kTileWaves][kDigits];
-    __shared__ uint32_t sums[kEach * 4];
+    __shared__ uint32_t sums[kEach * 4 + 1];   // the last one: of all digits
     const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     uint32_t total[kEach], tiles_before[kEach];
 #pragma unroll
@@ -369,8 +369,13 @@ __global__ __launch_bounds__(256) void k_scatter(SortArgs a, PassArgs s) {
     if (wave == 0) {   // the sums of 64 digits each, at most 64 of them
         const uint32_t here = lane < kEach * 4 ? sums[lane] : 0u, sum = scan_lanes<64>(here);
         if (lane < kEach * 4) sums[lane] = sum - here;
+        if (lane == 63) sums[kEach * 4] = sum;
     }
     __syncthreads();
+    // The places behind what the only pass sends hold the key of what contributes nothing: a list that is searched for its runs has
+    // to be sorted to its end.  (All tiles write some of them; no row or weight is read there.)
+    if (s.only && s.keys_out)
+        for (uint64_t p = sums[kEach * 4] + (uint64_t)blockIdx.x * 256 + threadIdx.x; p < a.n; p += (uint64_t)gridDim.x * 256) s.keys_out[p] = (uint32_t)a.n_keys;
 #pragma unroll
     for (uint32_t i = 0; i < kEach; ++i) {
         const uint32_t d = i * 256 + threadIdx.x;
