@@ -625,9 +625,9 @@ struct Row {
             return placed();
         };
         // Where k approximate keys are no smaller than t, and fewer are larger, the winners are no smaller than t - off: the k-th
-        // may seem larger than it is, and another one smaller.  (Every key > -inf; an infinite t has become a NaN, and all are
-        // candidates.)
-        const auto off = [&](float t) { return SHARES ? 2.0f * slack + fabsf(t) * 0x1p-21f : 0.0f; };
+        // may seem larger than it is, and another one smaller.  (Every key > -inf.  A bias makes a key infinite, not its rounding: an
+        // infinite t is off by nothing.)
+        const auto off = [&](float t) { return SHARES && t < INFINITY ? 2.0f * slack + fabsf(t) * 0x1p-21f : 0.0f; };
         const auto lowered = [&](float t) { return fmaxf(SHARES ? t - off(t) : t, -3.402823466e38f); };
         if (w.k <= kMostByThreshold<THREADS> && team.template count_all<kTops>([&](int h) { return tops[h] > none; }) >= w.k) {
             uint32_t least = 0xFFFFFFFFu;
@@ -648,14 +648,15 @@ struct Row {
                 return team.template count_all<R>([&](int r) { return key[r] >= t; });
             });
             const float t = key_at(lo << kDrop);
-            // keys that are larger for sure, and those that may be the k-th
-            const uint32_t more = w.k - collect(SHARES ? t + off(t) : key_at((lo + 1) << kDrop));
+            // keys that are larger for sure -- none where the k-th is infinite -- and those that may be the k-th
+            const float larger = !(t < INFINITY) ? NAN : SHARES ? t + off(t) : key_at((lo + 1) << kDrop);
+            const uint32_t more = w.k - collect(larger);
             const uint32_t sure = bits;
             n = collect(lowered(t));
             if (n > (uint32_t)THREADS * kHeld) {
                 // too many may be the k-th: where they are equal, the lowest ids fill the places
                 bits &= ~sure;
-                if (SHARES && more && !alike(bits)) return false;
+                if (SHARES && more && t < INFINITY && !alike(bits)) return false;
                 placed();
                 uint32_t taken = sure;
 #pragma unroll
