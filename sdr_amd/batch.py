@@ -42,7 +42,9 @@ def _torch_stream(device: int, stream):
     torch = _torch()
     if stream is None or hasattr(stream, "cuda_stream"):
         return torch.cuda.current_stream(device) if stream is None else stream
-    return torch.cuda.ExternalStream(int(stream), device=device)
+    handle = int(stream)
+    # (0 is the default stream's handle; ExternalStream takes it for "none given" and returns some stream of a pool)
+    return torch.cuda.ExternalStream(handle, device=device) if handle else torch.cuda.default_stream(device)
 
 
 def _empty(shape, dtype, device: int, stream):

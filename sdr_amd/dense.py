@@ -18,7 +18,7 @@ import ctypes as C
 
 from . import _lib
 from ._lib import Dense, Rows, WinnersSpec, check
-from .batch import _torch_stream
+from .batch import _stream_handle, _torch_stream
 
 _SCORES = {"softmax": 0, "sigmoid": 1}
 _types = {}
@@ -107,7 +107,7 @@ def _scratch(torch, size, like, stream):
 
 
 def _handle(device, stream) -> int:
-    return _raw_stream(device) if stream is None else _torch_stream(device, stream).cuda_stream
+    return _raw_stream(device) if stream is None else _stream_handle(device, stream)
 
 
 def _lookup(lib, rows, device, table, scale, dtype, out, stream):
