@@ -40,9 +40,11 @@ def _stream_handle(device: int, stream) -> int:
 def _torch_stream(device: int, stream):
     """``stream`` (None: the current one) as torch knows it."""
     torch = _torch()
-    if stream is None or hasattr(stream, "cuda_stream"):
-        return torch.cuda.current_stream(device) if stream is None else stream
-    handle = int(stream)
+    if stream is None:
+        return torch.cuda.current_stream(device)
+    if isinstance(stream, torch.cuda.Stream):
+        return stream
+    handle = _stream_handle(device, stream)
     # (0 is the default stream's handle; ExternalStream takes it for "none given" and returns some stream of a pool)
     return torch.cuda.ExternalStream(handle, device=device) if handle else torch.cuda.default_stream(device)
 

@@ -34,3 +34,9 @@ def test_the_current_stream_other_handles_and_stream_objects(streams):
     assert batch._torch_stream(0, 1234).cuda_stream == 1234 and dense._handle(0, 1234) == 1234
     own = types.SimpleNamespace(cuda_stream=55)
     assert batch._torch_stream(0, own).cuda_stream == 55 and dense._handle(0, own) == 55
+
+
+def test_an_object_that_carries_a_handle_alone(streams):
+    """it is enough for the calls; torch gets a stream of its own kind for it"""
+    for handle, kind in ((55, "external"), (0, "default")):
+        assert batch._torch_stream(0, types.SimpleNamespace(cuda_stream=handle)).kind == kind
