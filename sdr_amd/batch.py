@@ -50,13 +50,19 @@ def _torch_stream(device: int, stream):
 
 
 def _empty(shape, dtype, device: int, stream):
-    """Device memory for a call on ``stream``: the allocator hands it on only to what follows on that stream, so a result that
-    is dropped while its call still runs is not another stream's yet."""
+    """Device memory for a call's result.  It belongs to the call's ``stream``: one that is dropped while the call still runs is
+    not another stream's yet.  And the stream that is current now, on which the caller goes on, is known to use it: one that is
+    dropped there is not handed to the call's stream before that work is done."""
     torch = _torch()
     if stream is None:
         return torch.empty(shape, dtype=dtype, device=f"cuda:{device}")
-    with torch.cuda.stream(_torch_stream(device, stream)):
+    here, there = torch.cuda.current_stream(device), _torch_stream(device, stream)
+    if here.cuda_stream == there.cuda_stream:
         return torch.empty(shape, dtype=dtype, device=f"cuda:{device}")
+    with torch.cuda.stream(there):
+        t = torch.empty(shape, dtype=dtype, device=f"cuda:{device}")
+    t.record_stream(here)
+    return t
 
 
 def rows_to_csr(rows: Iterable, with_data: bool):

@@ -9,8 +9,9 @@ Matrices are float32, float16 or bfloat16, with adjacent elements in a row and a
 rounded once to the output's type, in an order that the shapes and offsets fix: calls repeat bit for bit.
 
 Everything is enqueued on ``stream`` (a torch stream or a handle; the current stream of the tensors' device by default), outputs
-and scratch are allocated on that stream, and nothing waits for the GPU, so the calls can be captured into a graph.  All
-computation happens in ``libsdr_amd.so``; torch is used only to allocate and to name streams.
+and scratch are allocated on that stream, and nothing waits for the GPU, so the calls can be captured into a graph.  An output that
+is used on a further stream than ``stream`` and the current one needs torch's ``record_stream``.  All computation happens in
+``libsdr_amd.so``; torch is used only to allocate and to name streams.
 """
 from __future__ import annotations
 
@@ -18,7 +19,7 @@ import ctypes as C
 
 from . import _lib
 from ._lib import Dense, Rows, WinnersSpec, check
-from .batch import _stream_handle, _torch_stream
+from .batch import _empty as _batch_empty, _stream_handle, _torch_stream
 
 _SCORES = {"softmax": 0, "sigmoid": 1}
 _types = {}
@@ -83,10 +84,7 @@ def _rows(torch, ids, weights, offsets) -> Rows:
 
 
 def _empty(torch, shape, dtype, like, stream):
-    if stream is None:
-        return like.new_empty(shape, dtype=dtype)
-    with torch.cuda.stream(_torch_stream(like.get_device(), stream)):   # memory that this stream may write at once
-        return like.new_empty(shape, dtype=dtype)
+    return like.new_empty(shape, dtype=dtype) if stream is None else _batch_empty(shape, dtype, like.get_device(), stream)
 
 
 def _result(torch, out, n, m, dtype, like, stream):
@@ -103,7 +101,14 @@ def _result(torch, out, n, m, dtype, like, stream):
 
 
 def _scratch(torch, size, like, stream):
-    return (None, 0, None) if size == 0 else (t := _empty(torch, size, torch.uint8, like, stream), size, t.data_ptr())
+    if size == 0:
+        return None, 0, None
+    if stream is None:
+        t = like.new_empty(size, dtype=torch.uint8)
+    else:
+        with torch.cuda.stream(_torch_stream(like.get_device(), stream)):   # of this call alone: no other stream meets it
+            t = like.new_empty(size, dtype=torch.uint8)
+    return t, size, t.data_ptr()
 
 
 def _handle(device, stream) -> int:
