@@ -9,6 +9,7 @@ device-resident CSR batch and offers the same operation names over every pair
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 from dataclasses import dataclass
 from typing import Iterable, Optional, Sequence
@@ -47,6 +48,11 @@ def _torch_stream(device: int, stream):
     handle = _stream_handle(device, stream)
     # (0 is the default stream's handle; ExternalStream takes it for "none given" and returns some stream of a pool)
     return torch.cuda.ExternalStream(handle, device=device) if handle else torch.cuda.default_stream(device)
+
+
+def _on(device: int, stream):
+    """For torch's own steps inside a call on ``stream``: they run there, between the call's kernels, and so does their memory."""
+    return contextlib.nullcontext() if stream is None else _torch().cuda.stream(_torch_stream(device, stream))
 
 
 def _empty(shape, dtype, device: int, stream):
@@ -703,10 +709,12 @@ class SDRBatch:
         if op == OP_AND:
             # the bound of an intersection is loose: the exact total decides
             sizes = self._size_op(op, other, swap, None, stream, algo if algo in ("merge", "rowtable") else None)
-            per_row = sizes.to(torch.int64).sum(dim=1).cpu().numpy()
+            with _on(other.device, stream):
+                per_row = sizes.to(torch.int64).sum(dim=1).cpu().numpy()
             del sizes
         else:
-            a_off = self.to_wire(stream=stream)[: self.n_rows + 1].to(torch.int64).cpu().numpy() & 0xFFFFFFFF
+            with _on(self.device, stream):
+                a_off = self.to_wire(stream=stream)[: self.n_rows + 1].to(torch.int64).cpu().numpy() & 0xFFFFFFFF
             a_len = np.diff(a_off)
             if op == OP_RM:
                 per_row = a_len * other.n_rows if not swap else np.full(self.n_rows, other.nnz, dtype=np.int64)
@@ -730,13 +738,16 @@ class SDRBatch:
         off_t, ids_t = wire[: n + 1], wire[n + 1: n + 1 + nnz]
         data_t = wire[n + 1 + nnz:].view(torch.float32) if self.data_kind != DATA_EMPTY else None
         stats = self.stats()
-        off_host = off_t.to(torch.int64).cpu().numpy() & 0xFFFFFFFF
+        with _on(self.device, stream):
+            off_host = off_t.to(torch.int64).cpu().numpy() & 0xFFFFFFFF
         chunks = []
         for c in range(len(starts) - 1):
             i0, i1 = starts[c], starts[c + 1]
             lo, hi = int(off_host[i0]), int(off_host[i1])
             part = SDRBatch(self.device, self.width, self.data_kind)
-            part.adopt_device((off_t[i0: i1 + 1] - off_t[i0]).contiguous(), ids_t[lo:hi],
+            with _on(self.device, stream):
+                part_off = (off_t[i0: i1 + 1] - off_t[i0]).contiguous()
+            part.adopt_device(part_off, ids_t[lo:hi],
                               data_t[lo:hi] if data_t is not None else None, max_row_len=stats["max_row_len"],
                               min_id=stats["min_id"], max_id=stats["max_id"])
             chunks.append(part._elem_op(op, other, swap, stream, algo))
@@ -812,7 +823,8 @@ class SDRBatch:
 
         ``combine`` is the reference's ``rmi_combiner`` (SDR.hpp:304-310, 1447-1513) in batched form: it is called
         ONCE with the payloads of all common ids -- ``combine(this_values, arg_values)``, float32 device tensors
-        in row order, ascending ids within a row (``arg_values`` is None for an EmptyData argument) -- and returns
+        in row order, ascending ids within a row (``arg_values`` is None for an EmptyData argument), with the call's
+        stream as the current one -- and returns
         the new payloads of those elements of ``this``; an element whose new payload is not ``rm_relevant`` (below
         0.1 for UnitData, UnitData.hpp:22-28; never for ArithData, ArithData.hpp:22-28) is removed, every other
         element stays.  The default combiner is the payload type's own ``rmi``."""
@@ -822,6 +834,12 @@ class SDRBatch:
             raise ValueError("a combiner needs payloads on this batch (EmptyData has nothing to combine)")
         if self.id_bits != 32 or other.id_bits != 32:
             raise ValueError("rmi with a combiner serves batches with 32-bit ids")
+        with _on(self.device, stream):
+            self._combine(other, combine, stream)
+        self._refresh_info()
+        return self
+
+    def _combine(self, other, combine, stream) -> None:
         torch = _torch()
         hits = self.andv(other, rowwise=True, stream=stream)
         wire = self.to_wire(stream=stream)
@@ -850,8 +868,6 @@ class SDRBatch:
         new_off = kept_upto[off]
         new_off32 = torch.where(new_off >= 2 ** 31, new_off - 2 ** 32, new_off).to(torch.int32)
         self.upload_device(new_off32, ids[keep].contiguous(), data[keep].contiguous(), stream=stream)
-        self._refresh_info()
-        return self
 
     def equals(self, other: "SDRBatch", *, rowwise=False, stream=None):
         """``out[i, j] = (self[i] == other[j])`` as 0/1 (int32), the reference's ``operator==`` (SDR.hpp:470-483):
@@ -944,7 +960,9 @@ class SDRBatch:
         st = self.stats()
         v = SDRBatch(self.device, self.width, kind)
         if data_t is None and kind != "empty":
-            data_t = torch.ones(nnz, dtype=torch.float32, device=wire.device)
+            data_t = _empty(nnz, torch.float32, self.device, stream)
+            with _on(self.device, stream):
+                data_t.fill_(1)
         v.adopt_device(wire[: n + 1], wire[n + 1: n + 1 + nnz], data_t if kind != "empty" else None,
                        max_row_len=st["max_row_len"], min_id=st["min_id"], max_id=st["max_id"])
         return v
@@ -985,8 +1003,12 @@ class SDRBatch:
         if op == OP_AND:
             res = self._elem_op(op, other.ids_only(stream=stream), False, stream, algo)
             for c in (res.chunks if isinstance(res, ChunkedElemResult) else [res]):
+                if stream is not None:
+                    _torch().cuda.current_stream(other.device).wait_stream(_torch_stream(other.device, stream))
                 c.total     # settles the buffers first (an estimate-sized result may be computed again, with room)
-                c.data_buffer = _torch().ones_like(c.ids_buffer, dtype=_torch().float32)
+                c.data_buffer = _empty(c.ids_buffer.shape, _torch().float32, other.device, stream)
+                with _on(other.device, stream):
+                    c.data_buffer.fill_(1)
             return res
         return self.as_unit(stream=stream)._elem_op(OP_OR, other, False, stream, algo)
 
