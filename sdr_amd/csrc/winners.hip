@@ -310,8 +310,9 @@ __device__ __forceinline__ float sigmoid(float x) {
 __device__ __forceinline__ double exp64(double x) {
     x = fmin(fmax(x, -800.0), 800.0);
     const double n = rint(x * 1.44269504088896340736);
-    double r = fma(n, -6.93147180369123816490e-01, x);   // ln 2 in two parts, the first short enough that n times it is exact
-    r = fma(n, -1.90821492927058770002e-10, r);
+    // ln 2 in two parts: cut behind its 41st binary place, so that 11 bits of n times it are exact, and the rest rounded to binary64
+    double r = fma(n, -0x1.62e42fefa3p-1, x);
+    r = fma(n, -0x1.3de6af278ece6p-42, r);
     double p = 1.0 / 6227020800.0;
     p = fma(p, r, 1.0 / 479001600.0);
     p = fma(p, r, 1.0 / 39916800.0);
