@@ -577,7 +577,9 @@ class SDRBatch:
         torch = _torch()
         if ids.dim() != 2 or ids.dtype != torch.int32 or (weights is not None and weights.shape != ids.shape):
             raise ValueError("ids must be int32 [rows, k], and weights have their shape")
-        device = ids.device.index
+        device = ids.get_device()
+        if device < 0 or (weights is not None and weights.get_device() != device):
+            raise ValueError("ids and weights must be on one GPU")
         b = cls(device, width, kind if kind is not None else ("arith" if weights is not None else "empty"))
         with torch.cuda.stream(_torch_stream(device, stream)):
             there = ids >= 0
