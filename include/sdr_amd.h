@@ -422,7 +422,8 @@ int sdrb_visit_fill(const sdrb_batch* a, const sdrb_batch* b, int which, unsigne
  * gives the same bits.
  * None of these calls allocates, waits for the GPU or keeps anything: they can be captured into a graph.  Scratch is the
  * caller's (its size from sdrb_*_scratch, any 16-byte aligned device memory; NULL where the size is 0), and calls that may
- * run at the same time need scratch of their own.  An output may not overlap an input or the scratch.
+ * run at the same time need scratch of their own.  An output may not overlap an input or the scratch (one that
+ * begins where its input matrix does is refused).
  */
 #define SDRB_F32 0
 #define SDRB_F16 1

@@ -45,6 +45,14 @@ int check_dense(const char* what, const char* name, const sdrb_dense* m) {
     return SDRB_OK;
 }
 
+// An output over an input: rows are written while others are read.  (Matrices side by side in one buffer share its addresses, not
+// their first element.)
+int check_apart(const char* what, const char* name, const sdrb_dense* in, const sdrb_dense* out) {
+    if (in->data != out->data || in->n_rows * in->n_cols == 0 || out->n_rows * out->n_cols == 0) return SDRB_OK;
+    set_error("%s: out is %s itself", what, name);
+    return SDRB_ERR_INVALID_ARG;
+}
+
 int check_scratch(const char* what, size_t need, const void* scratch, size_t bytes) {
     if (need && (!scratch || bytes < need)) {
         set_error("%s: needs %zu bytes of scratch, got %zu", what, need, scratch ? bytes : (size_t)0);
@@ -102,6 +110,7 @@ int sdrb_lookup(int device, const sdrb_rows* rows, const sdrb_dense* table, floa
     if (const int rc = check_dense(what, "out", out)) return rc;
     if (out->n_rows != rows->n_rows || out->n_cols != table->n_cols)
         return refuse(SDRB_ERR_INVALID_ARG, what, "out must have a row for every row and the table's columns");
+    if (const int rc = check_apart(what, "table", table, out)) return rc;
     if (out->n_rows == 0 || out->n_cols == 0) return SDRB_OK;
     const uint32_t chunk = segment_chunk(rows->n_rows, rows->n_elems, (uint32_t)out->n_cols, rows->row_offsets != nullptr);
     const size_t need = partial_bytes(chunk, rows->n_elems, (uint32_t)out->n_cols);
@@ -147,6 +156,7 @@ int sdrb_lookup_grad_table(int device, const sdrb_rows* rows, const sdrb_dense* 
     if (const int rc = check_dense(what, "out", out)) return rc;
     if (grad->n_rows != rows->n_rows || grad->n_cols != out->n_cols)
         return refuse(SDRB_ERR_INVALID_ARG, what, "grad must have a row for every row and the columns of out");
+    if (const int rc = check_apart(what, "grad", grad, out)) return rc;
     if (out->n_rows == 0 || out->n_cols == 0) return SDRB_OK;
     const size_t need = table_grad_scratch_bytes(*rows, out->n_rows, (uint32_t)out->n_cols);
     if (const int rc = check_scratch(what, need, scratch, scratch_bytes)) return rc;
@@ -193,6 +203,7 @@ int sdrb_winners_grad(int device, const sdrb_dense* scores, const sdrb_winners_s
     if (const int rc = check_spec(what, spec, scores->n_cols)) return rc;
     if (out->n_rows != scores->n_rows || out->n_cols != scores->n_cols)
         return refuse(SDRB_ERR_INVALID_ARG, what, "out must have the shape of the scores");
+    if (const int rc = check_apart(what, "scores", scores, out)) return rc;
     if (scores->n_rows == 0) return SDRB_OK;
     if (!ids || !grad_weights) return refuse(SDRB_ERR_INVALID_ARG, what, "ids or grad_weights is null");
     DeviceGuard guard(device);

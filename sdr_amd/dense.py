@@ -6,7 +6,8 @@ Rows are given as tensors: ``ids`` [n] -- one id a row (the tokens of a sequence
 id outside the dense matrix (a padded place holds -1) contributes nothing.  ``weights`` are float32, one an id.
 
 Matrices are float32, float16 or bfloat16, with adjacent elements in a row and any row stride.  Sums are kept in binary32 and
-rounded once to the output's type, in an order that the shapes and offsets fix: calls repeat bit for bit.
+rounded once to the output's type, in an order that the shapes and offsets fix: calls repeat bit for bit.  ``out``, where it is
+given, may not overlap an input.
 
 Everything is enqueued on ``stream`` (a torch stream or a handle; the current stream of the tensors' device by default), outputs
 and scratch are allocated on that stream, and nothing waits for the GPU, so the calls can be captured into a graph.  An output that
