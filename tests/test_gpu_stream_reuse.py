@@ -50,7 +50,8 @@ def test_memory_waits_for_the_stream_that_was_current(name, by_handle):
     apart = storage.data_ptr() >= end or storage.data_ptr() + storage.nbytes() <= at
     assert apart or busy.query()      # (a call that waits for the device in between may have the same memory again)
     torch.cuda.synchronize()
-    assert torch.equal(seen, later)   # (the same call)
+    written = getattr(q, name)(q).total if name in ("ande", "rme") else seen.shape[0]   # (buffers sized by a bound hold anything behind)
+    assert torch.equal(seen[:written], later[:written])   # (the same call)
     del storage, later
 
 
