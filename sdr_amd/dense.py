@@ -20,7 +20,7 @@ import ctypes as C
 
 from . import _lib
 from ._lib import Dense, Rows, WinnersSpec, check
-from .batch import _empty as _batch_empty, _stream_handle, _torch_stream
+from .batch import _empty as _batch_empty, _stream_handle
 
 _SCORES = {"softmax": 0, "sigmoid": 1}
 _types = {}
@@ -104,11 +104,7 @@ def _result(torch, out, n, m, dtype, like, stream):
 def _scratch(torch, size, like, stream):
     if size == 0:
         return None, 0, None
-    if stream is None:
-        t = like.new_empty(size, dtype=torch.uint8)
-    else:
-        with torch.cuda.stream(_torch_stream(like.get_device(), stream)):   # of this call alone: no other stream meets it
-            t = like.new_empty(size, dtype=torch.uint8)
+    t = like.new_empty(size, dtype=torch.uint8) if stream is None else _batch_empty(size, torch.uint8, like.get_device(), stream, result=False)
     return t, size, t.data_ptr()
 
 
