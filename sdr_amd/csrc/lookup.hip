@@ -9,7 +9,8 @@
 // to 4 bytes, are read by address.)
 // Short segments (tokens): whole waves, four slices at once, one element a turn: a copy, bound by HBM (16384 tokens of 4096 bf16
 // columns in 33-39 us: 245 MB read and written at 6.3 to 7.4 TB/s, some of it from the memory-side cache).
-// Long segments (codes): L = 16, two slices of 256 bytes a lane's turn, four elements in flight: bound by L2.  Each XCD (block
+// Long segments (codes): L = 16, two slices of 256 bytes a lane's turn, four elements in flight: bound by L2, and by the issue of vector
+// instructions (84 % of the CUs' busy time below; 36 % for fp32 rows of 4004 bytes, which touch a third more lines).  Each XCD (block
 // number modulo 8) works through slices of its own, one after another: 512 bytes of every row of a table are what its L2 has
 // to hold at a time, not the whole table.  Measured on 4096 rows of 328 of 16384 ids, 1024 bf16 columns (2.75 GB read):
 // 114 us = 24 TB/s; slices of 128 bytes 175 us, 256 bytes 128 us, one slice of 1 KiB for all XCDs 226 us.

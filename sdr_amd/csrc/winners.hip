@@ -22,9 +22,10 @@
 // equal keys take the lowest ids; where more keys than the list holds lie within an error of the threshold, the row is bisected by
 // exact keys.  These are rolled loops that read the row anew: what runs rarely has to be short, since fetching instructions that no
 // other wave has run costs more than running them (straight-line code of 900 instructions: 15 us).
-// Bound: instruction issue, not memory: 8192 rows of 2048 bf16 scores, k = 40, in 14.6 us (34 MB read at 2.3 TB/s), 16384 rows of 256
-// in 8 groups, 4 of them taken, k = 8, in 14.8 to 18 us (17 MB), 4096 rows of 16384, k = 328, in 122 us (134 MB); a single row of
-// 256 in 4.9 us.  The gradients of 16384 rows of 128 and of 4099 rows of 2047 take 5.9 and 7.1 us (17 MB each).
+// Bound: instruction issue, not memory: 8192 rows of 2048 bf16 scores, k = 40, in 14.7 us (34 MB read at 2.3 TB/s; 620 vector instructions
+// a row, issued in 58 % of the CUs' busy time), 16384 rows of 256 in 8 groups, 4 of them taken, k = 8, in 15 to 18 us (17 MB; 320 a row, 74 %),
+// 4096 rows of 16384, k = 328, in 124 us (134 MB); a single row of 256 in 4.9 us.  The gradients of 16384 rows of 128 and of 4099 rows of
+// 2047 take 5.9 and 6.9 us (17 MB each).
 #include <type_traits>
 
 #include "dense_rows.h"

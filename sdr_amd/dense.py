@@ -7,7 +7,8 @@ id outside the dense matrix (a padded place holds -1) contributes nothing.  ``we
 
 Matrices are float32, float16 or bfloat16, with adjacent elements in a row and any row stride.  Sums are kept in binary32 and
 rounded once to the output's type, in an order that the shapes and offsets fix: calls repeat bit for bit.  ``out``, where it is
-given, may not overlap an input.
+given, may not overlap an input.  None of the functions is an autograd operator: a result carries no gradient function, whatever the
+inputs require; a training step calls the gradients itself.
 
 Everything is enqueued on ``stream`` (a torch stream or a handle; the current stream of the tensors' device by default), outputs
 and scratch are allocated on that stream, and nothing waits for the GPU, so the calls can be captured into a graph.  An output that
